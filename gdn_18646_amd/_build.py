@@ -22,7 +22,10 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libgdn_amd.so")
 EXT = os.path.join(PKG, "_gdn_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
 
-HIP_SOURCES = ["abi.cpp", "decode.hip", "prefill.hip", "rmsnorm.hip", "proj.hip", "proj_packed.hip", "proj_plain.hip", "layer.hip"]
+HIP_SOURCES = ["abi.cpp", "decode.hip", "prefill.hip", "rmsnorm.hip", "proj.hip", "proj_packed.hip", "proj_plain.hip", "layer.hip",
+               "block_norm.hip", "block_norm_bwd.hip", "fp8_quantize.hip", "fp8_matmul.hip", "fp8_mm_e4m3_e4m3.hip",
+               "fp8_mm_e4m3_e5m2.hip", "fp8_mm_e5m2_e4m3.hip", "fp8_mm_e5m2_e5m2.hip"]
+BINDING_SOURCES = ["bindings.cpp", "bindings_block.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # Packed-FP32 VALU forms are disabled on purpose (some give wrong results on
 # the target boxes); the host pass warns that it does not know the feature.
@@ -75,7 +78,7 @@ def build_binding():
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_gdn_ext",
         "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         *[f"-I{p}" for p in incs],
-        os.path.join(CSRC, "bindings.cpp"),
+        *[os.path.join(CSRC, s) for s in BINDING_SOURCES],
         "-o", tmp,
         f"-L{PKG}", "-lgdn_amd",
         f"-L{os.path.join(tdir, 'lib')}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip",

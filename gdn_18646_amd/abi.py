@@ -51,6 +51,13 @@ SIGNATURES = {
     "gdn_out_proj_fits": (_I, [_I64, _I64, _I64]),
     "gdn_out_proj_hip": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "gdn_layer_decode_step_hip": (_I, [_P, _P, _F] + [_P] * 10 + [_F] + [_P] * 8 + [_I] * 6 + [_P]),
+    "gdn_block_norm_hip": (_I, [_P, _I64] * 3 + [_I64] + [_P] * 3 + [_F, _I, _F] + [_P, _I64] * 4 + [_P, _P]
+                           + [_I64] * 2 + [_I] * 3 + [_P]),
+    "gdn_block_norm_bwd_workspace_bytes": (_SZ, [_I64] * 3),
+    "gdn_block_norm_bwd_hip": (_I, [_P, _I64] * 5 + [_I64] + [_P] * 3 + [_F, _I] + [_P] * 8 + [_I64] * 2 + [_I] * 3
+                               + [_P, _SZ, _P]),
+    "gdn_fp8_quantize_hip": (_I, [_P, _I64, _I, _I64, _I64, _I, _I] + [_P, _I64] * 4 + [_P]),
+    "gdn_fp8_matmul_hip": (_I, [_P, _I64, _I, _P, _I64] * 2 + [_I, _I, _P, _I64, _I] + [_I64] * 3 + [_P]),
 }
 
 STATUS = {0: "GDN_OK", 1: "GDN_ERR_INVALID_ARGUMENT", 2: "GDN_ERR_UNSUPPORTED",

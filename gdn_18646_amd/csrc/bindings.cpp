@@ -19,6 +19,8 @@
 
 #include "../../include/gdn_amd.h"
 
+void bind_block_ops(pybind11::module_& rmsnorm, pybind11::module_& proj);  // bindings_block.cpp
+
 namespace {
 
 using at::Tensor;
@@ -624,4 +626,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     auto mj = m.def_submodule("proj", "Projection + causal conv + SiLU");
     mj.def("forward", &proj_forward, "Fused linear projection + causal depthwise conv1d + SiLU (bf16)",
            py::arg("input"), py::arg("weight"), py::arg("conv_w"));
+    bind_block_ops(mr, mj);
 }

@@ -1,0 +1,169 @@
+// The norms before and after a block, fused with its gate and residual:
+//   u = y rstd_y post_gamma            rstd_y = (mean(y^2) + eps)^-1/2   (u = y without post_gamma)
+//   h = residual + rs scale act(gate) u                                  (factors that are absent are 1)
+//   n = h rstd_h gamma                 rstd_h = (mean(h^2) + eps)^-1/2
+// in fp32; h and n are rounded once, where they are written (n follows from the
+// unrounded h), and n (h without gamma) may go out as e4m3 codes of 128 with
+// their scales instead, what a block-scaled product reads.
+//
+// What bounds it: HBM for many rows (each input read once, each output written
+// once, two row sums between them that never leave the registers), the one
+// chain of loads, sums and stores for a few.
+#include "block_norm.hpp"
+#include "fp8_blocks.hpp"
+
+namespace {
+
+template <class TY, class TR, class TP, int LPR, int NV, bool VEC>
+__global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(NormParams p) {
+    constexpr int SLOTS = LPR <= 64 ? 256 / LPR : 1;
+    __shared__ float sums[2][LPR > 64 ? LPR / 64 : 1];
+    const int tid = threadIdx.x, lane = tid % LPR;
+    const int row = static_cast<int>(blockIdx.x) * SLOTS + tid / LPR;
+    const bool live = row < p.R;
+    const long long r = live ? row : p.R - 1;  // rows past the end repeat the last one and write nothing
+    const int D = p.D;
+
+    Oct<TY> yr[NV], gr[NV];
+    Oct<TR> rr[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) yr[u] = Oct<TY>::template load<VEC>(p.y, r * p.ldy, 8 * (lane + LPR * u), D);
+    if (p.residual) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) rr[u] = Oct<TR>::template load<VEC>(p.residual, r * p.ldr, 8 * (lane + LPR * u), D);
+    }
+    if (p.gate) {
+        const long long g = static_cast<unsigned>(r) / p.rows_per_gate;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) gr[u] = Oct<TY>::template load<VEC>(p.gate, g * p.ldg, 8 * (lane + LPR * u), D);
+    }
+    auto inside = [&](int u, int e) { return VEC ? 8 * (lane + LPR * u) < D : 8 * (lane + LPR * u) + e < D; };
+
+    float h[NV][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        yr[u].get(h[u]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[u][e] = inside(u, e) ? h[u][e] : 0.f;
+            ss = fmaf(h[u][e], h[u][e], ss);
+        }
+    }
+    float f0 = p.rs;
+    if (p.post_gamma) {
+        const float inv = 1.f / sqrtf(row_sum<LPR>(ss, sums[0]) / static_cast<float>(D) + p.eps);
+        if (p.rstd_y && live && lane == 0) p.rstd_y[row] = inv;
+        f0 *= inv;
+    }
+    ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        float f[8], t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = f0;
+        const int c = 8 * (lane + LPR * u);
+        if (p.post_gamma) {
+            Oct<TP>::template load<VEC>(p.post_gamma, 0, c, D).get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= t[e];
+        }
+        if (p.scale) {
+            Oct<TP>::template load<VEC>(p.scale, 0, c, D).get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= t[e];
+        }
+        if (p.gate) {
+            gr[u].get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= act_f(t[e], p.act);
+        }
+        if (p.residual) {
+            rr[u].get(t);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[u][e] = inside(u, e) ? fmaf(f[e], h[u][e], t[e]) : 0.f;
+            ss = fmaf(h[u][e], h[u][e], ss);
+        }
+        if (p.h && live) store8<TR, VEC>(p.h, r * p.ldh, c, D, h[u]);
+    }
+    if (!p.n && !p.codes && !p.rstd_h) return;
+    float inv = 1.f;
+    if (p.gamma) {
+        inv = 1.f / sqrtf(row_sum<LPR>(ss, sums[1]) / static_cast<float>(D) + p.eps);
+        if (p.rstd_h && live && lane == 0) p.rstd_h[row] = inv;
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int c = 8 * (lane + LPR * u);
+        if (p.gamma) {
+            float t[8];
+            Oct<TP>::template load<VEC>(p.gamma, 0, c, D).get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[u][e] = inside(u, e) ? h[u][e] * inv * t[e] : 0.f;
+        }
+        if (p.n && live) store8<TY, VEC>(p.n, r * p.ldn, c, D, h[u]);
+        if (p.codes) {
+            const uint32_t s = Fp8<GDN_E4M3>::scale_byte(max16(amax8(h[u])));
+            const u32x2 w = Fp8<GDN_E4M3>::codes8(h[u], Fp8<GDN_E4M3>::inverse(s), s == 0xffu);
+            if (live && c / kBlk * kBlk < D) {  // a ragged last block is filled up with zero codes
+                *reinterpret_cast<u32x2*>(p.codes + r * p.ldc + c) = w;
+                if ((lane & 15) == 0) p.scales[static_cast<long long>(c / kBlk) * p.lds + row] = static_cast<uint8_t>(s);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residual, int64_t ldr, const void* gate,
+                                  int64_t ldg, int64_t rows_per_gate, const void* post_gamma, const void* gamma,
+                                  const void* scale, float residual_scale, int act, float eps, void* h, int64_t ldh,
+                                  void* n, int64_t ldn, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds,
+                                  float* rstd_y, float* rstd_h, int64_t R, int64_t D, int type_y, int type_r, int type_p,
+                                  void* stream) {
+    using gdn_host::aligned;
+    using gdn_host::fail;
+    if (R < 0 || D <= 0) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: R=%lld D=%lld", (long long)R, (long long)D);
+    if (D > kMostColumns || R > 0x7fffffffLL)
+        return fail(GDN_ERR_UNSUPPORTED, "block_norm: R=%lld D=%lld, at most 2^31 - 1 rows of %d", (long long)R, (long long)D, kMostColumns);
+    if (!types_ok(type_y, type_r, type_p))
+        return fail(GDN_ERR_UNSUPPORTED, "block_norm: types %d, %d, %d of y, residual and parameters", type_y, type_r, type_p);
+    if (act < GDN_ACT_NONE || act > GDN_ACT_TANH) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: act=%d", act);
+    if (!y || (!h && !n && !codes)) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: y or every output is null");
+    if (!gamma && (n || rstd_h)) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: n and rstd_h need gamma");
+    if (!post_gamma && rstd_y) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rstd_y needs post_gamma");
+    if (gate && rows_per_gate <= 0) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rows_per_gate=%lld", (long long)rows_per_gate);
+    if (codes && (!scales || !aligned(codes, 16) || ldc % 16 != 0 || ldc < (D + kBlk - 1) / kBlk * kBlk || lds < R))
+        return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: codes need scales [D / 128, >= R], 16-byte alignment and rows padded to 128");
+    const size_t by = type_bytes(type_y), br = type_bytes(type_r), bp = type_bytes(type_p);
+    if (!aligned(y, by) || !aligned(residual, br) || !aligned(gate, by) || !aligned(h, br) || !aligned(n, by) ||
+        !aligned(post_gamma, bp) || !aligned(gamma, bp) || !aligned(scale, bp))
+        return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: a buffer is not aligned to its elements");
+    if (R == 0) return GDN_OK;
+    const bool vec = D % 8 == 0 && vec_rows(y, ldy, type_y) && vec_rows(residual, ldr, type_r) && vec_rows(gate, ldg, type_y) &&
+                     vec_rows(h, ldh, type_r) && vec_rows(n, ldn, type_y) && vec_rows(post_gamma, 0, type_p) &&
+                     vec_rows(gamma, 0, type_p) && vec_rows(scale, 0, type_p);
+    NormParams p = {};
+    p.y = y, p.residual = residual, p.gate = gate, p.post_gamma = post_gamma, p.gamma = gamma, p.scale = scale;
+    p.ldy = ldy, p.ldr = ldr, p.ldg = ldg;
+    p.rows_per_gate = static_cast<unsigned>(rows_per_gate < R ? rows_per_gate : R);
+    p.rs = residual_scale, p.eps = eps, p.act = gate ? act : GDN_ACT_NONE;
+    p.h = h, p.n = n, p.ldh = ldh, p.ldn = ldn;
+    p.codes = codes, p.scales = scales, p.ldc = ldc, p.lds = lds;
+    p.rstd_y = rstd_y, p.rstd_h = rstd_h;
+    p.R = static_cast<int>(R), p.D = static_cast<int>(D);
+    return with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
+        return with_row_shape(p.D, vec, [&](auto lpr, auto nv, auto v) {
+            constexpr int LPR = decltype(lpr)::value, slots = LPR <= 64 ? 256 / LPR : 1;
+            const dim3 grid((p.R + slots - 1) / slots), block(LPR <= 64 ? 256 : LPR);
+            hipLaunchKernelGGL((gdn_block_norm_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
+                               grid, block, 0, static_cast<hipStream_t>(stream), p);
+            return gdn_host::check_launch("gdn_block_norm_kernel");
+        });
+    });
+}

@@ -1,0 +1,128 @@
+// Entry point of the fp8 block-scaled product, and its kernel for a few tokens.
+//
+// gdn_fp8_few_kernel (up to 16 tokens, one decode step): what counts is the
+// weights' bytes.  A workgroup of 8 waves owns 16 columns; each wave takes every
+// eighth block of K straight from memory into MFMA fragments (no LDS: nothing is
+// used twice), and the waves' sums meet in LDS.
+#include "fp8_matmul.hpp"
+
+namespace {
+
+constexpr int kFewWaves = 8;
+
+template <int FA, int FB, bool OUT32>
+__global__ __launch_bounds__(64 * kFewWaves) void gdn_fp8_few_kernel(gdn_fp8::MatmulParams p, int scales) {
+    __shared__ f32x4 sums[kFewWaves][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g4 = lane >> 4;
+    const int n0 = blockIdx.x * 16, nslices = p.K / 128;
+    const int row = min(n0 + r16, p.N - 1), tok = min(r16, p.M - 1);
+    const uint8_t* const w = p.b + static_cast<size_t>(row) * p.ldb + 16 * g4;
+    const uint8_t* const x = p.a + static_cast<size_t>(tok) * p.lda + 16 * g4;
+    const bool rows = scales == gdn_fp8::kE8Row || scales == gdn_fp8::kF32Row;
+    const bool f32 = scales == gdn_fp8::kF32Block || scales == gdn_fp8::kF32Row;
+    // e8m0: the lane's row of b; fp32: the four columns of its accumulator
+    const size_t sstep = rows ? p.ldb_s : 1;
+    const uint8_t* const s8 = static_cast<const uint8_t*>(p.b_scale) + (rows ? row : static_cast<size_t>(row / 128) * p.ldb_s);
+    size_t s4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = min(n0 + 4 * g4 + i, p.N - 1);
+        s4[i] = rows ? c : static_cast<size_t>(c / 128) * p.ldb_s;
+    }
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int kb = wave; kb < nslices; kb += kFewWaves) {
+        const u32x4* const wp = reinterpret_cast<const u32x4*>(w + static_cast<size_t>(kb) * 128);
+        const u32x4* const xp = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(kb) * 128);
+        const int sx = p.a_scale[kb * p.lda_s + tok];
+        const int sw = f32 ? 127 : s8[kb * sstep];
+        const i32x8 wc = join(wp[0], wp[4]), xc = join(xp[0], xp[4]);
+        f32x4 t = f32 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
+        if constexpr (OUT32) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                t = mfma16x16x32(codes_to_bf16<FB>(wc[2 * q], wc[2 * q + 1], sw), codes_to_bf16<FA>(xc[2 * q], xc[2 * q + 1], sx), t);
+        } else {
+            t = mfma_fp8<FB, FA, 0, 0>(wc, xc, t, sw, sx);
+        }
+        if (f32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(static_cast<const float*>(p.b_scale)[s4[i] + kb * sstep], t[i], acc[i]);
+        } else {
+            acc = t;
+        }
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 1; i < kFewWaves; ++i) acc += sums[i][lane];
+    if (r16 < p.M && n0 + 4 * g4 < p.N) store4<OUT32>(p, r16, n0 + 4 * g4, acc);
+}
+
+long long tiles(const gdn_fp8::MatmulParams& p, int cols, int toks) {
+    return static_cast<long long>((p.M + toks - 1) / toks) * ((p.N + cols - 1) / cols);
+}
+
+int choose_tile(const gdn_fp8::MatmulParams& p) {
+    constexpr long long kCUs = 256;
+    if (tiles(p, 32, 32) <= kCUs) return gdn_fp8::k32x32;
+    if (tiles(p, 64, 64) <= 2 * kCUs) return gdn_fp8::k64x64;
+    if (tiles(p, 128, 128) <= 2 * kCUs) return gdn_fp8::k128x128;
+    return gdn_fp8::k256x256;
+}
+
+template <int FA, int FB>
+int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t stream) {
+    if (p.M <= 16) {
+        const dim3 grid((p.N + 15) / 16), block(64 * kFewWaves);
+        if (f32)
+            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, true>), grid, block, 0, stream, p, scales);
+        else
+            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, false>), grid, block, 0, stream, p, scales);
+        return gdn_host::check_launch("gdn_fp8_few_kernel");
+    }
+    return gdn_fp8::launch_tile<FA, FB>(choose_tile(p), scales, f32, p, stream);
+}
+
+}  // namespace
+
+extern "C" int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_t* a_scale, int64_t lda_s,
+                                  const uint8_t* b, int64_t ldb, int format_b, const void* b_scale, int64_t ldb_s,
+                                  int b_block_rows, int type_b_scale, void* out, int64_t ldo, int type_out, int64_t M,
+                                  int64_t N, int64_t K, void* stream) {
+    using gdn_host::aligned;
+    using gdn_host::fail;
+    if (M < 0 || N < 0 || K <= 0) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+    if (K % 128 != 0) return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: K=%lld must be a multiple of 128 (pad with zero codes)", (long long)K);
+    if ((format_a != GDN_E4M3 && format_a != GDN_E5M2) || (format_b != GDN_E4M3 && format_b != GDN_E5M2))
+        return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: formats %d, %d", format_a, format_b);
+    if (b_block_rows != 1 && b_block_rows != 128) return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: b's blocks of %d x 128, 1 or 128 rows are supported", b_block_rows);
+    if (type_b_scale != GDN_E8M0 && type_b_scale != GDN_F32) return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: type %d of b's scales", type_b_scale);
+    if (type_out != GDN_BF16 && type_out != GDN_F32) return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: type %d of out", type_out);
+    // 32-bit copy offsets within a tile, 32-bit tile numbers
+    constexpr int64_t kMost = int64_t{1} << 22, kRows = 0x7fffff00LL;
+    if (lda > kMost || ldb > kMost || M > kRows || N > kRows || (M + 31) / 32 * ((N + 31) / 32) > 0x7fffffffLL)
+        return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: problem too large (rows of at most 2^22 codes)");
+    if (M == 0 || N == 0) return GDN_OK;
+    if (!a || !a_scale || !b || !b_scale || !out) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: null pointer argument");
+    if (!aligned(a, 16) || !aligned(b, 16) || lda % 16 != 0 || ldb % 16 != 0 || lda < K || ldb < K)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: codes need 16-byte aligned rows of at least K");
+    if (!aligned(a_scale, 16) || lda_s % 16 != 0 || lda_s < M)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: a's scales [K / 128, lda_s] need 16-byte aligned rows of at least M");
+    const size_t bs = type_b_scale == GDN_F32 ? 4 : 1, bo = type_out == GDN_F32 ? 4 : 2;
+    if (b_block_rows == 1 ? !aligned(b_scale, 16) || ldb_s % 16 != 0 || ldb_s < N : !aligned(b_scale, bs) || ldb_s < K / 128)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: b's scales: rows of at least N, 16-byte aligned ([K / 128, ldb_s]), or of K / 128 (128 x 128 blocks)");
+    if (!aligned(out, bo) || ldo < N) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: out unaligned or ldo < N");
+    gdn_fp8::MatmulParams p = {};
+    p.a = a, p.b = b, p.a_scale = a_scale, p.b_scale = b_scale, p.out = out;
+    p.lda = lda, p.ldb = ldb, p.lda_s = lda_s, p.ldb_s = ldb_s, p.ldo = ldo;
+    p.M = static_cast<int>(M), p.N = static_cast<int>(N), p.K = static_cast<int>(K);
+    p.wide = aligned(out, 16) && ldo * static_cast<int64_t>(bo) % 16 == 0;
+    const int scales = type_b_scale == GDN_F32 ? (b_block_rows == 1 ? gdn_fp8::kF32Row : gdn_fp8::kF32Block)
+                                               : (b_block_rows == 1 ? gdn_fp8::kE8Row : gdn_fp8::kE8Block);
+    const auto s = static_cast<hipStream_t>(stream);
+    if (format_a == GDN_E4M3) return format_b == GDN_E4M3 ? launch<GDN_E4M3, GDN_E4M3>(p, scales, type_out == GDN_F32, s) : launch<GDN_E4M3, GDN_E5M2>(p, scales, type_out == GDN_F32, s);
+    return format_b == GDN_E4M3 ? launch<GDN_E5M2, GDN_E4M3>(p, scales, type_out == GDN_F32, s) : launch<GDN_E5M2, GDN_E5M2>(p, scales, type_out == GDN_F32, s);
+}

@@ -1,0 +1,110 @@
+// Parameter block and launches of the fp8 block-scaled product (fp8_matmul.hip
+// holds its entry point and the rule that picks its kernel; fp8_tiles.hpp the
+// tiled kernel, instantiated for each pair of formats in fp8_mm_*.hip).
+#pragma once
+
+#include "gdn_common.hpp"
+
+namespace gdn_fp8 {
+
+struct MatmulParams {
+    const uint8_t *a, *b;        // codes [M, lda], [N, ldb]
+    const uint8_t* a_scale;      // e8m0 [K / 128][lda_s]
+    const void* b_scale;         // see Scales
+    void* out;                   // [M, ldo] bf16 or fp32
+    long long lda, ldb, lda_s, ldb_s, ldo;
+    int M, N, K;
+    int wide;  // 16-byte stores fit
+};
+
+// b's scales: e8m0 or fp32, one a 128 x 128 block [ceil(N / 128)][ldb_s >= K / 128]
+// or one a row and block of 128, [K / 128][ldb_s >= N].
+enum Scales { kE8Block = 0, kE8Row = 1, kF32Block = 2, kF32Row = 3 };
+
+// Tiles of the tiled kernel (columns x tokens), largest first.
+enum Tile { k256x256 = 0, k128x128, k64x64, k32x32, kTiles };
+
+// Defined in fp8_mm_*.hip for each pair of formats (of a, of b).  f32: out is
+// fp32 (and the products are summed in full, see fp8_tiles.hpp), else bf16.
+template <int FA, int FB>
+int launch_tile(int tile, int scales, bool f32, const MatmulParams& p, hipStream_t stream);
+
+}  // namespace gdn_fp8
+
+namespace {
+
+using namespace gdn;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ i32x8 join(const u32x4 lo, const u32x4 hi) {
+    return i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
+                 static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
+}
+
+// MFMA 16x16x128 of fp8 operands with fp32 sums: rows of W (format FW) as the A
+// operand, tokens (format FX) as the B operand, so a lane's accumulator is four
+// neighbouring columns of one token.  Lane l supplies row l % 16 of its operand
+// and 32 of the 128 k values, which 32 is free as long as both agree (one scale
+// covers all 128).  SW, SX: byte of `sw`, `sx` that is the lane's row's e8m0
+// scale; 127 is 1.
+//
+// The instruction lines a block's products up with the largest and drops what
+// lies below about 2^-17 of that (measured: 2^-1 next to 1.75 * 2^16 is lost),
+// 1.4e-5 of a sum over normal values: nothing beside a bf16 result's 2^-9, too
+// much for an fp32 one.
+template <int FW, int FX, int SW, int SX>
+__device__ __forceinline__ f32x4 mfma_fp8(const i32x8 w, const i32x8 x, const f32x4 c, int sw, int sx) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, FW, FX, SW, sw, SX, sx);
+}
+
+// Eight codes times a power of two as bf16, exactly (but where it leaves bf16's
+// range): an e8m0 scale byte s as the fp32 bits s << 23, 255 giving NaN.  Their
+// products are exact in fp32 and the bf16 MFMA sums them in fp32.
+template <int F>
+__device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi, uint32_t scale_byte) {
+    const float s = __uint_as_float(scale_byte << 23);
+    union {
+        bf16x2 p[4];
+        bf16x8 v;
+    } u;
+    if constexpr (F == GDN_E4M3) {
+        u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false);
+        u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+        u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false);
+        u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+    } else {
+        u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, s, false);
+        u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, s, true);
+        u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, s, false);
+        u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, s, true);
+    }
+    return u.v;
+}
+
+// Writes four neighbouring columns from col on of row `row`.
+template <bool F32>
+__device__ __forceinline__ void store4(const gdn_fp8::MatmulParams& p, long long row, int col, const f32x4 v) {
+    const size_t at = static_cast<size_t>(row) * p.ldo + col;
+    if constexpr (F32) {
+        float* const o = static_cast<float*>(p.out) + at;
+        if (p.wide && col + 4 <= p.N) {
+            *reinterpret_cast<f32x4*>(o) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < p.N) o[i] = v[i];
+        }
+    } else {
+        uint16_t* const o = static_cast<uint16_t*>(p.out) + at;
+        if (p.wide && col + 4 <= p.N) {
+            *reinterpret_cast<u32x2*>(o) = pack4_bf16(v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < p.N) o[i] = f2bf_bits(v[i]);
+        }
+    }
+}
+
+}  // namespace

@@ -1,0 +1,168 @@
+// Quantisation to 8-bit floating point in blocks of 128 (fp8_blocks.hpp), along
+// the rows of x [M, K], along its columns (the codes of x^T, for a product that
+// sums over x's rows), or both from one read; a block is 1 x 128 values along
+// the codes' own rows, or 128 x 128 of x.
+//
+// One workgroup a 128 x 128 tile: a thread holds 8 x 8 of it in registers, a
+// row's maximum meets over 16 lanes by DPP, a column's over LDS, and the
+// transposed codes pass through LDS so that both layouts leave in whole
+// 128-byte lines.  What bounds it: HBM (2 bytes read, 1 or 2 written a value).
+#include "block_norm.hpp"
+#include "fp8_blocks.hpp"
+
+namespace {
+
+struct QuantParams {
+    const void* x;
+    long long ldx;
+    uint8_t *codes, *scales, *codes_t, *scales_t;  // codes [M, ldc], codes_t [K, ldt]; null: not wanted
+    long long ldc, lds, ldt, ldst;
+    int M, K, kb;  // kb: tiles along K
+    int vec;       // 16-byte loads fit
+};
+
+template <class TX, int FMT, bool BLOCK>
+__global__ __launch_bounds__(256) void gdn_fp8_quantize_kernel(QuantParams p) {
+    constexpr int kRowB = 144;  // bytes of a transposed row in LDS
+    __shared__ __attribute__((aligned(16))) unsigned char tile[128 * kRowB];
+    __shared__ uint32_t most[16][132];
+    __shared__ uint32_t bytes[128];
+    const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4;
+    const int k0 = static_cast<int>(blockIdx.x % p.kb) * kBlk, m0 = static_cast<int>(blockIdx.x / p.kb) * kBlk;
+    const int c = k0 + 8 * cg, r0 = m0 + 8 * rg;
+
+    float f[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long row = static_cast<long long>(min(r0 + i, p.M - 1)) * p.ldx;
+        if (p.vec)
+            Oct<TX>::template load<true>(p.x, row, c, p.K).get(f[i]);
+        else
+            Oct<TX>::template load<false>(p.x, row, c, p.K).get(f[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[i][j] = r0 + i < p.M && c + j < p.K ? f[i][j] : 0.f;
+
+    uint32_t rowb[8];  // scale bytes of the thread's rows
+    if constexpr (BLOCK) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, amax8(f[i]));
+        m = max16(m);
+        if (cg == 0) most[rg][0] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, most[i][0]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rowb[i] = Fp8<FMT>::scale_byte(m);
+        if (tid == 0) {
+            const int kt = k0 / kBlk, mt = m0 / kBlk;
+            if (p.codes) p.scales[mt * p.lds + kt] = static_cast<uint8_t>(rowb[0]);
+            if (p.codes_t) p.scales_t[kt * p.ldst + mt] = static_cast<uint8_t>(rowb[0]);
+        }
+    } else if (p.codes) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rowb[i] = Fp8<FMT>::scale_byte(max16(amax8(f[i])));
+        if (cg == 0 && r0 < p.lds) {
+            uint32_t w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[i] = rowb[4 * i] | rowb[4 * i + 1] << 8 | rowb[4 * i + 2] << 16 | rowb[4 * i + 3] << 24;
+            *reinterpret_cast<u32x2*>(p.scales + static_cast<long long>(k0 / kBlk) * p.lds + r0) = u32x2{w[0], w[1]};
+        }
+    }
+    if (p.codes) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const u32x2 w = Fp8<FMT>::codes8(f[i], Fp8<FMT>::inverse(rowb[i]), rowb[i] == 0xffu);
+            if (r0 + i < p.M) *reinterpret_cast<u32x2*>(p.codes + static_cast<long long>(r0 + i) * p.ldc + c) = w;
+        }
+    }
+    if (!p.codes_t) return;
+
+    uint32_t colb[8];
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) colb[j] = rowb[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i][j]) & 0x7fffffffu);
+            most[rg][8 * cg + j] = m;
+        }
+        __syncthreads();
+        if (tid < 128) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = max(m, most[i][tid]);
+            const uint32_t b = Fp8<FMT>::scale_byte(m);
+            bytes[tid] = b;
+            if (k0 + tid < p.K) p.scales_t[static_cast<long long>(m0 / kBlk) * p.ldst + k0 + tid] = static_cast<uint8_t>(b);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) colb[j] = bytes[8 * cg + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = f[i][j];
+        *reinterpret_cast<u32x2*>(tile + (8 * cg + j) * kRowB + 8 * rg) =
+            Fp8<FMT>::codes8(t, Fp8<FMT>::inverse(colb[j]), colb[j] == 0xffu);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = 32 * i + tid / 8;
+        if (k0 + k < p.K)
+            *reinterpret_cast<u32x4*>(p.codes_t + static_cast<long long>(k0 + k) * p.ldt + m0 + 16 * (tid & 7)) =
+                *reinterpret_cast<const u32x4*>(tile + k * kRowB + 16 * (tid & 7));
+    }
+}
+
+}  // namespace
+
+extern "C" int gdn_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, int block_rows, int format,
+                                    uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, uint8_t* codes_t, int64_t ldt,
+                                    uint8_t* scales_t, int64_t ldst, void* stream) {
+    using gdn_host::aligned;
+    using gdn_host::fail;
+    if (M < 0 || K < 0) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_quantize: M=%lld K=%lld", (long long)M, (long long)K);
+    if (block_rows != 1 && block_rows != kBlk) return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: blocks of %d x 128, 1 or 128 rows are supported", block_rows);
+    if (type_x != GDN_BF16 && type_x != GDN_F32) return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: type %d of x", type_x);
+    if (format != GDN_E4M3 && format != GDN_E5M2) return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: format %d", format);
+    const int64_t MB = (M + kBlk - 1) / kBlk, KB = (K + kBlk - 1) / kBlk;
+    if (M > 0x7fffffffLL - kBlk || K > 0x7fffffffLL - kBlk || MB * KB > 0x7fffffffLL)
+        return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: problem too large");
+    if (!codes && !codes_t) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_quantize: no output");
+    if (M == 0 || K == 0) return GDN_OK;
+    if (!x || !aligned(x, type_bytes(type_x)) || ldx < K) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_quantize: x null, unaligned or ldx < K");
+    const bool block = block_rows == kBlk;
+    if (codes && (!scales || !aligned(codes, 16) || ldc % 16 != 0 || ldc < KB * kBlk ||
+                  (block ? lds < KB : lds < M || lds % 16 != 0 || !aligned(scales, 16))))
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_quantize: codes [M, ldc >= K padded to 128] with 16-byte rows, scales of lds >= %lld",
+                    (long long)(block ? KB : M));
+    if (codes_t && (!scales_t || !aligned(codes_t, 16) || ldt % 16 != 0 || ldt < MB * kBlk || ldst < (block ? MB : K)))
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_quantize: codes_t [K, ldt >= M padded to 128] with 16-byte rows, scales_t of ldst >= %lld",
+                    (long long)(block ? MB : K));
+    QuantParams p = {};
+    p.x = x, p.ldx = ldx, p.M = static_cast<int>(M), p.K = static_cast<int>(K), p.kb = static_cast<int>(KB);
+    p.codes = codes, p.scales = scales, p.ldc = ldc, p.lds = lds;
+    p.codes_t = codes_t, p.scales_t = scales_t, p.ldt = ldt, p.ldst = ldst;
+    p.vec = K % 8 == 0 && vec_rows(x, ldx, type_x);
+    const auto launch = [&](auto tx, auto fmt, auto blk) {
+        hipLaunchKernelGGL((gdn_fp8_quantize_kernel<decltype(tx), decltype(fmt)::value, decltype(blk)::value>),
+                           dim3(static_cast<unsigned>(MB * KB)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+        return gdn_host::check_launch("gdn_fp8_quantize_kernel");
+    };
+    const auto of_format = [&](auto tx, auto blk) {
+        return format == GDN_E4M3 ? launch(tx, std::integral_constant<int, GDN_E4M3>{}, blk)
+                                  : launch(tx, std::integral_constant<int, GDN_E5M2>{}, blk);
+    };
+    const auto of_type = [&](auto blk) { return type_x == GDN_F32 ? of_format(0.f, blk) : of_format(bf16(), blk); };
+    return block ? of_type(std::true_type{}) : of_type(std::false_type{});
+}

@@ -30,6 +30,10 @@
  *   gdn_decode_out_proj_hip   <- GDNLayerCustom.decode's output projection, gdn_layer.py:309
  *   gdn_out_proj_hip, _fits   <- GDNLayerCustom.forward's output projection, gdn_layer.py:263
  *   gdn_layer_decode_step_hip <- GDNLayerCustom.decode as a whole, gdn_layer.py:265-316
+ *   gdn_block_norm_hip, _bwd  <- no reference counterpart (the reference layer has no residual,
+ *                                gate or norm after the block, and no backward pass)
+ *   gdn_fp8_quantize_hip,     <- no reference counterpart (8-bit projections)
+ *   gdn_fp8_matmul_hip
  */
 #ifndef GDN_AMD_H
 #define GDN_AMD_H
@@ -354,6 +358,93 @@ int gdn_layer_decode_step_hip(const gdn_bf16_t* x, const gdn_bf16_t* gamma, floa
                               const float* S_in, float* S_out, float scale, const gdn_bf16_t* W_o, gdn_bf16_t* q,
                               gdn_bf16_t* k, gdn_bf16_t* v, gdn_bf16_t* a, gdn_bf16_t* b, float* o, gdn_bf16_t* y,
                               int B, int D, int H, int dk, int dv, int conv_k, void* stream);
+
+/* Element types, 8-bit formats (e4m3: largest 448; e5m2: largest 57344) and gate activations. */
+enum { GDN_BF16 = 0, GDN_F32 = 1, GDN_E8M0 = 2 };
+enum { GDN_E4M3 = 0, GDN_E5M2 = 1 };
+enum { GDN_ACT_NONE = 0, GDN_ACT_SIGMOID = 1, GDN_ACT_SILU = 2, GDN_ACT_TANH = 3 };
+
+/*
+ * The norms before and after a block, fused with its gate and residual:
+ *   u = RMSNorm(y) post_gamma                       (u = y without post_gamma)
+ *   h = residual + residual_scale scale act(gate) u (absent: 0 and 1)
+ *   n = RMSNorm(h) gamma
+ * in fp32, rounded once where written; n follows from the unrounded h.
+ *   y [R, D], gate [ceil(R / rows_per_gate), D] (row r takes gate row
+ *   r / rows_per_gate: 1 = a gate row a token, T = one a sequence of T, R =
+ *   one for all), n [R, D]: type_y; residual, h [R, D]: type_r;
+ *   post_gamma, gamma, scale [D]: type_p.  Inputs but y may be NULL, outputs
+ *   too.  Types (y, r, p): bf16 bf16 bf16, bf16 bf16 fp32, bf16 fp32 fp32,
+ *   fp32 fp32 fp32.  ld*: elements from a row to the next.  h may be residual
+ *   itself (same stride).
+ *   codes [R, ldc >= D padded to 128] and scales [ceil(D / 128), lds >= R]: n
+ *   (h without gamma), unrounded, as e4m3 codes in blocks of 128 columns (see
+ *   gdn_fp8_quantize_hip); codes 16-byte aligned, ldc % 16 == 0.
+ *   rstd_y, rstd_h [R]: 1 / rms of y (with post_gamma) and of h (with gamma),
+ *   which gdn_block_norm_bwd_hip takes.
+ * D <= 16384, any D and alignment (16-byte ones and D % 8 == 0 are faster).
+ */
+int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residual, int64_t ldr, const void* gate, int64_t ldg,
+                       int64_t rows_per_gate, const void* post_gamma, const void* gamma, const void* scale,
+                       float residual_scale, int act, float eps, void* h, int64_t ldh, void* n, int64_t ldn,
+                       uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, float* rstd_y, float* rstd_h,
+                       int64_t R, int64_t D, int type_y, int type_r, int type_p, void* stream);
+
+/*
+ * Gradients of gdn_block_norm_hip.  dh [R, D] (type_r) and dn [R, D] (type_y)
+ * are those of h and n, either may be NULL (0; dn, gamma and rstd_h go
+ * together, as do post_gamma and rstd_y); the other inputs and the rstd are the
+ * forward pass's.  Outputs, contiguous, of their inputs' types, NULL = not
+ * wanted (dy is): dresidual, dy [R, D], dgate [gate rows, D], dpost_gamma,
+ * dgamma, dscale [D].  A gate row that rows share, and the parameters, get
+ * fp32 sums in a fixed order.  workspace: gdn_block_norm_bwd_workspace_bytes
+ * (R, D, rows_per_gate, or 1 without a gate) bytes, 16-byte aligned, where a
+ * parameter's or a shared gate's gradient is wanted.  R == 0: the parameters'
+ * gradients are zeros, dgate is not written.  At most 65535 shared gate rows.
+ */
+size_t gdn_block_norm_bwd_workspace_bytes(int64_t R, int64_t D, int64_t rows_per_gate);
+
+int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* dn, int64_t lddn, const void* y, int64_t ldy,
+                           const void* residual, int64_t ldr, const void* gate, int64_t ldg, int64_t rows_per_gate,
+                           const void* post_gamma, const void* gamma, const void* scale, float residual_scale, int act,
+                           const float* rstd_y, const float* rstd_h, void* dresidual, void* dy, void* dgate,
+                           void* dpost_gamma, void* dgamma, void* dscale, int64_t R, int64_t D, int type_y, int type_r,
+                           int type_p, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * x [M, K] (bf16 or fp32, rows ldx elements apart) to 8-bit floating point
+ * (GDN_E4M3 or GDN_E5M2), one power-of-two scale a block of block_rows (1 or
+ * 128) x 128 values: 2^e with the least e >= -127 for which the block's largest
+ * magnitude over 2^e is no larger than the format's largest number (e = 0 for
+ * zeros), kept as the byte e + 127 (e8m0); a code is value / 2^e to the nearest,
+ * ties to even.  A block with an infinity or NaN gets scale NaN (0xff), codes
+ * NaN.  Along the rows: codes [M, ldc], columns K up to the next multiple of 128
+ * zero; scales [ceil(K / 128), lds >= M] (block_rows 1; lds % 16 == 0) or
+ * [ceil(M / 128), lds >= ceil(K / 128)] (128).  Along the columns, the same of
+ * x^T: codes_t [K, ldt], columns M up to the next multiple of 128 zero; scales_t
+ * [ceil(M / 128), ldst >= K] or [ceil(K / 128), ldst >= ceil(M / 128)].  Either
+ * pair may be NULL.  Code rows 16-byte aligned.
+ */
+int gdn_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, int block_rows, int format,
+                         uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, uint8_t* codes_t, int64_t ldt,
+                         uint8_t* scales_t, int64_t ldst, void* stream);
+
+/*
+ * Product of fp8 codes with a scale for each block of 128:
+ *   out[m, n] = sum_kb a_scale[m, kb] b_scale[n, kb] sum_{k in kb} a[m, k] b[n, k]
+ * fp32 sums, out [M, ldo] bf16 or fp32 (type_out).
+ *   a [M, lda], b [N, ldb] codes (16-byte aligned rows, lda and ldb <= 2^22);
+ *   a_scale e8m0 [K / 128, lda_s >= M], 16-byte aligned, lda_s % 16 == 0;
+ *   b_scale e8m0 or fp32 (type_b_scale), a 128 x 128 block each
+ *   [ceil(N / 128), ldb_s >= K / 128] (b_block_rows 128) or a row and block
+ *   each [K / 128, ldb_s >= N], 16-byte aligned, ldb_s % 16 == 0 (1).
+ * K % 128 == 0 (zero codes pad), any M and N.  A row's sums do not depend on
+ * other rows' values; their order follows M, N and K.
+ */
+int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_t* a_scale, int64_t lda_s,
+                       const uint8_t* b, int64_t ldb, int format_b, const void* b_scale, int64_t ldb_s, int b_block_rows,
+                       int type_b_scale, void* out, int64_t ldo, int type_out, int64_t M, int64_t N, int64_t K,
+                       void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,222 @@
+"""fp8 quantisation and the fp8 block-scaled product on the GPU against their
+definitions.
+
+Quantisation has one answer, so codes and scales are compared bit for bit.  The
+product's terms are exact in fp32 (two 4-bit significands, or their product with
+powers of two), so an fp32 result is off by at most K additions' half steps,
+K 2^-24 of the terms' magnitudes, whatever their order; a 32-bit scale of b
+adds one rounding a block and one a term (two more steps).  A bf16 result adds
+half its own step, and what the fp8 matrix instruction drops of a block's 128
+products: 2^-17 of the largest at most for each, so 2^-10 of the product of the
+block's largest codes and scales.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E4, E5, E8 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
+TOP = {E4: 448.0, E5: 57344.0}
+
+
+def _up(n, to):
+    return -(-n // to) * to
+
+
+def _quantize64(x, rows, fmt):
+    """(codes, scale bytes) of x by definition, on the CPU."""
+    M, K = x.shape
+    p = torch.zeros(_up(M, rows), _up(K, 128), dtype=torch.float64)
+    p[:M, :K] = x.double().cpu()
+    t = p.view(p.shape[0] // rows, rows, -1, 128)
+    bad = ~torch.isfinite(t).all(3).all(1)
+    amax = torch.where(torch.isfinite(t), t.abs(), 0).amax((1, 3))
+    m, e = torch.frexp(amax / TOP[fmt])  # amax / top = m 2^e, 1/2 <= m < 1: 2^(e - 1) holds it only at m = 1/2
+    e = torch.where(amax > 0, torch.where(m == 0.5, e - 1, e), 0).clamp(min=-127)
+    codes = (t / torch.ldexp(torch.ones_like(amax), e)[:, None, :, None]).float().to(fmt).view(torch.uint8)
+    codes = torch.where(bad[:, None, :, None], torch.tensor(0x7f, dtype=torch.uint8), codes)
+    scales = torch.where(bad, 255, e + 127).to(torch.uint8)
+    return codes.view(p.shape)[:M], scales
+
+
+SPECIAL = torch.tensor([0.0, -0.0, 448.0, 448.5, 57344.0, 57600.0, 1e-38, 1e-40, 3e38, -3e38, 1.0, 2.0 ** -126, 2.0 ** -133])
+
+
+@pytest.mark.parametrize("fmt", [E4, E5], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,K", [(1, 16), (1, 2048), (3, 130), (77, 1000), (128, 128), (129, 384), (300, 513), (1, 1), (260, 8)])
+def test_quantize(exts, dev, M, K, dtype, block, fmt):
+    g = torch.Generator().manual_seed(M * K)
+    x = (torch.randn(M, K, generator=g) * torch.exp(3 * torch.randn(M, 1, generator=g))).to(dtype)
+    x.view(-1)[torch.randint(0, M * K, (min(13, M * K),), generator=g)] = SPECIAL[:min(13, M * K)].to(dtype)
+    if M > 2:
+        x[1] = 0
+    got = exts["proj"].fp8_quantize(x.to(dev), block_rows=block, dtype=fmt, rows=True, columns=True)
+    for (codes, scales), t in ((got[:2], x), (got[2:], x.t())):
+        rc, rs = _quantize64(t, block, fmt)
+        assert codes.dtype == fmt and scales.dtype == E8
+        assert torch.equal(scales.view(torch.uint8).cpu(), rs)
+        got_c = codes.view(torch.uint8).cpu()
+        assert got_c.shape == rc.shape
+        same = (got_c == rc) | ((got_c & 0x7f == 0) & (rc & 0x7f == 0))  # the sign of an underflowed zero is free
+        assert same.all(), (codes.float().cpu()[~same][:5], rc.view(fmt).float()[~same][:5])
+    # each alone gives the same
+    for kw, pair in ((dict(rows=True), got[:2]), (dict(rows=False, columns=True), got[2:])):
+        alone = exts["proj"].fp8_quantize(x.to(dev), block_rows=block, dtype=fmt, **kw)
+        assert len(alone) == 2 and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(alone, pair))
+
+
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_not_finite(exts, dev, block):
+    x = torch.randn(200, 300, generator=torch.Generator().manual_seed(1))
+    x[5, 7], x[150, 290] = float("nan"), float("-inf")
+    got = exts["proj"].fp8_quantize(x.to(dev), block_rows=block, rows=True, columns=True)
+    for (codes, scales), t in ((got[:2], x), (got[2:], x.t())):
+        rc, rs = _quantize64(t, block, E4)
+        assert torch.equal(scales.view(torch.uint8).cpu(), rs) and torch.equal(codes.view(torch.uint8).cpu(), rc)
+
+
+def test_quantize_strided_rows(exts, dev):
+    wide = torch.randn(90, 700, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(dev)
+    for lo, hi in ((64, 320), (3, 290), (64, 321)):
+        a = exts["proj"].fp8_quantize(wide[:, lo:hi], rows=True, columns=True)
+        b = exts["proj"].fp8_quantize(wide[:, lo:hi].contiguous(), rows=True, columns=True)
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
+# ---------------------------------------------------------------------------
+# The product
+# ---------------------------------------------------------------------------
+def _codes(M, K, fmt, g):
+    return (torch.randn(M, K, generator=g) * (100 if fmt == E4 else 3000)).clamp(-TOP[fmt], TOP[fmt]).to(fmt)
+
+
+def _scales(M, KB, g):
+    return torch.randint(110, 140, (M, KB), generator=g).to(torch.uint8).view(E8)
+
+
+def _product64(a, sa, b, sb):
+    rows = 128 if sb.shape[0] != b.shape[0] or b.shape[0] == 1 else 1
+    A = a.double() * sa.double().repeat_interleave(128, 1)
+    B = b.double() * sb.double().repeat_interleave(128, 1).repeat_interleave(rows, 0)[:b.shape[0]]
+    return A @ B.t(), A.abs() @ B.abs().t()
+
+
+def _check(out, a, sa, b, sb):
+    ref, mag = _product64(a, sa, b, sb)
+    tol = (a.shape[1] + 2) * 2.0 ** -24 * mag
+    if out.dtype == torch.bfloat16:
+        rows = 128 if sb.shape[0] != b.shape[0] or b.shape[0] == 1 else 1
+        top = lambda t, s: t.double().abs().view(t.shape[0], -1, 128).amax(2) * s  # noqa: E731
+        tol += 2.0 ** -10 * top(a, sa.double()) @ top(b, sb.double().repeat_interleave(rows, 0)[:b.shape[0]]).t()
+        tol += 2.0 ** -8 * (ref.abs() + tol)
+    far = (out.double() - ref).abs() - tol
+    assert out.shape == ref.shape and not (far > 0).any(), f"{(far > 0).sum().item()} values, the worst {far.max().item():.3g} past its bound"
+
+
+def _operands(M, N, K, fa, fb, bscale, rows, dev, seed=0):
+    g = torch.Generator().manual_seed(seed + M + 31 * N + 7 * K)
+    a, b = _codes(M, K, fa, g), _codes(N, K, fb, g)
+    sa = _scales(M, K // 128, g)
+    sb = _scales(N if rows == 1 else -(-N // 128), K // 128, g)
+    if bscale == "fp32":
+        sb = sb.float() * (1 + torch.rand(sb.shape, generator=g))
+    return a.to(dev), sa.to(dev), b.to(dev), sb.to(dev)
+
+
+SIZES = [(1, 1, 128), (1, 2048, 2048), (2, 100, 384), (16, 129, 1152), (17, 40, 128), (33, 65, 256), (77, 300, 1280), (64, 64, 8448),
+         (130, 1040, 384), (300, 1030, 512), (513, 2100, 256), (1030, 2050, 384), (2500, 5003, 256), (5, 33, 8448)]
+
+
+@pytest.mark.parametrize("fa,fb", [(E4, E4), (E5, E4), (E4, E5), (E5, E5)], ids=["e4e4", "e5e4", "e4e5", "e5e5"])
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_product(exts, dev, M, N, K, bscale, rows, fa, fb):
+    a, sa, b, sb = _operands(M, N, K, fa, fb, bscale, rows, dev)
+    for out in (torch.float32, torch.bfloat16):
+        y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
+        assert y.dtype == out and y.shape == (M, N)
+        _check(y, a, sa, b, sb)
+
+
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("fp32", 128), ("e8m0", 1)])
+@pytest.mark.parametrize("M,N", [(2100, 4400), (300, 1030)])
+def test_product_long(exts, dev, M, N, bscale, rows):
+    """More blocks than a wave holds scales for at once."""
+    a, sa, b, sb = _operands(M, N, 8448, E4, E4, bscale, rows, dev)
+    _check(exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=torch.float32), a, sa, b, sb)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 200, 256), (150, 300, 256)])
+def test_product_strides_and_scale_layouts(exts, dev, M, N, K):
+    """Codes in wider rows, scales in any layout: the same bits."""
+    a, sa, b, sb = _operands(M, N, K, E4, E4, "e8m0", 1, dev)
+    f = exts["proj"].fp8_matmul
+    want = f(a, sa, b, sb)
+    wa = torch.zeros(M, K + 64, dtype=torch.uint8, device=dev)
+    wa[:, 16:16 + K] = a.view(torch.uint8)
+    wb = torch.zeros(N, 2 * K, dtype=torch.uint8, device=dev)
+    wb[:, :K] = b.view(torch.uint8)
+    assert torch.equal(f(wa.view(E4)[:, 16:16 + K], sa, wb.view(E4)[:, :K], sb), want)
+    buf = torch.full((K // 128, _up(M, 16) + 32), 77, dtype=torch.uint8, device=dev)
+    buf[:, 16:16 + M] = sa.view(torch.uint8).t()
+    assert torch.equal(f(a, buf.view(E8)[:, 16:16 + M].t(), b, sb), want)
+    wide = torch.zeros(M, 40, dtype=torch.uint8, device=dev)
+    wide[:, 3:3 + K // 128] = sa.view(torch.uint8)
+    assert torch.equal(f(a, wide.view(E8)[:, 3:3 + K // 128], b, sb.contiguous()), want)
+
+
+def test_product_special_codes(exts, dev):
+    """NaN codes and NaN scales reach exactly the outputs whose sums meet them."""
+    a, sa, b, sb = _operands(40, 300, 256, E4, E4, "e8m0", 128, dev)
+    clean = exts["proj"].fp8_matmul(a, sa, b, sb)
+    a.view(torch.uint8)[3, 200] = 0x7f
+    sa.view(torch.uint8)[7, 0] = 255
+    sb.view(torch.uint8)[1, 1] = 255
+    y = exts["proj"].fp8_matmul(a, sa, b, sb)
+    want = torch.zeros(40, 300, dtype=torch.bool)
+    want[3], want[7], want[:, 128:256] = True, True, True
+    assert torch.equal(y.isnan().cpu(), want)
+    assert torch.equal(y[~want.to(dev)], clean[~want.to(dev)])
+
+
+def test_product_empty(exts, dev):
+    a, sa, b, sb = _operands(4, 32, 128, E4, E4, "e8m0", 1, dev)
+    assert exts["proj"].fp8_matmul(a[:0], sa[:0], b, sb).shape == (0, 32)
+    assert exts["proj"].fp8_matmul(a, sa, b[:0], sb[:0]).shape == (4, 0)
+
+
+def test_rows_do_not_depend_on_their_neighbours(exts, dev):
+    a, sa, b, sb = _operands(200, 300, 512, E4, E4, "e8m0", 128, dev)
+    want = exts["proj"].fp8_matmul(a, sa, b, sb)
+    a2, sa2 = a.clone(), sa.clone()
+    a2.view(torch.uint8)[100:] = 0x7f
+    assert torch.equal(exts["proj"].fp8_matmul(a2, sa2, b, sb)[:100], want[:100])
+    assert torch.equal(exts["proj"].fp8_matmul(a, sa, b, sb), want)
+
+
+def test_product_graph_replays_match_eager(exts, dev):
+    x = torch.randn(130, 512, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(dev)
+    w = torch.randn(300, 512, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(dev)
+    wq, ws = exts["proj"].fp8_quantize(w, block_rows=128)
+
+    def f():
+        return exts["proj"].fp8_matmul(*exts["proj"].fp8_quantize(x), wq, ws)
+
+    eager = f()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        f()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = f()
+    for _ in range(3):
+        y.fill_(7.0)
+        graph.replay()
+        exts["proj"].fp8_matmul(*exts["proj"].fp8_quantize(w), wq, ws)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
