@@ -21,44 +21,43 @@ __global__ __launch_bounds__(64 * kFewWaves) void gdn_fp8_few_kernel(gdn_fp8::Ma
     const uint8_t* const x = p.a + static_cast<size_t>(tok) * p.lda + 16 * g4;
     const bool rows = scales == gdn_fp8::kE8Row || scales == gdn_fp8::kF32Row;
     const bool f32 = scales == gdn_fp8::kF32Block || scales == gdn_fp8::kF32Row;
-    // e8m0: the lane's row of b; fp32: the four columns of its accumulator
-    const size_t sstep = rows ? p.ldb_s : 1;
-    const uint8_t* const s8 = static_cast<const uint8_t*>(p.b_scale) + (rows ? row : static_cast<size_t>(row / 128) * p.ldb_s);
-    size_t s4[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = min(n0 + 4 * g4 + i, p.N - 1);
-        s4[i] = rows ? c : static_cast<size_t>(c / 128) * p.ldb_s;
-    }
+    // the scale of the lane's row of b, its accumulator's column
+    const size_t sstep = rows ? p.ldb_s : 1, sat = rows ? row : static_cast<size_t>(row / 128) * p.ldb_s;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int kb = wave; kb < nslices; kb += kFewWaves) {
         const u32x4* const wp = reinterpret_cast<const u32x4*>(w + static_cast<size_t>(kb) * 128);
         const u32x4* const xp = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(kb) * 128);
         const int sx = p.a_scale[kb * p.lda_s + tok];
-        const int sw = f32 ? 127 : s8[kb * sstep];
+        int sw = 127;
+        float fw = 1.f;
+        if (f32)
+            fw = static_cast<const float*>(p.b_scale)[sat + kb * sstep];
+        else
+            sw = static_cast<const uint8_t*>(p.b_scale)[sat + kb * sstep];
         const i32x8 wc = join(wp[0], wp[4]), xc = join(xp[0], xp[4]);
-        f32x4 t = f32 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
+        f32x4 t = {0.f, 0.f, 0.f, 0.f};
         if constexpr (OUT32) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                t = mfma16x16x32(codes_to_bf16<FB>(wc[2 * q], wc[2 * q + 1], sw), codes_to_bf16<FA>(xc[2 * q], xc[2 * q + 1], sx), t);
+                t = mfma16x16x32(codes_to_bf16<FA>(xc[2 * q], xc[2 * q + 1], sx), codes_to_bf16<FB>(wc[2 * q], wc[2 * q + 1], sw), t);
         } else {
-            t = mfma_fp8<FB, FA, 0, 0>(wc, xc, t, sw, sx);
+            t = mfma_fp8<FA, FB, 0, 0>(xc, wc, t, sx, sw);
         }
-        if (f32) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(static_cast<const float*>(p.b_scale)[s4[i] + kb * sstep], t[i], acc[i]);
-        } else {
-            acc = t;
-        }
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(fw, t[i], acc[i]);
     }
     sums[wave][lane] = acc;
     __syncthreads();
     if (wave > 0) return;
 #pragma unroll
     for (int i = 1; i < kFewWaves; ++i) acc += sums[i][lane];
-    if (r16 < p.M && n0 + 4 * g4 < p.N) store4<OUT32>(p, r16, n0 + 4 * g4, acc);
+    if (n0 + r16 >= p.N) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v[1] = {acc[i]};
+        if (4 * g4 + i < p.M) store_cols<OUT32>(p, 4 * g4 + i, n0 + r16, v);
+    }
 }
 
 long long tiles(const gdn_fp8::MatmulParams& p, int cols, int toks) {

@@ -42,20 +42,21 @@ __device__ __forceinline__ i32x8 join(const u32x4 lo, const u32x4 hi) {
                  static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
 }
 
-// MFMA 16x16x128 of fp8 operands with fp32 sums: rows of W (format FW) as the A
-// operand, tokens (format FX) as the B operand, so a lane's accumulator is four
-// neighbouring columns of one token.  Lane l supplies row l % 16 of its operand
+// MFMA 16x16x128 of fp8 operands with fp32 sums: tokens (format FX) as the A
+// operand, rows of W (format FW) as the B operand, so a lane's accumulator is
+// one column (lane % 16) of four tokens (4 (lane / 16) + i), and neighbouring
+// lanes store neighbouring columns.  Lane l supplies row l % 16 of its operand
 // and 32 of the 128 k values, which 32 is free as long as both agree (one scale
-// covers all 128).  SW, SX: byte of `sw`, `sx` that is the lane's row's e8m0
+// covers all 128).  SX, SW: byte of `sx`, `sw` that is the lane's row's e8m0
 // scale; 127 is 1.
 //
 // The instruction lines a block's products up with the largest and drops what
 // lies below about 2^-17 of that (measured: 2^-1 next to 1.75 * 2^16 is lost),
 // 1.4e-5 of a sum over normal values: nothing beside a bf16 result's 2^-9, too
 // much for an fp32 one.
-template <int FW, int FX, int SW, int SX>
-__device__ __forceinline__ f32x4 mfma_fp8(const i32x8 w, const i32x8 x, const f32x4 c, int sw, int sx) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, FW, FX, SW, sw, SX, sx);
+template <int FX, int FW, int SX, int SW>
+__device__ __forceinline__ f32x4 mfma_fp8(const i32x8 x, const i32x8 w, const f32x4 c, int sx, int sw) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, c, FX, FW, SX, sx, SW, sw);
 }
 
 // Eight codes times a power of two as bf16, exactly (but where it leaves bf16's
@@ -82,29 +83,23 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi, uint32
     return u.v;
 }
 
-// Writes four neighbouring columns from col on of row `row`.
-template <bool F32>
-__device__ __forceinline__ void store4(const gdn_fp8::MatmulParams& p, long long row, int col, const f32x4 v) {
-    const size_t at = static_cast<size_t>(row) * p.ldo + col;
-    if constexpr (F32) {
-        float* const o = static_cast<float*>(p.out) + at;
-        if (p.wide && col + 4 <= p.N) {
-            *reinterpret_cast<f32x4*>(o) = v;
-        } else {
+// Writes NC neighbouring columns from col on of row `row`, in one store where
+// they fit.
+template <bool F32, int NC>
+__device__ __forceinline__ void store_cols(const gdn_fp8::MatmulParams& p, long long row, int col, const float (&v)[NC]) {
+    using T = std::conditional_t<F32, float, bf16>;
+    typedef T vec __attribute__((ext_vector_type(NC)));
+    T* const o = static_cast<T*>(p.out) + static_cast<size_t>(row) * p.ldo + col;
+    if (p.wide && col + NC <= p.N) {
+        vec w;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < p.N) o[i] = v[i];
-        }
-    } else {
-        uint16_t* const o = static_cast<uint16_t*>(p.out) + at;
-        if (p.wide && col + 4 <= p.N) {
-            *reinterpret_cast<u32x2*>(o) = pack4_bf16(v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < p.N) o[i] = f2bf_bits(v[i]);
-        }
+        for (int i = 0; i < NC; ++i) w[i] = static_cast<T>(v[i]);
+        *reinterpret_cast<vec*>(o) = w;
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+        if (col + i < p.N) o[i] = static_cast<T>(v[i]);
 }
 
 }  // namespace
