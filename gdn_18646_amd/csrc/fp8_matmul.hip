@@ -60,16 +60,58 @@ __global__ __launch_bounds__(64 * kFewWaves) void gdn_fp8_few_kernel(gdn_fp8::Ma
     }
 }
 
-long long tiles(const gdn_fp8::MatmulParams& p, int cols, int toks) {
-    return static_cast<long long>((p.M + toks - 1) / toks) * ((p.N + cols - 1) / cols);
-}
+// What a call on a tile takes, us: c + rounds (a + b blocks of K), rounds of 256
+// workgroups, or, where two share a CU, of 512, and of up to 256 alone.  Fitted
+// to 114 products, 17 to 16384 tokens, N 512 to 8192, K 1024 to 4096 (kernels
+// back to back): the tile that the fit picks takes at most 1.16 times the best
+// one's time and 1.01 on average; 24 tiles were timed, those here are the ones
+// whose absence costs.
+struct TileCost {
+    int tile, cols, toks, per_cu;
+    float c, a1, b1, a2, b2;  // per_cu 2: alone (1) and two (2)
+};
+constexpr TileCost kBf16[] = {
+    {gdn_fp8::k256x256, 256, 256, 1, 0.f, 6.58f, 1.211f, 0.f, 0.f},
+    {gdn_fp8::k256x192, 256, 192, 1, 0.f, 5.86f, 1.081f, 0.f, 0.f},
+    {gdn_fp8::k256x128, 256, 128, 1, 0.f, 4.88f, 0.776f, 0.f, 0.f},
+    {gdn_fp8::k128x128, 128, 128, 1, 0.46f, 3.33f, 0.539f, 0.f, 0.f},
+    {gdn_fp8::k64x128, 64, 128, 1, 0.86f, 3.31f, 0.333f, 0.f, 0.f},
+    {gdn_fp8::k64x64, 64, 64, 1, 1.04f, 2.76f, 0.236f, 0.f, 0.f},
+    {gdn_fp8::k64x32, 64, 32, 1, 1.15f, 2.49f, 0.150f, 0.f, 0.f},
+    {gdn_fp8::k32x32, 32, 32, 2, 1.86f, 1.20f, 0.123f, 1.80f, 0.192f},
+};
+constexpr TileCost kF32[] = {
+    {gdn_fp8::k128x128, 128, 128, 2, 0.85f, 2.61f, 0.957f, 4.54f, 1.676f},
+    {gdn_fp8::k64x128, 64, 128, 1, 0.77f, 3.24f, 0.538f, 0.f, 0.f},
+    {gdn_fp8::k64x64, 64, 64, 1, 1.09f, 2.65f, 0.361f, 0.f, 0.f},
+    {gdn_fp8::k64x32, 64, 32, 1, 1.26f, 2.56f, 0.213f, 0.f, 0.f},
+    {gdn_fp8::k32x32, 32, 32, 2, 2.16f, 1.02f, 0.156f, 1.97f, 0.228f},
+};
 
-int choose_tile(const gdn_fp8::MatmulParams& p) {
+struct Choice {
+    int tile;
+    float us;
+};
+Choice choose_tile(long long M, long long N, int K, bool f32) {
     constexpr long long kCUs = 256;
-    if (tiles(p, 32, 32) <= kCUs) return gdn_fp8::k32x32;
-    if (tiles(p, 64, 64) <= 2 * kCUs) return gdn_fp8::k64x64;
-    if (tiles(p, 128, 128) <= 2 * kCUs) return gdn_fp8::k128x128;
-    return gdn_fp8::k256x256;
+    const TileCost* const table = f32 ? kF32 : kBf16;
+    const int n = static_cast<int>(f32 ? sizeof(kF32) / sizeof(kF32[0]) : sizeof(kBf16) / sizeof(kBf16[0]));
+    const float nk = static_cast<float>(K / 128);
+    Choice best = {0, 0.f};
+    for (int i = 0; i < n; ++i) {
+        const TileCost& t = table[i];
+        const long long tiles = (M + t.toks - 1) / t.toks * ((N + t.cols - 1) / t.cols);
+        float us = t.c;
+        if (t.per_cu == 1) {
+            us += static_cast<float>((tiles + kCUs - 1) / kCUs) * (t.a1 + t.b1 * nk);
+        } else {
+            const long long rest = tiles % (2 * kCUs);
+            us += static_cast<float>(tiles / (2 * kCUs) + (rest > kCUs ? 1 : 0)) * (t.a2 + t.b2 * nk);
+            if (rest > 0 && rest <= kCUs) us += t.a1 + t.b1 * nk;
+        }
+        if (i == 0 || us < best.us) best = {t.tile, us};
+    }
+    return best;
 }
 
 template <int FA, int FB>
@@ -82,7 +124,29 @@ int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t str
             hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, false>), grid, block, 0, stream, p, scales);
         return gdn_host::check_launch("gdn_fp8_few_kernel");
     }
-    return gdn_fp8::launch_tile<FA, FB>(choose_tile(p), scales, f32, p, stream);
+    // The last columns past a multiple of 256 in a launch of their own, on a tile
+    // of their size, where the fit says that this is faster than a column of
+    // large tiles for them: 16384 x 6176 x 2048, 32 columns past 6144, 209 us in
+    // one launch.
+    const Choice whole = choose_tile(p.M, p.N, p.K, f32);
+    const int rest = p.N % 256, main = p.N - rest;
+    if (rest > 0 && main > 0) {
+        const Choice left = choose_tile(p.M, main, p.K, f32), right = choose_tile(p.M, rest, p.K, f32);
+        if (left.us + right.us < whole.us) {
+            gdn_fp8::MatmulParams q = p;
+            q.N = main;
+            const int st = gdn_fp8::launch_tile<FA, FB>(left.tile, scales, f32, q, stream);
+            if (st != GDN_OK) return st;
+            const bool rows = scales == gdn_fp8::kE8Row || scales == gdn_fp8::kF32Row;
+            const size_t at = rows ? main : static_cast<size_t>(main / 128) * p.ldb_s;
+            q.N = rest;
+            q.b = p.b + static_cast<size_t>(main) * p.ldb;
+            q.b_scale = static_cast<const uint8_t*>(p.b_scale) + at * (scales == gdn_fp8::kF32Block || scales == gdn_fp8::kF32Row ? 4 : 1);
+            q.out = static_cast<uint8_t*>(p.out) + static_cast<size_t>(main) * (f32 ? 4 : 2);
+            return gdn_fp8::launch_tile<FA, FB>(right.tile, scales, f32, q, stream);
+        }
+    }
+    return gdn_fp8::launch_tile<FA, FB>(whole.tile, scales, f32, p, stream);
 }
 
 }  // namespace

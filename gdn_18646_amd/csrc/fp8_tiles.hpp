@@ -547,10 +547,14 @@ __global__ __launch_bounds__(TL::waves * 64)
 namespace gdn_fp8 {
 
 using Tile256x256 = Fp8Tile<4, 2, 4, 8, 2, 1, 1, true>;
-using Tile256x128 = Fp8Tile<4, 2, 4, 4, 3, 1>;  // fp32 results
-using Tile128x128 = Fp8Tile<4, 2, 2, 4, 4, 1>;
-using Tile64x64 = Fp8Tile<2, 2, 2, 2, 2, 2, 2>;
-using Tile32x32 = Fp8Tile<2, 2, 1, 1, 3, 1, 4>;
+using Tile256x192 = Fp8Tile<4, 2, 4, 6, 2, 1, 1, true>;
+using Tile256x128 = Fp8Tile<4, 2, 4, 4, 3, 1, 1, true>;
+using Tile128x128 = Fp8Tile<2, 4, 4, 2, 4, 1>;
+using Tile128x128Pair = Fp8Tile<2, 4, 4, 2, 2, 2>;  // fp32 results: two workgroups a CU, one converts while the other multiplies
+using Tile64x128 = Fp8Tile<1, 4, 4, 2, 3, 1, 2>;
+using Tile64x64 = Fp8Tile<2, 2, 2, 2, 3, 1, 2>;
+using Tile64x32 = Fp8Tile<1, 2, 4, 1, 3, 1, 4>;
+using Tile32x32 = Fp8Tile<1, 2, 2, 1, 2, 2, 4>;
 
 template <class TL, int FA, int FB, int SB, bool OUT32>
 int launch_scaled(const MatmulParams& p, hipStream_t stream) {
@@ -573,25 +577,23 @@ int launch_tiled(int scales, const MatmulParams& p, hipStream_t stream) {
 
 template <int FA, int FB>
 int launch_tile(int tile, int scales, bool f32, const MatmulParams& p, hipStream_t stream) {
-    const auto launch = [&](auto out32) {
+    const auto small = [&](auto out32) {
         constexpr bool O = decltype(out32)::value;
         switch (tile) {
-            case k128x128: return launch_tiled<Tile128x128, FA, FB, O>(scales, p, stream);
+            case k64x128: return launch_tiled<Tile64x128, FA, FB, O>(scales, p, stream);
             case k64x64: return launch_tiled<Tile64x64, FA, FB, O>(scales, p, stream);
+            case k64x32: return launch_tiled<Tile64x32, FA, FB, O>(scales, p, stream);
             case k32x32: return launch_tiled<Tile32x32, FA, FB, O>(scales, p, stream);
-            default: break;
-        }
-        // Two sets of accumulators (fp32 scales, fp32 results) do not fit the largest tile.
-        if constexpr (O) {
-            if (scales == kF32Row) return launch_scaled<Tile128x128, FA, FB, kF32Row, true>(p, stream);
-            if (scales == kF32Block) return launch_scaled<Tile128x128, FA, FB, kF32Block, true>(p, stream);
-            return scales == kE8Row ? launch_scaled<Tile256x128, FA, FB, kE8Row, true>(p, stream)
-                                    : launch_scaled<Tile256x128, FA, FB, kE8Block, true>(p, stream);
-        } else {
-            return launch_tiled<Tile256x256, FA, FB, false>(scales, p, stream);
+            default: return launch_tiled<std::conditional_t<O, Tile128x128Pair, Tile128x128>, FA, FB, O>(scales, p, stream);
         }
     };
-    return f32 ? launch(std::true_type{}) : launch(std::false_type{});
+    if (f32) return small(std::true_type{});
+    switch (tile) {
+        case k256x256: return launch_tiled<Tile256x256, FA, FB, false>(scales, p, stream);
+        case k256x192: return launch_tiled<Tile256x192, FA, FB, false>(scales, p, stream);
+        case k256x128: return launch_tiled<Tile256x128, FA, FB, false>(scales, p, stream);
+        default: return small(std::false_type{});
+    }
 }
 
 }  // namespace gdn_fp8
