@@ -8,7 +8,9 @@
 //
 // What bounds it: HBM for many rows (each input read once, each output written
 // once, two row sums between them that never leave the registers), the one
-// chain of loads, sums and stores for a few.
+// chain of loads, sums and stores for a few.  A workgroup walks rows with the
+// parameters of its columns in registers, and the next row's loads are under way
+// while a row is worked on.
 #include "block_norm.hpp"
 #include "fp8_blocks.hpp"
 
@@ -16,107 +18,138 @@ namespace {
 
 template <class TY, class TR, class TP, int LPR, int NV, bool VEC>
 __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(NormParams p) {
-    constexpr int SLOTS = LPR <= 64 ? 256 / LPR : 1;
-    __shared__ float sums[2][LPR > 64 ? LPR / 64 : 1];
+    constexpr int SLOTS = slots_of(LPR);
+    constexpr bool kAhead = NV == 1;  // the next row is loaded a row ahead (with two vectors a lane it does not fit)
+    __shared__ float sums[2][2][LPR > 64 ? LPR / 64 : 1];
     const int tid = threadIdx.x, lane = tid % LPR;
-    const int row = static_cast<int>(blockIdx.x) * SLOTS + tid / LPR;
-    const bool live = row < p.R;
-    const long long r = live ? row : p.R - 1;  // rows past the end repeat the last one and write nothing
     const int D = p.D;
-
-    Oct<TY> yr[NV], gr[NV];
-    Oct<TR> rr[NV];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) yr[u] = Oct<TY>::template load<VEC>(p.y, r * p.ldy, 8 * (lane + LPR * u), D);
-    if (p.residual) {
-#pragma unroll
-        for (int u = 0; u < NV; ++u) rr[u] = Oct<TR>::template load<VEC>(p.residual, r * p.ldr, 8 * (lane + LPR * u), D);
-    }
-    if (p.gate) {
-        const long long g = static_cast<unsigned>(r) / p.rows_per_gate;
-#pragma unroll
-        for (int u = 0; u < NV; ++u) gr[u] = Oct<TY>::template load<VEC>(p.gate, g * p.ldg, 8 * (lane + LPR * u), D);
-    }
     auto inside = [&](int u, int e) { return VEC ? 8 * (lane + LPR * u) < D : 8 * (lane + LPR * u) + e < D; };
 
-    float h[NV][8];
-    float ss = 0.f;
+    struct Row {
+        Oct<TY> y[NV], g[NV];
+        Oct<TR> r[NV];
+    };
+    // Rows past the end repeat the last one and write nothing.
+    auto load = [&](long long base, Row& w) {
+        const long long r = min(base + tid / LPR, static_cast<long long>(p.R - 1));
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        yr[u].get(h[u]);
+        for (int u = 0; u < NV; ++u) w.y[u] = Oct<TY>::template load<VEC>(p.y, r * p.ldy, 8 * (lane + LPR * u), D);
+        if (p.residual) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            h[u][e] = inside(u, e) ? h[u][e] : 0.f;
-            ss = fmaf(h[u][e], h[u][e], ss);
+            for (int u = 0; u < NV; ++u) w.r[u] = Oct<TR>::template load<VEC>(p.residual, r * p.ldr, 8 * (lane + LPR * u), D);
         }
-    }
-    float f0 = p.rs;
-    if (p.post_gamma) {
-        const float inv = 1.f / sqrtf(row_sum<LPR>(ss, sums[0]) / static_cast<float>(D) + p.eps);
-        if (p.rstd_y && live && lane == 0) p.rstd_y[row] = inv;
-        f0 *= inv;
-    }
-    ss = 0.f;
+        if (p.gate) {
+            const long long g = static_cast<unsigned>(r) / p.rows_per_gate;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) w.g[u] = Oct<TY>::template load<VEC>(p.gate, g * p.ldg, 8 * (lane + LPR * u), D);
+        }
+    };
+    const long long step = static_cast<long long>(gridDim.x) * SLOTS;
+    long long base = static_cast<long long>(blockIdx.x) * SLOTS;
+    Row cur;
+    load(base, cur);
+    // rs post_gamma scale, and gamma, of the lane's columns
+    float f[NV][8], gm[NV][8];
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-        float f[8], t[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = f0;
         const int c = 8 * (lane + LPR * u);
+        float t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[u][e] = p.rs;
         if (p.post_gamma) {
             Oct<TP>::template load<VEC>(p.post_gamma, 0, c, D).get(t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= t[e];
+            for (int e = 0; e < 8; ++e) f[u][e] *= t[e];
         }
         if (p.scale) {
             Oct<TP>::template load<VEC>(p.scale, 0, c, D).get(t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= t[e];
+            for (int e = 0; e < 8; ++e) f[u][e] *= t[e];
         }
-        if (p.gate) {
-            gr[u].get(t);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= act_f(t[e], p.act);
-        }
-        if (p.residual) {
-            rr[u].get(t);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            h[u][e] = inside(u, e) ? fmaf(f[e], h[u][e], t[e]) : 0.f;
-            ss = fmaf(h[u][e], h[u][e], ss);
-        }
-        if (p.h && live) store8<TR, VEC>(p.h, r * p.ldh, c, D, h[u]);
+        if (p.gamma) Oct<TP>::template load<VEC>(p.gamma, 0, c, D).get(gm[u]);
     }
-    if (!p.n && !p.codes && !p.rstd_h) return;
-    float inv = 1.f;
-    if (p.gamma) {
-        inv = 1.f / sqrtf(row_sum<LPR>(ss, sums[1]) / static_cast<float>(D) + p.eps);
-        if (p.rstd_h && live && lane == 0) p.rstd_h[row] = inv;
-    }
+
+    for (int parity = 0; base < p.R; parity ^= 1) {
+        Row next;
+        const bool more = base + step < p.R;
+        if (kAhead && more) load(base + step, next);
+        const long long r = base + tid / LPR;
+        const bool live = r < p.R;
+        float h[NV][8];
+        float ss = 0.f;
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-        const int c = 8 * (lane + LPR * u);
-        if (p.gamma) {
-            float t[8];
-            Oct<TP>::template load<VEC>(p.gamma, 0, c, D).get(t);
+        for (int u = 0; u < NV; ++u) {
+            cur.y[u].get(h[u]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[u][e] = inside(u, e) ? h[u][e] * inv * t[e] : 0.f;
-        }
-        if (p.n && live) store8<TY, VEC>(p.n, r * p.ldn, c, D, h[u]);
-        if (p.codes) {
-            const uint32_t s = Fp8<GDN_E4M3>::scale_byte(max16(amax8(h[u])));
-            const u32x2 w = Fp8<GDN_E4M3>::codes8(h[u], Fp8<GDN_E4M3>::inverse(s), s == 0xffu);
-            if (live && c / kBlk * kBlk < D) {  // a ragged last block is filled up with zero codes
-                *reinterpret_cast<u32x2*>(p.codes + r * p.ldc + c) = w;
-                if ((lane & 15) == 0) p.scales[static_cast<long long>(c / kBlk) * p.lds + row] = static_cast<uint8_t>(s);
+            for (int e = 0; e < 8; ++e) {
+                h[u][e] = inside(u, e) ? h[u][e] : 0.f;
+                ss = fmaf(h[u][e], h[u][e], ss);
             }
         }
+        float inv = 1.f;
+        if (p.post_gamma) {
+            inv = rstd_of(row_sum<LPR>(ss, sums[parity][0]), p.inv_D, p.eps);
+            if (p.rstd_y && live && lane == 0) p.rstd_y[r] = inv;
+        }
+        ss = 0.f;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            float t[8], a[8];
+            if (p.gate) {
+                cur.g[u].get(t);
+                act8<false>(t, p.act, a, nullptr);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) a[e] *= inv * f[u][e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) a[e] = inv * f[u][e];
+            }
+            if (p.residual) {
+                cur.r[u].get(t);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[u][e] = inside(u, e) ? fmaf(a[e], h[u][e], t[e]) : 0.f;
+                ss = fmaf(h[u][e], h[u][e], ss);
+            }
+            if (p.h && live) store8<TR, VEC>(p.h, r * p.ldh, 8 * (lane + LPR * u), D, h[u]);
+        }
+        inv = 1.f;
+        if (p.gamma) {
+            inv = rstd_of(row_sum<LPR>(ss, sums[parity][1]), p.inv_D, p.eps);
+            if (p.rstd_h && live && lane == 0) p.rstd_h[r] = inv;
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int c = 8 * (lane + LPR * u);
+            if (p.gamma) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[u][e] = inside(u, e) ? h[u][e] * inv * gm[u][e] : 0.f;
+            }
+            if (p.n && live) store8<TY, VEC>(p.n, r * p.ldn, c, D, h[u]);
+            if (p.codes) {
+                const uint32_t s = Fp8<GDN_E4M3>::scale_byte(max16(amax8(h[u])));
+                const u32x2 w = Fp8<GDN_E4M3>::codes8(h[u], Fp8<GDN_E4M3>::inverse(s), s == 0xffu);
+                if (live && c / kBlk * kBlk < D) {  // a ragged last block is filled up with zero codes
+                    *reinterpret_cast<u32x2*>(p.codes + r * p.ldc + c) = w;
+                    if ((lane & 15) == 0) p.scales[static_cast<long long>(c / kBlk) * p.lds + r] = static_cast<uint8_t>(s);
+                }
+            }
+        }
+        if (!more) break;
+        base += step;
+        if (kAhead)
+            cur = next;
+        else
+            load(base, cur);
     }
 }
+
+// Workgroups of 256 lanes or more on the chip at once: eight a CU of 256.
+int most_groups(int threads) { return 256 * (threads <= 256 ? 8 : threads <= 512 ? 4 : 2); }
 
 }  // namespace
 
@@ -156,11 +189,12 @@ extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residu
     p.h = h, p.n = n, p.ldh = ldh, p.ldn = ldn;
     p.codes = codes, p.scales = scales, p.ldc = ldc, p.lds = lds;
     p.rstd_y = rstd_y, p.rstd_h = rstd_h;
-    p.R = static_cast<int>(R), p.D = static_cast<int>(D);
+    p.R = static_cast<int>(R), p.D = static_cast<int>(D), p.inv_D = 1.f / static_cast<float>(D);
     return with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
         return with_row_shape(p.D, vec, [&](auto lpr, auto nv, auto v) {
-            constexpr int LPR = decltype(lpr)::value, slots = LPR <= 64 ? 256 / LPR : 1;
-            const dim3 grid((p.R + slots - 1) / slots), block(LPR <= 64 ? 256 : LPR);
+            constexpr int LPR = decltype(lpr)::value, threads = LPR <= 64 ? 256 : LPR;
+            const int all = (p.R + slots_of(LPR) - 1) / slots_of(LPR), most = most_groups(threads);
+            const dim3 grid(all < most ? all : most), block(threads);
             hipLaunchKernelGGL((gdn_block_norm_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
                                grid, block, 0, static_cast<hipStream_t>(stream), p);
             return gdn_host::check_launch("gdn_block_norm_kernel");

@@ -24,6 +24,7 @@ struct NormParams {
     long long ldc, lds;
     float *rstd_y, *rstd_h;
     int R, D;
+    float inv_D;
 };
 
 struct NormBwdParams {
@@ -37,6 +38,7 @@ struct NormBwdParams {
     float* part;                   // [groups * chunks][2][D] column sums
     int R, D;
     int group_rows, chunks;  // rows of a gate group, workgroups a group
+    float inv_D;
     int shared;              // rows share gate rows: the column sums leave the gate to the second launch
 };
 
@@ -104,36 +106,50 @@ __device__ __forceinline__ void store8(void* base, long long row, int c, int D, 
     }
 }
 
-// act(g) and its derivative.
-__device__ __forceinline__ float act_f(float g, int act) {
-    switch (act) {
-        case GDN_ACT_SIGMOID: return sigmoid_f(g);
-        case GDN_ACT_SILU: return g * sigmoid_f(g);
-        case GDN_ACT_TANH: return tanhf(g);
-        default: return g;
-    }
+// act(g) of eight gates and, with DERIV, its derivative, on the hardware's exp2
+// and reciprocal (about 1 ulp each).
+__device__ __forceinline__ float fast_sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
-__device__ __forceinline__ float act_grad_f(float g, int act) {
-    switch (act) {
-        case GDN_ACT_SIGMOID: {
-            const float s = sigmoid_f(g);
-            return s * (1.f - s);
+// Around 0, where 1 - 2 / (1 + e^2x) cancels, the Taylor series to x^11 (its next
+// term is 6e-8 of x at 0.4).
+__device__ __forceinline__ float fast_tanh(float x) {
+    const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x)), 1.f);
+    const float s = x * x;
+    float p = fmaf(s, -8.8632355e-3f, 2.1869488e-2f);
+    p = fmaf(s, p, -5.3968254e-2f);
+    p = fmaf(s, p, 1.3333333e-1f);
+    p = fmaf(s, p, -3.3333333e-1f);
+    return s < 0.16f ? fmaf(x * s, p, x) : far;
+}
+template <bool DERIV>
+__device__ __forceinline__ void act8(const float* g, int act, float* a, float* d) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        a[e] = g[e];
+        if (DERIV) d[e] = 1.f;
+    }
+    if (act == GDN_ACT_NONE) return;
+    if (act == GDN_ACT_TANH) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] = fast_tanh(g[e]);
+            if (DERIV) d[e] = fmaf(-a[e], a[e], 1.f);
         }
-        case GDN_ACT_SILU: {
-            const float s = sigmoid_f(g);
-            return s * (1.f + g * (1.f - s));
-        }
-        case GDN_ACT_TANH: {
-            const float t = tanhf(g);
-            return 1.f - t * t;
-        }
-        default: return 1.f;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float s = fast_sigmoid(g[e]);
+        const float ds = s * (1.f - s);
+        a[e] = act == GDN_ACT_SILU ? g[e] * s : s;
+        if (DERIV) d[e] = act == GDN_ACT_SILU ? fmaf(g[e], ds, s) : ds;
     }
 }
 
 // Sum over the LPR lanes of a row, the same in each of them, in a fixed order.
-// `slot`: the call's own LDS words (a kernel's calls use different ones, so one
-// barrier a call is enough within a row).
+// `slot`: the call's own LDS words (a row's calls and the next row's use
+// different ones, so one barrier a call is enough).
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
     if constexpr (LPR <= 32) {
@@ -154,30 +170,13 @@ __device__ __forceinline__ float row_sum(float v, float* slot) {
     }
 }
 
-// Lanes a row and vectors a lane for rows of D: f(LPR, NV).  Up to 512 columns
-// a part of a wave or a wave with one vector, up to 2048 a wave, above that a
-// workgroup with two vectors a lane.  Rows that 16-byte accesses do not fit run
-// on two of these forms.
+// Lanes a row and vectors a lane for rows of D: f(LPR, NV).  Up to 512 columns a
+// part of a wave or a wave, up to 8192 a workgroup, one vector a lane, so that
+// what a lane keeps over its rows (the parameters of its columns, in the backward
+// pass their column sums) stays in registers.  Rows that 16-byte accesses do not
+// fit run on three of these forms.
 template <class F>
 int with_row_shape(int D, bool vec, F&& f) {
-    using std::integral_constant;
-    if (!vec) {
-        if (D <= 2048) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{}, std::false_type{});
-        return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, std::false_type{});
-    }
-    if (D <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 2048) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{}, std::true_type{});
-    if (D <= 4096) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{}, std::true_type{});
-    if (D <= 8192) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{}, std::true_type{});
-    return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, std::true_type{});
-}
-
-// The same for the backward pass, which holds three times as much a column: one
-// vector a lane up to 8192 columns.
-template <class F>
-int with_row_shape_bwd(int D, bool vec, F&& f) {
     using std::integral_constant;
     if (!vec) {
         if (D <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, std::false_type{});
@@ -192,6 +191,8 @@ int with_row_shape_bwd(int D, bool vec, F&& f) {
     if (D <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 1>{}, std::true_type{});
     return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, std::true_type{});
 }
+// Rows a workgroup holds at a time.
+constexpr int slots_of(int lpr) { return lpr <= 64 ? 256 / lpr : 1; }
 
 constexpr int kMostColumns = 16384;
 
@@ -208,6 +209,9 @@ int with_types(int ty, int tr, int tp, F&& f) {
     if (tp == GDN_F32) return f(bf16(), bf16(), 0.f);
     return f(bf16(), bf16(), bf16());
 }
+
+// (mean + eps)^-1/2 of a sum of squares, 1 ulp.
+__device__ __forceinline__ float rstd_of(float sum, float inv_D, float eps) { return __builtin_amdgcn_rsqf(fmaf(sum, inv_D, eps)); }
 
 inline size_t type_bytes(int t) { return t == GDN_F32 ? 4 : 2; }
 

@@ -19,8 +19,9 @@
 namespace {
 
 template <class TY, class TR, class TP, int LPR, int NV, bool VEC>
-__global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_bwd_kernel(NormBwdParams p) {
-    constexpr int SLOTS = LPR <= 64 ? 256 / LPR : 1;
+__global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_per_eu(LPR >= 1024 ? 4 : sizeof(TR) == 2 ? 3 : 2))) void gdn_block_norm_bwd_kernel(NormBwdParams p) {
+    constexpr int SLOTS = slots_of(LPR);
+    constexpr bool kAhead = LPR < 1024;   // the next row is loaded a row ahead (sixteen waves have no registers for it)
     constexpr bool kShared = LPR <= 64;  // several rows at a time: their column sums meet in LDS
     __shared__ float sums[2][2][LPR > 64 ? LPR / 64 : 1];
     __shared__ float cols[kShared ? 2 * LPR * NV * 8 : 1];
@@ -29,96 +30,114 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_bwd_kern
     const int group = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
     const long long first = static_cast<long long>(group) * p.group_rows;
     const int end = static_cast<int>(min(first + p.group_rows, static_cast<long long>(p.R)));
+    const long long step = static_cast<long long>(p.chunks) * SLOTS;
     auto inside = [&](int u, int e) { return VEC ? 8 * (lane + LPR * u) < D : 8 * (lane + LPR * u) + e < D; };
 
-    float se[NV][8], sg[NV][8];
-#pragma unroll
-    for (int u = 0; u < NV; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) se[u][e] = sg[u][e] = 0.f;
-
-    int parity = 0;
-    for (long long base = first + static_cast<long long>(chunk) * SLOTS; base < end; base += static_cast<long long>(p.chunks) * SLOTS, parity ^= 1) {
-        const bool live = base + tid / LPR < end;
-        const long long r = live ? base + tid / LPR : end - 1;
-        Oct<TY> yr[NV], gr[NV], nr[NV];
-        Oct<TR> rr[NV], hr[NV];
+    struct Row {
+        Oct<TY> y[NV], dn[NV], g[NV];
+        Oct<TR> r[NV], dh[NV];
+        float ry, rh;
+    };
+    auto load = [&](long long base, Row& w) {
+        const long long r = min(base + tid / LPR, static_cast<long long>(end - 1));
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             const int c = 8 * (lane + LPR * u);
-            yr[u] = Oct<TY>::template load<VEC>(p.y, r * p.ldy, c, D);
-            if (p.dh) hr[u] = Oct<TR>::template load<VEC>(p.dh, r * p.lddh, c, D);
+            w.y[u] = Oct<TY>::template load<VEC>(p.y, r * p.ldy, c, D);
+            if (p.dh) w.dh[u] = Oct<TR>::template load<VEC>(p.dh, r * p.lddh, c, D);
+            if (p.residual && p.dn) w.r[u] = Oct<TR>::template load<VEC>(p.residual, r * p.ldr, c, D);
+            if (p.dn) w.dn[u] = Oct<TY>::template load<VEC>(p.dn, r * p.lddn, c, D);
+            if (p.gate && !p.shared) w.g[u] = Oct<TY>::template load<VEC>(p.gate, r * p.ldg, c, D);
         }
-        if (p.residual) {
-#pragma unroll
-            for (int u = 0; u < NV; ++u) rr[u] = Oct<TR>::template load<VEC>(p.residual, r * p.ldr, 8 * (lane + LPR * u), D);
-        }
-        if (p.dn) {
-#pragma unroll
-            for (int u = 0; u < NV; ++u) nr[u] = Oct<TY>::template load<VEC>(p.dn, r * p.lddn, 8 * (lane + LPR * u), D);
-        }
-        if (p.gate) {
-            const long long g = static_cast<unsigned>(r) / p.rows_per_gate;
-#pragma unroll
-            for (int u = 0; u < NV; ++u) gr[u] = Oct<TY>::template load<VEC>(p.gate, g * p.ldg, 8 * (lane + LPR * u), D);
-        }
-        const float ry = p.rstd_y ? p.rstd_y[r] : 1.f, rh = p.rstd_h ? p.rstd_h[r] : 1.f;
+        w.ry = p.rstd_y ? p.rstd_y[r] : 1.f;
+        w.rh = p.rstd_h ? p.rstd_h[r] : 1.f;
+    };
+    long long base = first + static_cast<long long>(chunk) * SLOTS;
+    Row cur;
+    if (base < end) load(base, cur);
 
-        // dH: dh, and through the second norm dn
-        float dH[NV][8], hn[NV][8];
+    // The lane's columns: rs post_gamma scale (times a shared gate's act), gamma,
+    // the sums of e a (of e with a shared gate) and of dn hn.
+    float ps[NV][8], gm[NV][8], se[NV][8], sg[NV][8];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int c = 8 * (lane + LPR * u);
+        float t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ps[u][e] = p.rs;
+            gm[u][e] = se[u][e] = sg[u][e] = 0.f;
+        }
+        if (p.post_gamma) {
+            Oct<TP>::template load<VEC>(p.post_gamma, 0, c, D).get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ps[u][e] *= t[e];
+        }
+        if (p.scale) {
+            Oct<TP>::template load<VEC>(p.scale, 0, c, D).get(t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ps[u][e] *= t[e];
+        }
+        if (p.gate && p.shared) {
+            float a[8];
+            Oct<TY>::template load<VEC>(p.gate, group * p.ldg, c, D).get(t);
+            act8<false>(t, p.act, a, nullptr);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ps[u][e] *= a[e];
+        }
+        if (p.gamma) Oct<TP>::template load<VEC>(p.gamma, 0, c, D).get(gm[u]);
+    }
+
+    for (int parity = 0; base < end; parity ^= 1) {
+        Row next;
+        const bool more = base + step < end;
+        if (kAhead && more) load(base + step, next);
+        const long long r = base + tid / LPR;
+        const bool live = r < end;
+
+        // The gate's act (a, of a gate a token) and derivative (da), y rstd_y.
+        float a[NV][8], da[NV][8], yn[NV][8], dH[NV][8], hn[NV][8];
         float m = 0.f;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
+            float t[8];
+            if (p.gate && !p.shared) {
+                cur.g[u].get(t);
+                act8<true>(t, p.act, a[u], da[u]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) a[u][e] = 1.f;
+            }
+            cur.y[u].get(yn[u]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) yn[u][e] = inside(u, e) ? yn[u][e] * cur.ry : 0.f;
             if (p.dh) {
-                hr[u].get(dH[u]);
+                cur.dh[u].get(dH[u]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dH[u][e] = 0.f;
             }
-        }
-        if (p.dn) {
-#pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                const int c = 8 * (lane + LPR * u);
-                float f[8], t[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = p.rs * ry;
-                if (p.post_gamma) {
-                    Oct<TP>::template load<VEC>(p.post_gamma, 0, c, D).get(t);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= t[e];
-                }
-                if (p.scale) {
-                    Oct<TP>::template load<VEC>(p.scale, 0, c, D).get(t);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= t[e];
-                }
-                if (p.gate) {
-                    gr[u].get(t);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= act_f(t[e], p.act);
-                }
-                float yv[8];
-                yr[u].get(yv);
+            if (p.dn) {  // h again, and what comes through the second norm
+                float dn[8];
                 if (p.residual) {
-                    rr[u].get(t);
+                    cur.r[u].get(t);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) t[e] = 0.f;
                 }
-                float gm[8], dn[8];
-                Oct<TP>::template load<VEC>(p.gamma, 0, c, D).get(gm);
-                nr[u].get(dn);
+                cur.dn[u].get(dn);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    hn[u][e] = fmaf(f[e], yv[e], t[e]) * rh;
-                    const float tt = inside(u, e) ? dn[e] * gm[e] : 0.f;
+                    hn[u][e] = fmaf(ps[u][e] * a[u][e], yn[u][e], t[e]) * cur.rh;
+                    const float tt = dn[e] * gm[u][e];
                     if (inside(u, e)) m = fmaf(tt, hn[u][e], m);
-                    if (live && inside(u, e)) sg[u][e] = fmaf(dn[e], hn[u][e], sg[u][e]);
-                    dH[u][e] = fmaf(tt, rh, dH[u][e]);
+                    if (live) sg[u][e] = fmaf(dn[e], hn[u][e], sg[u][e]);
+                    dH[u][e] = fmaf(tt, cur.rh, dH[u][e]);
                 }
             }
-            m = row_sum<LPR>(m, sums[parity][0]) / static_cast<float>(D) * rh;
+        }
+        if (p.dn) {
+            m = row_sum<LPR>(m, sums[parity][0]) * p.inv_D * cur.rh;
 #pragma unroll
             for (int u = 0; u < NV; ++u)
 #pragma unroll
@@ -129,50 +148,38 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_bwd_kern
             for (int u = 0; u < NV; ++u) store8<TR, VEC>(p.dresidual, r * D, 8 * (lane + LPR * u), D, dH[u]);
         }
 
-        // dgate, the column sums, and z
+        // dgate, the column sums, and z (which takes dH's place)
         float q = 0.f;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            const int c = 8 * (lane + LPR * u);
-            float ps[8], t[8], yv[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ps[e] = 1.f;
-            if (p.post_gamma) Oct<TP>::template load<VEC>(p.post_gamma, 0, c, D).get(ps);
-            if (p.scale) {
-                Oct<TP>::template load<VEC>(p.scale, 0, c, D).get(t);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ps[e] *= t[e];
-            }
-            yr[u].get(yv);
-            if (p.gate) gr[u].get(t);
             float dg[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float yn = yv[e] * ry;
-                const float ev = p.rs * dH[u][e] * yn;
-                const float a = p.gate ? act_f(t[e], p.act) : 1.f;
-                if (p.dgate) dg[e] = ev * ps[e] * act_grad_f(t[e], p.act);
-                if (live && inside(u, e)) se[u][e] += p.shared ? ev : ev * a;
-                const float z = dH[u][e] * p.rs * ps[e] * a;
-                if (inside(u, e)) q = fmaf(z, yn, q);
-                dH[u][e] = z;
+                const float ev = dH[u][e] * yn[u][e];  // without rs, which the sums' launch puts in
+                if (p.dgate) dg[e] = ev * ps[u][e] * da[u][e];
+                if (live) se[u][e] = fmaf(ev, a[u][e], se[u][e]);
+                dH[u][e] *= ps[u][e] * a[u][e];
+                if (inside(u, e)) q = fmaf(dH[u][e], yn[u][e], q);
             }
-            if (p.dgate && live) store8<TY, VEC>(p.dgate, r * D, c, D, dg);
+            if (p.dgate && live) store8<TY, VEC>(p.dgate, r * D, 8 * (lane + LPR * u), D, dg);
         }
         if (p.rstd_y) {
-            q = row_sum<LPR>(q, sums[parity][1]) / static_cast<float>(D);
+            q = row_sum<LPR>(q, sums[parity][1]) * p.inv_D;
 #pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                float yv[8];
-                yr[u].get(yv);
+            for (int u = 0; u < NV; ++u)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dH[u][e] = ry * (dH[u][e] - yv[e] * ry * q);
-            }
+                for (int e = 0; e < 8; ++e) dH[u][e] = cur.ry * fmaf(-yn[u][e], q, dH[u][e]);
         }
         if (live) {
 #pragma unroll
             for (int u = 0; u < NV; ++u) store8<TY, VEC>(p.dy, r * D, 8 * (lane + LPR * u), D, dH[u]);
         }
+        if (!more) break;
+        base += step;
+        if (kAhead)
+            cur = next;
+        else
+            load(base, cur);
     }
     if (!p.part) return;
 
@@ -220,13 +227,14 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_bwd_kern
     }
 }
 
-// Adds the sums of `chunks` workgroups of each group (blockIdx.y), 32 columns a
-// workgroup, and writes what follows from them: the gradient of a shared gate
-// row, and either the parameters' gradients (one group) or the group's part of
-// them (part2).
+// Adds the sums of `chunks` workgroups of each group (blockIdx.y), 16 columns a
+// workgroup, 64 at a time, and writes what follows from them: the gradient of a
+// shared gate row, and either the parameters' gradients (one group) or the
+// group's part of them (part2).
 struct SumParams {
     const float* part;
     int chunks, D;
+    float rs;
     const void *gate, *post_gamma, *scale;
     long long ldg;
     int act;
@@ -235,15 +243,15 @@ struct SumParams {
 };
 
 template <class TY, class TP>
-__global__ __launch_bounds__(256) void gdn_block_norm_sum_kernel(SumParams p) {
-    __shared__ float lds[2][8][32];
-    const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, d = blockIdx.x * 32 + col, D = p.D;
+__global__ __launch_bounds__(1024) void gdn_block_norm_sum_kernel(SumParams p) {
+    __shared__ float lds[2][64][17];
+    const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, d = blockIdx.x * 16 + col, D = p.D;
     const long long g = blockIdx.y;
     float e = 0.f, s = 0.f;
     if (d < D) {
         const float* src = p.part + static_cast<size_t>(g) * p.chunks * 2 * D + d;
 #pragma unroll 4
-        for (int i = lane; i < p.chunks; i += 8) {
+        for (int i = lane; i < p.chunks; i += 64) {
             e += src[static_cast<size_t>(i) * 2 * D];
             s += src[static_cast<size_t>(i) * 2 * D + D];
         }
@@ -251,19 +259,22 @@ __global__ __launch_bounds__(256) void gdn_block_norm_sum_kernel(SumParams p) {
     lds[0][lane][col] = e;
     lds[1][lane][col] = s;
     __syncthreads();
-    if (lane > 0 || d >= D) return;
-    e = s = 0.f;
+    if (threadIdx.x >= 32) return;
+    float sum = 0.f;  // threads 0 .. 15 of e, 16 .. 31 of s
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        e += lds[0][i][col];
-        s += lds[1][i][col];
-    }
+    for (int i = 0; i < 64; ++i) sum += lds[threadIdx.x >> 4][i][col];
+    s = __shfl(sum, 16 + col);
+    if (threadIdx.x >= 16 || d >= D) return;
+    e = sum * p.rs;
     const float pg = p.post_gamma ? static_cast<float>(static_cast<const TP*>(p.post_gamma)[d]) : 1.f;
     const float sc = p.scale ? static_cast<float>(static_cast<const TP*>(p.scale)[d]) : 1.f;
     if (p.gate) {
-        const float x = static_cast<float>(static_cast<const TY*>(p.gate)[g * p.ldg + d]);
-        if (p.dgate) static_cast<TY*>(p.dgate)[g * D + d] = static_cast<TY>(e * pg * sc * act_grad_f(x, p.act));
-        e *= act_f(x, p.act);
+        float x[8], a[8], da[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<const TY*>(p.gate)[g * p.ldg + d]);
+        act8<true>(x, p.act, a, da);
+        if (p.dgate) static_cast<TY*>(p.dgate)[g * D + d] = static_cast<TY>(e * pg * sc * da[0]);
+        e *= a[0];
     }
     if (p.part2) {
         p.part2[static_cast<size_t>(g) * 2 * D + d] = e;
@@ -352,10 +363,10 @@ extern "C" int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* 
         p.rstd_y = rstd_y, p.rstd_h = rstd_h;
         p.dresidual = dresidual, p.dy = dy, p.dgate = shared ? nullptr : dgate;
         p.part = part;
-        p.R = static_cast<int>(R), p.D = static_cast<int>(D);
+        p.R = static_cast<int>(R), p.D = static_cast<int>(D), p.inv_D = 1.f / static_cast<float>(D);
         p.group_rows = q.group_rows, p.chunks = q.chunks, p.shared = shared;
         const int st = with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
-            return with_row_shape_bwd(p.D, vec, [&](auto lpr, auto nv, auto v) {
+            return with_row_shape(p.D, vec, [&](auto lpr, auto nv, auto v) {
                 constexpr int LPR = decltype(lpr)::value;
                 const dim3 grid(static_cast<unsigned>(q.groups * q.chunks)), block(LPR <= 64 ? 256 : LPR);
                 hipLaunchKernelGGL((gdn_block_norm_bwd_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
@@ -368,6 +379,7 @@ extern "C" int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* 
         return GDN_OK;
     }
     SumParams t = {};
+    t.rs = residual_scale;
     t.part = part, t.chunks = R > 0 ? q.chunks : 0, t.D = static_cast<int>(D);
     t.post_gamma = post_gamma, t.scale = scale, t.act = act, t.dpost_gamma = dpost_gamma, t.dscale = dscale, t.dgamma = dgamma;
     if (shared && R > 0) t.gate = gate, t.ldg = ldg, t.dgate = dgate;
@@ -375,13 +387,13 @@ extern "C" int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* 
     t.part2 = part2;
     return with_types(type_y, type_r, type_p, [&](auto ty, auto, auto tp) {
         const auto launch = [&](long long groups) {
-            hipLaunchKernelGGL((gdn_block_norm_sum_kernel<decltype(ty), decltype(tp)>), dim3((t.D + 31) / 32, static_cast<unsigned>(groups)),
-                               dim3(256), 0, s, t);
+            hipLaunchKernelGGL((gdn_block_norm_sum_kernel<decltype(ty), decltype(tp)>), dim3((t.D + 15) / 16, static_cast<unsigned>(groups)),
+                               dim3(1024), 0, s, t);
             return gdn_host::check_launch("gdn_block_norm_sum_kernel");
         };
         const int st = launch(q.groups);
         if (st != GDN_OK || !part2) return st;
-        t.part = part2, t.chunks = static_cast<int>(q.groups), t.part2 = nullptr, t.gate = nullptr, t.dgate = nullptr;
+        t.part = part2, t.chunks = static_cast<int>(q.groups), t.part2 = nullptr, t.rs = 1.f, t.gate = nullptr, t.dgate = nullptr;
         return launch(1);
     });
 }
