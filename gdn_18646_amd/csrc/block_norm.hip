@@ -8,9 +8,11 @@
 //
 // What bounds it: HBM for many rows (each input read once, each output written
 // once, two row sums between them that never leave the registers), the one
-// chain of loads, sums and stores for a few.  A workgroup walks rows with the
-// parameters of its columns in registers, and the next row's loads are under way
-// while a row is worked on.
+// chain of loads, sums and stores for a few.  Rows of up to 4096 columns have a
+// workgroup each or share one; rows above that keep sixteen waves busy alone, and
+// a workgroup a CU walks them, the next row's loads under way while a row is
+// worked on (4096 x 8192: 78 us against 102 with a workgroup a row; walking rows
+// of 2048 columns instead took 70 against 64).
 #include "block_norm.hpp"
 #include "fp8_blocks.hpp"
 
@@ -19,7 +21,8 @@ namespace {
 template <class TY, class TR, class TP, int LPR, int NV, bool VEC>
 __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(NormParams p) {
     constexpr int SLOTS = slots_of(LPR);
-    constexpr bool kAhead = NV == 1;  // the next row is loaded a row ahead (with two vectors a lane it does not fit)
+    constexpr bool kWalk = LPR == 1024;         // a workgroup walks rows
+    constexpr bool kAhead = kWalk && NV == 1;  // the next one is loaded a row ahead (with two vectors a lane it does not fit)
     __shared__ float sums[2][2][LPR > 64 ? LPR / 64 : 1];
     const int tid = threadIdx.x, lane = tid % LPR;
     const int D = p.D;
@@ -71,7 +74,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
 
     for (int parity = 0; base < p.R; parity ^= 1) {
         Row next;
-        const bool more = base + step < p.R;
+        const bool more = kWalk && base + step < p.R;
         if (kAhead && more) load(base + step, next);
         const long long r = base + tid / LPR;
         const bool live = r < p.R;
@@ -148,9 +151,6 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
     }
 }
 
-// Workgroups of 256 lanes or more on the chip at once: eight a CU of 256.
-int most_groups(int threads) { return 256 * (threads <= 256 ? 8 : threads <= 512 ? 4 : 2); }
-
 }  // namespace
 
 extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residual, int64_t ldr, const void* gate,
@@ -191,10 +191,10 @@ extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residu
     p.rstd_y = rstd_y, p.rstd_h = rstd_h;
     p.R = static_cast<int>(R), p.D = static_cast<int>(D), p.inv_D = 1.f / static_cast<float>(D);
     return with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
-        return with_row_shape(p.D, vec, [&](auto lpr, auto nv, auto v) {
+        return with_row_shape<false>(p.D, vec, [&](auto lpr, auto nv, auto v) {
             constexpr int LPR = decltype(lpr)::value, threads = LPR <= 64 ? 256 : LPR;
-            const int all = (p.R + slots_of(LPR) - 1) / slots_of(LPR), most = most_groups(threads);
-            const dim3 grid(all < most ? all : most), block(threads);
+            const int all = (p.R + slots_of(LPR) - 1) / slots_of(LPR);
+            const dim3 grid(LPR == 1024 && all > 256 ? 256 : all), block(threads);
             hipLaunchKernelGGL((gdn_block_norm_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
                                grid, block, 0, static_cast<hipStream_t>(stream), p);
             return gdn_host::check_launch("gdn_block_norm_kernel");

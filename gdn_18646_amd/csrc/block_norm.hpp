@@ -56,8 +56,9 @@ struct Oct {
     u32x4 w[sizeof(T) / 2];
 
     // Columns c .. c + 7 of the row at `row` of D columns; columns past the end
-    // repeat one inside it (the callers drop them).  VEC: rows and D allow
-    // 16-byte loads.
+    // repeat one inside it (the callers drop them).  VEC: rows lie at multiples of
+    // 16 bytes and D is one of 8; else the lane with the row's end takes it element
+    // by element.
     template <bool VEC>
     __device__ __forceinline__ static Oct load(const void* base, long long row, int c, int D) {
         const T* p = static_cast<const T*>(base) + row;
@@ -66,12 +67,13 @@ struct Oct {
             const u32x4* q = reinterpret_cast<const u32x4*>(p + (c < D ? c : 0));
 #pragma unroll
             for (unsigned i = 0; i < sizeof(T) / 2; ++i) o.w[i] = q[i];
+        } else if (c + 8 <= D) {
+            __builtin_memcpy(o.w, p + c, 8 * sizeof(T));  // 16-byte loads at any address
         } else {
             T e[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) e[i] = p[min(c + i, D - 1)];
-#pragma unroll
-            for (unsigned i = 0; i < sizeof(T) / 2; ++i) o.w[i] = reinterpret_cast<const u32x4*>(e)[i];
+            __builtin_memcpy(o.w, e, 8 * sizeof(T));
         }
         return o;
     }
@@ -88,17 +90,20 @@ struct Oct {
 template <class T, bool VEC>
 __device__ __forceinline__ void store8(void* base, long long row, int c, int D, const float* f) {
     T* p = static_cast<T*>(base) + row;
+    u32x4 w[sizeof(T) / 2];
+    if constexpr (sizeof(T) == 2) {
+        w[0] = u32x4{pack2_bf16(f[0], f[1]), pack2_bf16(f[2], f[3]), pack2_bf16(f[4], f[5]), pack2_bf16(f[6], f[7])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(f[i]);
+    }
     if constexpr (VEC) {
         if (c >= D) return;
         u32x4* q = reinterpret_cast<u32x4*>(p + c);
-        if constexpr (sizeof(T) == 2) {
-            q[0] = u32x4{pack2_bf16(f[0], f[1]), pack2_bf16(f[2], f[3]), pack2_bf16(f[4], f[5]), pack2_bf16(f[6], f[7])};
-        } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                q[i] = u32x4{__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
-                             __float_as_uint(f[4 * i + 3])};
-        }
+        for (unsigned i = 0; i < sizeof(T) / 2; ++i) q[i] = w[i];
+    } else if (c + 8 <= D) {
+        __builtin_memcpy(p + c, w, 8 * sizeof(T));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -171,25 +176,32 @@ __device__ __forceinline__ float row_sum(float v, float* slot) {
 }
 
 // Lanes a row and vectors a lane for rows of D: f(LPR, NV).  Up to 512 columns a
-// part of a wave or a wave, up to 8192 a workgroup, one vector a lane, so that
-// what a lane keeps over its rows (the parameters of its columns, in the backward
-// pass their column sums) stays in registers.  Rows that 16-byte accesses do not
-// fit run on three of these forms.
-template <class F>
+// part of a wave or a wave, above that a workgroup, one vector a lane as far as
+// that goes (the backward pass, which holds three times as much, has two a lane
+// from 4096 columns on, sixteen waves having too few registers).  Rows that
+// 16-byte accesses do not fit run on some of these forms.
+template <bool BWD, class F>
 int with_row_shape(int D, bool vec, F&& f) {
     using std::integral_constant;
-    if (!vec) {
-        if (D <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, std::false_type{});
-        if (D <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 1>{}, std::false_type{});
-        return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, std::false_type{});
-    }
-    if (D <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 4096) return f(integral_constant<int, 512>{}, integral_constant<int, 1>{}, std::true_type{});
-    if (D <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 1>{}, std::true_type{});
-    return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, std::true_type{});
+    const auto shape = [&](auto v) {
+        if constexpr (decltype(v)::value) {
+            if (D <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, v);
+            if (D <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, v);
+        }
+        if (D <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, v);
+        if (D <= 1024) return f(integral_constant<int, 128>{}, integral_constant<int, 1>{}, v);
+        if (D <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, v);
+        if constexpr (decltype(v)::value) {
+            if (D <= 4096) return f(integral_constant<int, 512>{}, integral_constant<int, 1>{}, v);
+        }
+        if constexpr (BWD) {
+            if (D <= 8192) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{}, v);
+        } else {
+            if (D <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 1>{}, v);
+        }
+        return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, v);
+    };
+    return vec ? shape(std::true_type{}) : shape(std::false_type{});
 }
 // Rows a workgroup holds at a time.
 constexpr int slots_of(int lpr) { return lpr <= 64 ? 256 / lpr : 1; }

@@ -19,12 +19,13 @@
 namespace {
 
 template <class TY, class TR, class TP, int LPR, int NV, bool VEC>
-__global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_per_eu(LPR >= 1024 ? 4 : sizeof(TR) == 2 ? 3 : 2))) void gdn_block_norm_bwd_kernel(NormBwdParams p) {
+__global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_per_eu(LPR >= 1024 ? 4 : VEC && NV == 1 && LPR >= 128 && sizeof(TR) == 2 ? 3 : 2))) void gdn_block_norm_bwd_kernel(NormBwdParams p) {
     constexpr int SLOTS = slots_of(LPR);
-    constexpr bool kAhead = LPR < 1024;   // the next row is loaded a row ahead (sixteen waves have no registers for it)
+    constexpr bool kAhead = NV == 1;  // the next row is loaded a row ahead (with two vectors a lane it does not fit)
     constexpr bool kShared = LPR <= 64;  // several rows at a time: their column sums meet in LDS
+    constexpr bool kLds = LPR == 1024;   // the lane's column sums lie in LDS, and its parameters are read a row
     __shared__ float sums[2][2][LPR > 64 ? LPR / 64 : 1];
-    __shared__ float cols[kShared ? 2 * LPR * NV * 8 : 1];
+    __shared__ __attribute__((aligned(16))) float cols[kShared || kLds ? 2 * LPR * NV * 8 : 1];
     const int tid = threadIdx.x, lane = tid % LPR;
     const int D = p.D;
     const int group = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
@@ -58,15 +59,14 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
 
     // The lane's columns: rs post_gamma scale (times a shared gate's act), gamma,
     // the sums of e a (of e with a shared gate) and of dn hn.
-    float ps[NV][8], gm[NV][8], se[NV][8], sg[NV][8];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
+    float ps[NV][8], gm[NV][8], se[kLds ? 1 : NV][8], sg[kLds ? 1 : NV][8];
+    auto params = [&](int u) {
         const int c = 8 * (lane + LPR * u);
         float t[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             ps[u][e] = p.rs;
-            gm[u][e] = se[u][e] = sg[u][e] = 0.f;
+            gm[u][e] = 0.f;
         }
         if (p.post_gamma) {
             Oct<TP>::template load<VEC>(p.post_gamma, 0, c, D).get(t);
@@ -86,6 +86,29 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
             for (int e = 0; e < 8; ++e) ps[u][e] *= a[e];
         }
         if (p.gamma) Oct<TP>::template load<VEC>(p.gamma, 0, c, D).get(gm[u]);
+    };
+    // Adds v to the sums `which` (0: e a, 1: dn hn) of vector u's columns.
+    auto add = [&](int which, int u, const float* v) {
+        if constexpr (kLds) {
+            f32x4* const at = reinterpret_cast<f32x4*>(cols + ((which * NV + u) * LPR + lane) * 8);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) at[i] += f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) (which ? sg : se)[u][e] += v[e];
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if constexpr (kLds) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                reinterpret_cast<f32x4*>(cols + (((i >> 1) * NV + u) * LPR + lane) * 8)[i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
+            params(u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) se[u][e] = sg[u][e] = 0.f;
+        }
     }
 
     for (int parity = 0; base < end; parity ^= 1) {
@@ -100,6 +123,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
         float m = 0.f;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
+            if constexpr (kLds) params(u);
             float t[8];
             if (p.gate && !p.shared) {
                 cur.g[u].get(t);
@@ -131,9 +155,10 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
                     hn[u][e] = fmaf(ps[u][e] * a[u][e], yn[u][e], t[e]) * cur.rh;
                     const float tt = dn[e] * gm[u][e];
                     if (inside(u, e)) m = fmaf(tt, hn[u][e], m);
-                    if (live) sg[u][e] = fmaf(dn[e], hn[u][e], sg[u][e]);
+                    dn[e] = live ? dn[e] * hn[u][e] : 0.f;
                     dH[u][e] = fmaf(tt, cur.rh, dH[u][e]);
                 }
+                add(1, u, dn);
             }
         }
         if (p.dn) {
@@ -152,15 +177,16 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
         float q = 0.f;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            float dg[8];
+            float dg[8], ea[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float ev = dH[u][e] * yn[u][e];  // without rs, which the sums' launch puts in
                 if (p.dgate) dg[e] = ev * ps[u][e] * da[u][e];
-                if (live) se[u][e] = fmaf(ev, a[u][e], se[u][e]);
+                ea[e] = live ? ev * a[u][e] : 0.f;
                 dH[u][e] *= ps[u][e] * a[u][e];
                 if (inside(u, e)) q = fmaf(dH[u][e], yn[u][e], q);
             }
+            add(0, u, ea);
             if (p.dgate && live) store8<TY, VEC>(p.dgate, r * D, 8 * (lane + LPR * u), D, dg);
         }
         if (p.rstd_y) {
@@ -193,8 +219,8 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
             for (int e = 0; e < 8; ++e)
                 if (inside(u, e)) {
                     const int c = 8 * (lane + LPR * u) + e;
-                    out[c] = se[u][e];
-                    out[D + c] = sg[u][e];
+                    out[c] = kLds ? cols[(u * LPR + lane) * 8 + e] : se[kLds ? 0 : u][e];
+                    out[D + c] = kLds ? cols[((NV + u) * LPR + lane) * 8 + e] : sg[kLds ? 0 : u][e];
                 }
     } else {
         constexpr int kC = LPR * NV * 8;
@@ -286,8 +312,10 @@ __global__ __launch_bounds__(1024) void gdn_block_norm_sum_kernel(SumParams p) {
     if (p.dgamma) static_cast<TP*>(p.dgamma)[d] = static_cast<TP>(s);
 }
 
-// How R rows with a gate row each `per` are split over workgroups: 512 of them
-// in all (two a CU) while each has a row for every one of its slots.
+// How R rows with a gate row each `per` are split over workgroups: 512 of them in
+// all, two a CU, or 256 for rows of over 2048 columns, while each has a row for
+// every one of its slots (16384 x 2048: 123 us with 512, 172 with 256, 138 with
+// 1024; 8192 x 4096: 131 with 256, 138 with 512).
 struct Plan {
     long long groups;
     int group_rows, chunks;
@@ -299,7 +327,7 @@ Plan plan_rows(long long R, long long D, long long per) {
     Plan q;
     q.group_rows = static_cast<int>(rows);
     q.groups = shared ? (R + rows - 1) / rows : 1;
-    const long long most = (512 + q.groups - 1) / q.groups, need = (rows + slots - 1) / slots;
+    const long long all = D <= 2048 ? 512 : 256, most = (all + q.groups - 1) / q.groups, need = (rows + slots - 1) / slots;
     q.chunks = static_cast<int>(need < most ? need : most);
     return q;
 }
@@ -366,7 +394,7 @@ extern "C" int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* 
         p.R = static_cast<int>(R), p.D = static_cast<int>(D), p.inv_D = 1.f / static_cast<float>(D);
         p.group_rows = q.group_rows, p.chunks = q.chunks, p.shared = shared;
         const int st = with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
-            return with_row_shape(p.D, vec, [&](auto lpr, auto nv, auto v) {
+            return with_row_shape<true>(p.D, vec, [&](auto lpr, auto nv, auto v) {
                 constexpr int LPR = decltype(lpr)::value;
                 const dim3 grid(static_cast<unsigned>(q.groups * q.chunks)), block(LPR <= 64 ? 256 : LPR);
                 hipLaunchKernelGGL((gdn_block_norm_bwd_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
