@@ -2,6 +2,7 @@
 //   rmsnorm.block_norm, rmsnorm.block_norm_backward, proj.fp8_quantize, proj.fp8_matmul
 // Errors surface as RuntimeError; launches go to torch's current HIP stream of
 // the tensors' device.
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -119,11 +120,18 @@ Operands operands(const Tensor& y, const Opt& residual, const Opt& gate, const O
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// An output on t's device, without the dispatcher's way round (a third of a
+// small call's host time).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& t) {
+    return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
+}
+
 // Scales of M rows in KB blocks as the product reads them: a block's adjacent.
-Tensor down_columns(int64_t M, int64_t KB, const at::TensorOptions& o, at::ScalarType type) {
+Tensor down_columns(int64_t M, int64_t KB, at::ScalarType type, const Tensor& t) {
     const int64_t Mp = up(M, 16);
-    auto t = at::empty_strided({Mp, KB}, {1, Mp}, o.dtype(type));
-    return Mp == M ? t : t.narrow(0, 0, M);
+    Tensor s = at::detail::empty_strided_cuda({Mp, KB}, {1, Mp}, type, t.device());
+    if (Mp != M) s.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({M, KB}), at::IntArrayRef({1, Mp}));
+    return s;
 }
 
 std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gate, const Opt& post_gamma, const Opt& gamma,
@@ -136,27 +144,27 @@ std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gat
     std::vector<Opt> out(stats ? 6 : 4);
     Rows h, n;
     if (store_h) {
-        out[0] = inplace ? *residual : at::empty(y.sizes(), (given(residual) ? *residual : y).options());
+        out[0] = inplace ? *residual : fresh(y.sizes(), (given(residual) ? *residual : y).scalar_type(), y);
         h = rows_of(*out[0], "h");
     }
     if (given(gamma) && !quantize) {
-        out[1] = at::empty(y.sizes(), y.options());
+        out[1] = fresh(y.sizes(), y.scalar_type(), y);
         n = rows_of(*out[1], "n");
     }
     uint8_t *codes = nullptr, *scales = nullptr;
     int64_t ldc = 0, lds = 0;
     if (quantize) {
         ldc = up(o.D, 128);
-        out[2] = at::empty({o.R, ldc}, y.options().dtype(at::kFloat8_e4m3fn));
-        out[3] = down_columns(o.R, ldc / 128, y.options(), at::kFloat8_e8m0fnu);
+        out[2] = fresh({o.R, ldc}, at::kFloat8_e4m3fn, y);
+        out[3] = down_columns(o.R, ldc / 128, at::kFloat8_e8m0fnu, y);
         codes = static_cast<uint8_t*>(out[2]->data_ptr());
         scales = static_cast<uint8_t*>(out[3]->data_ptr());
         lds = up(o.R, 16);
     }
     float *ry = nullptr, *rh = nullptr;
     if (stats) {
-        if (given(post_gamma)) ry = (out[4] = at::empty({o.R}, y.options().dtype(at::kFloat)))->data_ptr<float>();
-        if (given(gamma)) rh = (out[5] = at::empty({o.R}, y.options().dtype(at::kFloat)))->data_ptr<float>();
+        if (given(post_gamma)) ry = (out[4] = fresh({o.R}, at::kFloat, y))->data_ptr<float>();
+        if (given(gamma)) rh = (out[5] = fresh({o.R}, at::kFloat, y))->data_ptr<float>();
     }
     if (o.R == 0) return out;
     check_status(gdn_block_norm_hip(o.y.ptr, o.y.ld, o.residual.ptr, o.residual.ld, o.gate.ptr, o.gate.ld, o.rows_per_gate,
@@ -196,9 +204,9 @@ std::vector<Opt> block_norm_backward(const Opt& dh, const Opt& dn, const Tensor&
     const float* const rh = rstd(rstd_h, normed, "rstd_h");
     const c10::DeviceGuard guard(y.device());
     std::vector<Opt> out(6);
-    auto like = [&](const Opt& t) { return at::empty(t->sizes(), t->options()); };
+    auto like = [&](const Opt& t) { return fresh(t->sizes(), t->scalar_type(), y); };
     if (given(residual)) out[0] = like(residual);
-    out[1] = at::empty(y.sizes(), y.options());
+    out[1] = fresh(y.sizes(), y.scalar_type(), y);
     if (given(gate)) out[2] = like(gate);
     if (given(post_gamma)) out[3] = like(post_gamma);
     if (given(gamma)) out[4] = normed ? like(gamma) : at::zeros(gamma->sizes(), gamma->options());
@@ -210,7 +218,7 @@ std::vector<Opt> block_norm_backward(const Opt& dh, const Opt& dn, const Tensor&
     }
     const bool sums = given(post_gamma) || normed || given(scale) || (given(gate) && o.rows_per_gate > 1);
     const size_t bytes = sums ? gdn_block_norm_bwd_workspace_bytes(o.R, o.D, given(gate) ? o.rows_per_gate : 1) : 0;
-    auto ws = at::empty({static_cast<int64_t>(bytes)}, y.options().dtype(at::kByte));
+    const Tensor ws = fresh({static_cast<int64_t>(bytes)}, at::kByte, y);
     auto ptr = [&](int i) { return given(out[i]) ? out[i]->data_ptr() : nullptr; };
     check_status(gdn_block_norm_bwd_hip(rdh.ptr, rdh.ld, rdn.ptr, rdn.ld, o.y.ptr, o.y.ld, o.residual.ptr, o.residual.ld,
                                         o.gate.ptr, o.gate.ld, o.rows_per_gate, o.post_gamma, normed ? o.gamma : nullptr, o.scale,
@@ -239,13 +247,13 @@ std::vector<Tensor> fp8_quantize(const Tensor& x, int64_t block_rows, at::Scalar
     uint8_t* ptr[4] = {};
     int64_t lds[2] = {};
     auto make = [&](int at, int64_t m, int64_t mp, int64_t kp) {
-        out.push_back(at::empty({m, kp}, x.options().dtype(dtype)));
+        out.push_back(fresh({m, kp}, dtype, x));
         ptr[at] = static_cast<uint8_t*>(out.back().data_ptr());
         if (block_rows == 1) {
-            out.push_back(down_columns(m, kp / 128, x.options(), at::kFloat8_e8m0fnu));
+            out.push_back(down_columns(m, kp / 128, at::kFloat8_e8m0fnu, x));
             lds[at / 2] = up(m, 16);
         } else {
-            out.push_back(at::empty({mp / 128, kp / 128}, x.options().dtype(at::kFloat8_e8m0fnu)));
+            out.push_back(fresh({mp / 128, kp / 128}, at::kFloat8_e8m0fnu, x));
             lds[at / 2] = kp / 128;
         }
         ptr[at + 1] = static_cast<uint8_t*>(out.back().data_ptr());
@@ -273,7 +281,7 @@ Tensor scale_rows(const Tensor& s, int64_t* ld) {
         *ld = step;
         return s;
     }
-    auto t = down_columns(M, KB, s.options(), s.scalar_type());
+    auto t = down_columns(M, KB, s.scalar_type(), s);
     *ld = up(M, 16);
     t.view(e == 1 ? at::kByte : at::kFloat).copy_(s.view(e == 1 ? at::kByte : at::kFloat));
     return t;
@@ -295,7 +303,7 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     TORCH_CHECK(b_scale.dim() == 2 && (b_scale.size(0) == N || b_scale.size(0) == NB) && b_scale.size(1) == KB,
                 "b_scale must be [N, K / 128] or [ceil(N / 128), K / 128]");
     const c10::DeviceGuard guard(a.device());
-    auto out = at::empty({M, N}, a.options().dtype(out_dtype));
+    auto out = fresh({M, N}, out_dtype, a);
     if (M == 0 || N == 0) return out;
     int64_t lda_s = 0, ldb_s = 0;
     const Tensor as = scale_rows(a_scale, &lda_s);
