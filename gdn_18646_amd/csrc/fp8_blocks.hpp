@@ -29,22 +29,20 @@ struct Fp8 {
     }
     // 2^-e of a scale byte.
     __device__ __forceinline__ static float inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
-    // Codes of eight values times inv (a scale's inverse), all NaN where bad.
-    __device__ __forceinline__ static gdn::u32x2 codes8(const float* f, float inv, bool bad) {
-        gdn::u32x2 w;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            int v = 0;
-            if constexpr (FMT == GDN_E4M3) {
-                v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, v, false);
-                v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, v, true);
-            } else {
-                v = __builtin_amdgcn_cvt_pk_bf8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, v, false);
-                v = __builtin_amdgcn_cvt_pk_bf8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, v, true);
-            }
-            w[i] = bad ? 0x7f7f7f7fu : static_cast<uint32_t>(v);
+    // Codes of four values times inv (a scale's inverse), all NaN where bad.
+    __device__ __forceinline__ static uint32_t codes4(float a, float b, float c, float d, float inv, bool bad) {
+        int v = 0;
+        if constexpr (FMT == GDN_E4M3) {
+            v = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, v, false);
+            v = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, v, true);
+        } else {
+            v = __builtin_amdgcn_cvt_pk_bf8_f32(a * inv, b * inv, v, false);
+            v = __builtin_amdgcn_cvt_pk_bf8_f32(c * inv, d * inv, v, true);
         }
-        return w;
+        return bad ? 0x7f7f7f7fu : static_cast<uint32_t>(v);
+    }
+    __device__ __forceinline__ static gdn::u32x2 codes8(const float* f, float inv, bool bad) {
+        return gdn::u32x2{codes4(f[0], f[1], f[2], f[3], inv, bad), codes4(f[4], f[5], f[6], f[7], inv, bad)};
     }
 };
 

@@ -3,10 +3,12 @@
 // sums over x's rows), or both from one read; a block is 1 x 128 values along
 // the codes' own rows, or 128 x 128 of x.
 //
-// One workgroup a 128 x 128 tile: a thread holds 8 x 8 of it in registers, a
+// One workgroup a 128 x 128 tile: a thread holds 4 x 8 of it in registers, a
 // row's maximum meets over 16 lanes by DPP, a column's over LDS, and the
 // transposed codes pass through LDS so that both layouts leave in whole
-// 128-byte lines.  What bounds it: HBM (2 bytes read, 1 or 2 written a value).
+// 128-byte lines.  What bounds it: HBM (2 bytes read, 1 or 2 written a value)
+// above some 1000 tiles, below that a tile's chain of loads, maxima and stores,
+// which is why eight waves share one.
 #include "block_norm.hpp"
 #include "fp8_blocks.hpp"
 
@@ -22,41 +24,43 @@ struct QuantParams {
 };
 
 template <class TX, int FMT, bool BLOCK>
-__global__ __launch_bounds__(256) void gdn_fp8_quantize_kernel(QuantParams p) {
-    constexpr int kRowB = 144;  // bytes of a transposed row in LDS
-    __shared__ __attribute__((aligned(16))) unsigned char tile[128 * kRowB];
-    __shared__ uint32_t most[16][132];
-    __shared__ uint32_t bytes[128];
+__global__ __launch_bounds__(512) void gdn_fp8_quantize_kernel(QuantParams p) {
+    constexpr int RT = 4;  // rows of a thread
+    __shared__ __attribute__((aligned(16))) unsigned char tile[128 * 128];
+    __shared__ __attribute__((aligned(16))) uint32_t most[32][132];
+    __shared__ __attribute__((aligned(16))) uint32_t bytes[128];
     const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4;
     const int k0 = static_cast<int>(blockIdx.x % p.kb) * kBlk, m0 = static_cast<int>(blockIdx.x / p.kb) * kBlk;
-    const int c = k0 + 8 * cg, r0 = m0 + 8 * rg;
+    const int c = k0 + 8 * cg, r0 = m0 + RT * rg;
 
-    float f[8][8];
+    Oct<TX> o[RT];
+    if (p.vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long row = static_cast<long long>(min(r0 + i, p.M - 1)) * p.ldx;
-        if (p.vec)
-            Oct<TX>::template load<true>(p.x, row, c, p.K).get(f[i]);
-        else
-            Oct<TX>::template load<false>(p.x, row, c, p.K).get(f[i]);
+        for (int i = 0; i < RT; ++i) o[i] = Oct<TX>::template load<true>(p.x, min(r0 + i, p.M - 1) * p.ldx, c, p.K);
+    } else {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) o[i] = Oct<TX>::template load<false>(p.x, min(r0 + i, p.M - 1) * p.ldx, c, p.K);
     }
+    float f[RT][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < RT; ++i) {
+        o[i].get(f[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[i][j] = r0 + i < p.M && c + j < p.K ? f[i][j] : 0.f;
+    }
 
-    uint32_t rowb[8];  // scale bytes of the thread's rows
+    uint32_t rowb[RT];  // scale bytes of the thread's rows
     if constexpr (BLOCK) {
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, amax8(f[i]));
+        for (int i = 0; i < RT; ++i) m = max(m, amax8(f[i]));
         m = max16(m);
-        if (cg == 0) most[rg][0] = m;
+        if (cg == 0) bytes[rg] = m;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, most[i][0]);
+        for (int i = 0; i < 32; ++i) m = max(m, bytes[i]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rowb[i] = Fp8<FMT>::scale_byte(m);
+        for (int i = 0; i < RT; ++i) rowb[i] = Fp8<FMT>::scale_byte(m);
         if (tid == 0) {
             const int kt = k0 / kBlk, mt = m0 / kBlk;
             if (p.codes) p.scales[mt * p.lds + kt] = static_cast<uint8_t>(rowb[0]);
@@ -64,17 +68,14 @@ __global__ __launch_bounds__(256) void gdn_fp8_quantize_kernel(QuantParams p) {
         }
     } else if (p.codes) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rowb[i] = Fp8<FMT>::scale_byte(max16(amax8(f[i])));
-        if (cg == 0 && r0 < p.lds) {
-            uint32_t w[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) w[i] = rowb[4 * i] | rowb[4 * i + 1] << 8 | rowb[4 * i + 2] << 16 | rowb[4 * i + 3] << 24;
-            *reinterpret_cast<u32x2*>(p.scales + static_cast<long long>(k0 / kBlk) * p.lds + r0) = u32x2{w[0], w[1]};
-        }
+        for (int i = 0; i < RT; ++i) rowb[i] = Fp8<FMT>::scale_byte(max16(amax8(f[i])));
+        if (cg == 0 && r0 < p.lds)
+            *reinterpret_cast<uint32_t*>(p.scales + static_cast<long long>(k0 / kBlk) * p.lds + r0) =
+                rowb[0] | rowb[1] << 8 | rowb[2] << 16 | rowb[3] << 24;
     }
     if (p.codes) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < RT; ++i) {
             const u32x2 w = Fp8<FMT>::codes8(f[i], Fp8<FMT>::inverse(rowb[i]), rowb[i] == 0xffu);
             if (r0 + i < p.M) *reinterpret_cast<u32x2*>(p.codes + static_cast<long long>(r0 + i) * p.ldc + c) = w;
         }
@@ -86,18 +87,21 @@ __global__ __launch_bounds__(256) void gdn_fp8_quantize_kernel(QuantParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) colb[j] = rowb[0];
     } else {
+        u32x4 w[2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i][j]) & 0x7fffffffu);
-            most[rg][8 * cg + j] = m;
+            for (int i = 0; i < RT; ++i) m = max(m, __float_as_uint(f[i][j]) & 0x7fffffffu);
+            w[j / 4][j % 4] = m;
         }
+        *reinterpret_cast<u32x4*>(&most[rg][8 * cg]) = w[0];
+        *reinterpret_cast<u32x4*>(&most[rg][8 * cg + 4]) = w[1];
         __syncthreads();
         if (tid < 128) {
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m = max(m, most[i][tid]);
+            for (int i = 0; i < 32; ++i) m = max(m, most[i][tid]);
             const uint32_t b = Fp8<FMT>::scale_byte(m);
             bytes[tid] = b;
             if (k0 + tid < p.K) p.scales_t[static_cast<long long>(m0 / kBlk) * p.ldst + k0 + tid] = static_cast<uint8_t>(b);
@@ -106,21 +110,20 @@ __global__ __launch_bounds__(256) void gdn_fp8_quantize_kernel(QuantParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) colb[j] = bytes[8 * cg + j];
     }
+    // Row k of the transposed tile holds its 4-byte piece q (rows m0 + 4 q ..) at
+    // slot q ^ 4 (k / 8 % 8): the 16 lanes of a row group write to different
+    // banks, and 16 bytes stay together.
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float t[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = f[i][j];
-        *reinterpret_cast<u32x2*>(tile + (8 * cg + j) * kRowB + 8 * rg) =
-            Fp8<FMT>::codes8(t, Fp8<FMT>::inverse(colb[j]), colb[j] == 0xffu);
-    }
+    for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<uint32_t*>(tile + (8 * cg + j) * 128 + 4 * (rg ^ (4 * (cg & 7)))) =
+            Fp8<FMT>::codes4(f[0][j], f[1][j], f[2][j], f[3][j], Fp8<FMT>::inverse(colb[j]), colb[j] == 0xffu);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = 32 * i + tid / 8;
+    for (int i = 0; i < 2; ++i) {
+        const int k = 64 * i + tid / 8;
         if (k0 + k < p.K)
             *reinterpret_cast<u32x4*>(p.codes_t + static_cast<long long>(k0 + k) * p.ldt + m0 + 16 * (tid & 7)) =
-                *reinterpret_cast<const u32x4*>(tile + k * kRowB + 16 * (tid & 7));
+                *reinterpret_cast<const u32x4*>(tile + k * 128 + 16 * ((tid & 7) ^ (k / 8 & 7)));
     }
 }
 
@@ -156,7 +159,7 @@ extern "C" int gdn_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int6
     p.vec = K % 8 == 0 && vec_rows(x, ldx, type_x);
     const auto launch = [&](auto tx, auto fmt, auto blk) {
         hipLaunchKernelGGL((gdn_fp8_quantize_kernel<decltype(tx), decltype(fmt)::value, decltype(blk)::value>),
-                           dim3(static_cast<unsigned>(MB * KB)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+                           dim3(static_cast<unsigned>(MB * KB)), dim3(512), 0, static_cast<hipStream_t>(stream), p);
         return gdn_host::check_launch("gdn_fp8_quantize_kernel");
     };
     const auto of_format = [&](auto tx, auto blk) {
