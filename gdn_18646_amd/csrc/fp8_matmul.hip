@@ -1,18 +1,17 @@
 // Entry point of the fp8 block-scaled product, and its kernel for a few tokens.
 //
-// gdn_fp8_few_kernel (up to 16 tokens, one decode step): what counts is the
-// weights' bytes.  A workgroup of 8 waves owns 16 columns; each wave takes every
-// eighth block of K straight from memory into MFMA fragments (no LDS: nothing is
-// used twice), and the waves' sums meet in LDS.
+// gdn_fp8_few_kernel (a decode step's tokens): what counts is the weights' bytes.
+// A workgroup owns 16 columns; each of its waves takes every WAVES-th block of K
+// straight from memory into MFMA fragments (no LDS: nothing is used twice), and
+// the waves' sums meet in LDS.  One token, us (GB/s of weights): N 2048, K 2048 3.5
+// (launch bound), 8224 x 2048 5.4, 8192 x 8192 12.0 (5.6 TB/s).
 #include "fp8_matmul.hpp"
 
 namespace {
 
-constexpr int kFewWaves = 8;
-
-template <int FA, int FB, bool OUT32>
-__global__ __launch_bounds__(64 * kFewWaves) void gdn_fp8_few_kernel(gdn_fp8::MatmulParams p, int scales) {
-    __shared__ f32x4 sums[kFewWaves][64];
+template <int FA, int FB, bool OUT32, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::MatmulParams p, int scales) {
+    __shared__ f32x4 sums[WAVES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
     const int n0 = blockIdx.x * 16, nslices = p.K / 128;
@@ -25,7 +24,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gdn_fp8_few_kernel(gdn_fp8::Ma
     const size_t sstep = rows ? p.ldb_s : 1, sat = rows ? row : static_cast<size_t>(row / 128) * p.ldb_s;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int kb = wave; kb < nslices; kb += kFewWaves) {
+    for (int kb = wave; kb < nslices; kb += WAVES) {
         const u32x4* const wp = reinterpret_cast<const u32x4*>(w + static_cast<size_t>(kb) * 128);
         const u32x4* const xp = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(kb) * 128);
         const int sx = p.a_scale[kb * p.lda_s + tok];
@@ -51,7 +50,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gdn_fp8_few_kernel(gdn_fp8::Ma
     __syncthreads();
     if (wave > 0) return;
 #pragma unroll
-    for (int i = 1; i < kFewWaves; ++i) acc += sums[i][lane];
+    for (int i = 1; i < WAVES; ++i) acc += sums[i][lane];
     if (n0 + r16 >= p.N) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -116,13 +115,21 @@ Choice choose_tile(long long M, long long N, int K, bool f32) {
 
 template <int FA, int FB>
 int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t stream) {
-    if (p.M <= 16) {
-        const dim3 grid((p.N + 15) / 16), block(64 * kFewWaves);
-        if (f32)
-            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, true>), grid, block, 0, stream, p, scales);
-        else
-            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, false>), grid, block, 0, stream, p, scales);
-        return gdn_host::check_launch("gdn_fp8_few_kernel");
+    // Few tokens.  Above four the tokens' own codes, which every workgroup reads,
+    // begin to count, and more so the more workgroups: 16 tokens of K = 2048 take
+    // 4.0 us (tiles 4.8) at N = 2048, 7.4 (5.6) at 8224.  Many columns give every
+    // CU enough waves with four a workgroup (8224: 5.4 us against 5.8 with eight),
+    // few do not (2048, K = 4096: 5.0 against 4.4).
+    if (p.M <= 4 || (p.M <= 16 && p.N <= 4096)) {
+        const auto few = [&](auto out32, auto waves) {
+            constexpr int W = decltype(waves)::value;
+            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, scales);
+            return gdn_host::check_launch("gdn_fp8_few_kernel");
+        };
+        const auto of_n = [&](auto out32) {
+            return p.N <= 4096 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
+        };
+        return f32 ? of_n(std::true_type{}) : of_n(std::false_type{});
     }
     // The last columns past a multiple of 256 in a launch of their own, on a tile
     // of their size, where the fit says that this is faster than a column of

@@ -127,7 +127,8 @@ def _operands(M, N, K, fa, fb, bscale, rows, dev, seed=0):
 
 
 SIZES = [(1, 1, 128), (1, 2048, 2048), (2, 100, 384), (16, 129, 1152), (17, 40, 128), (33, 65, 256), (77, 300, 1280), (64, 64, 8448),
-         (130, 1040, 384), (300, 1030, 512), (513, 2100, 256), (1030, 2050, 384), (2500, 5003, 256), (5, 33, 8448)]
+         (130, 1040, 384), (300, 1030, 512), (513, 2100, 256), (1030, 2050, 384), (2500, 5003, 256), (5, 33, 8448), (3, 5000, 640),
+         (16, 4100, 640)]
 
 
 @pytest.mark.parametrize("fa,fb", [(E4, E4), (E5, E4), (E4, E5), (E5, E5)], ids=["e4e4", "e5e4", "e4e5", "e5e5"])
@@ -147,6 +148,14 @@ def test_product_long(exts, dev, M, N, bscale, rows):
     """More blocks than a wave holds scales for at once."""
     a, sa, b, sb = _operands(M, N, 8448, E4, E4, bscale, rows, dev)
     _check(exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=torch.float32), a, sa, b, sb)
+
+
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
+@pytest.mark.parametrize("M,N,K,out", [(4096, 4118, 256, torch.bfloat16), (3000, 1297, 512, torch.float32)])
+def test_product_in_two_launches(exts, dev, M, N, K, out, bscale, rows):
+    """A few columns past a multiple of 256 run on tiles of their own."""
+    a, sa, b, sb = _operands(M, N, K, E4, E4, bscale, rows, dev)
+    _check(exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out), a, sa, b, sb)
 
 
 @pytest.mark.parametrize("M,N,K", [(3, 200, 256), (150, 300, 256)])
