@@ -19,7 +19,7 @@
 
 #include "../../include/gdn_amd.h"
 
-void bind_block_ops(pybind11::module_& rmsnorm, pybind11::module_& proj);  // bindings_block.cpp
+void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11::module_& proj);  // bindings_block.cpp
 
 namespace {
 
@@ -626,5 +626,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     auto mj = m.def_submodule("proj", "Projection + causal conv + SiLU");
     mj.def("forward", &proj_forward, "Fused linear projection + causal depthwise conv1d + SiLU (bf16)",
            py::arg("input"), py::arg("weight"), py::arg("conv_w"));
-    bind_block_ops(mr, mj);
+    bind_block_ops(m, mr, mj);
 }

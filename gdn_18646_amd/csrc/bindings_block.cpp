@@ -324,10 +324,23 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     return out;
 }
 
+// Whether a gradient accumulator of one of these leaves lives that belongs to
+// another stream than the current one of the leaf's device.
+bool leaves_of_another_stream(const std::vector<Tensor>& leaves) {
+    for (const auto& t : leaves) {
+        if (!t.is_cuda()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+        const auto stream = node ? node->stream() : std::nullopt;
+        if (stream.has_value() && stream->id() != c10::hip::getCurrentHIPStream(t.get_device()).id()) return true;
+    }
+    return false;
+}
+
 }  // namespace
 
-void bind_block_ops(pybind11::module_& rmsnorm, pybind11::module_& proj) {
+void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11::module_& proj) {
     namespace py = pybind11;
+    top.def("_leaves_of_another_stream", &leaves_of_another_stream);
     const py::object none = py::none();
     rmsnorm.def("block_norm", &block_norm,
                 "u = RMSNorm(y) post_gamma; h = residual + residual_scale scale act(gate) u; n = RMSNorm(h) gamma.\n"

@@ -1,0 +1,251 @@
+"""The differentiable operators of gdn_18646_amd.blocks on the GPU, alone and as
+a run: projection, block norm with quantised output, projection, backward."""
+
+import pytest
+import torch
+
+from gdn_18646_amd.blocks import Fp8Weight, block_norm, fp8_linear
+from tests.test_fp8_gpu import E4, E5, _quantize64
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(shape, dtype, dev, seed, std=1.0, grad=True):
+    t = (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype).to(dev)
+    return t.requires_grad_(grad)
+
+
+def _value64(x, rows, fmt):
+    """What quantisation makes of x, in float64 on the CPU, padded columns cut off."""
+    codes, s = _quantize64(x.detach(), rows, fmt)
+    s = torch.ldexp(torch.ones(s.shape, dtype=torch.float64), s.int() - 127)
+    wide = s.repeat_interleave(rows, 0)[:codes.shape[0]].repeat_interleave(128, 1)
+    return (codes.view(fmt).double() * wide)[:, :x.shape[1]]
+
+
+def _near(x, ref, mag, K, what):
+    """bf16: half a step, and 2^-10 of the largest product a block (the fp8 matrix
+    instruction), bounded by 2^-10 of the magnitudes; fp32: K half steps of them."""
+    x = x.detach().double().cpu()
+    bf = what.startswith("bf16")
+    tol = (2.0 ** -10 if bf else (K + 2) * 2.0 ** -24) * mag + (2.0 ** -8 * ref.abs() if bf else 0) + 1e-30
+    far = (x - ref).abs() - tol
+    assert x.shape == ref.shape and not (far > 0).any(), f"{what}: {(far > 0).sum().item()} values, the worst {far.max().item():.3g} past its bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shape,N", [((2, 37, 256), 384), ((5, 200), 130), ((1, 640), 2048), ((300, 130), 300)], ids=str)
+def test_fp8_linear(dev, shape, N, dtype):
+    K, kind = shape[-1], "bf16" if dtype == torch.bfloat16 else "fp32"
+    x, w = _rand(shape, dtype, dev, 1), _rand((N, K), dtype, dev, 2, 0.05)
+    y = fp8_linear(x, w)
+    dy = _rand(y.shape, dtype, dev, 3, 0.01, grad=False)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.dtype == dtype and dx.dtype == dtype and dw.dtype == dtype and y.shape == (*shape[:-1], N)
+    x2, d2 = x.reshape(-1, K), dy.reshape(-1, N)
+    xv, wv, dv = _value64(x2, 1, E4), _value64(w, 128, E4), _value64(d2, 1, E5)
+    xt, dt = _value64(x2.t(), 1, E4), _value64(d2.t(), 1, E5)
+    _near(y.reshape(-1, N), xv @ wv.t(), xv.abs() @ wv.abs().t(), K, kind + " y")
+    _near(dx.reshape(-1, K), dv @ wv, dv.abs() @ wv.abs(), N, kind + " dx")
+    _near(dw, dt @ xt.t(), dt.abs() @ xt.abs().t(), x2.shape[0], kind + " dw")
+    # a weight quantised once gives the same
+    q = Fp8Weight(w, transposed=True)
+    y2 = fp8_linear(x, q)
+    assert torch.equal(y2, y) and torch.equal(torch.autograd.grad(y2, x, dy)[0], dx)
+
+
+def test_fp8_linear_partial_gradients(dev):
+    x, w = _rand((40, 256), torch.bfloat16, dev, 1), _rand((128, 256), torch.bfloat16, dev, 2, 0.05)
+    dy = _rand((40, 128), torch.bfloat16, dev, 3, grad=False)
+    dx, dw = torch.autograd.grad(fp8_linear(x, w), (x, w), dy)
+    assert torch.equal(torch.autograd.grad(fp8_linear(x, w.detach()), x, dy)[0], dx)
+    assert torch.equal(torch.autograd.grad(fp8_linear(x.detach(), w), w, dy)[0], dw)
+    assert not fp8_linear(x.detach(), Fp8Weight(w)).requires_grad
+    with pytest.raises(ValueError, match="transposed"):
+        fp8_linear(x, Fp8Weight(w))
+    with pytest.raises(ValueError, match="weight"):
+        fp8_linear(x, w[:, :128])
+    e = torch.zeros(0, 256, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    y = fp8_linear(e, w)
+    dx, dw = torch.autograd.grad(y, (e, w), torch.zeros_like(y))
+    assert y.shape == (0, 128) and dx.shape == (0, 256) and (dw == 0).all()
+
+
+def test_block_norm_gradients_through_autograd(dev):
+    """Expanded, missing and accumulated gradients reach the kernel as they should."""
+    D = 512
+    y, r = _rand((3, 11, D), torch.float32, dev, 1), _rand((3, 11, D), torch.float32, dev, 2)
+    g, pg, gm = _rand((3, D), torch.float32, dev, 3), _rand((D,), torch.float32, dev, 4), _rand((D,), torch.float32, dev, 5)
+
+    def ref(y, r, g, pg, gm):
+        u = y * (y.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt() * pg * torch.tanh(g)[:, None]
+        h = r + 0.5 * u
+        return h, h * (h.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt() * gm
+
+    leaves = (y, r, g, pg, gm)
+    wide = tuple(t.detach().double().cpu().requires_grad_() for t in leaves)
+    for loss in (lambda h, n: h.sum() + n.sum(), lambda h, n: h[1].pow(2).sum(), lambda h, n: (n * n).mean(),
+                 lambda h, n: (h.transpose(0, 1) * 2).sum() + n[..., ::2].sum()):
+        h, n = block_norm(y, residual=r, gate=g, post_gamma=pg, gamma=gm, residual_scale=0.5, act="tanh")
+        got = torch.autograd.grad(loss(h, n), leaves, allow_unused=True)
+        want = torch.autograd.grad(loss(*ref(*wide)), wide, allow_unused=True)
+        for a, b in zip(got, want):
+            if b is None:
+                assert a is None or (a == 0).all()
+            else:  # fp32 sums of at most 33 rows: 1e-5 of the largest value
+                assert (a.double().cpu() - b).abs().max() <= 1e-5 * b.abs().max() + 1e-12
+    only = torch.autograd.grad(block_norm(y, gamma=gm.detach())[1].sum(), y)[0]
+    assert torch.isfinite(only).all()
+
+
+def _run(x, h0, w1, w2, pg, gm):
+    """A block's tail and the next block's head: project, join the residual
+    stream, norm, project."""
+    y = fp8_linear(x, w1)
+    h, n = block_norm(y, residual=h0, post_gamma=pg, gamma=gm)
+    return h, fp8_linear(n, w2)
+
+
+def test_a_run_of_them(exts, dev):
+    """The training run's results against float64 on its own intermediate values,
+    and the serving run (norm straight to codes) against the training run."""
+    T, D, N = 77, 512, 640
+    x, h0 = _rand((T, D), torch.bfloat16, dev, 1), _rand((T, D), torch.bfloat16, dev, 2)
+    w1, w2 = _rand((D, D), torch.bfloat16, dev, 3, 0.05), _rand((N, D), torch.bfloat16, dev, 4, 0.05)
+    pg, gm = _rand((D,), torch.bfloat16, dev, 5, 0.1), _rand((D,), torch.bfloat16, dev, 6, 0.1)
+    h, z = _run(x, h0, w1, w2, pg, gm)
+    grads = torch.autograd.grad([h, z], (x, h0, w1, w2, pg, gm), [torch.ones_like(h), torch.ones_like(z)])
+    assert all(torch.isfinite(g.float()).all() and g.abs().max() > 0 for g in grads)
+    # gradients repeat bit for bit
+    h2, z2 = _run(x, h0, w1, w2, pg, gm)
+    again = torch.autograd.grad([h2, z2], (x, h0, w1, w2, pg, gm), [torch.ones_like(h), torch.ones_like(z)])
+    assert torch.equal(h, h2) and torch.equal(z, z2) and all(torch.equal(a, b) for a, b in zip(grads, again))
+    # serving: the norm writes the codes that the product reads
+    with torch.no_grad():
+        q1, q2 = Fp8Weight(w1), Fp8Weight(w2)
+        y = fp8_linear(x, q1)
+        hs, _, codes, scales = exts["rmsnorm"].block_norm(y, residual=h0, post_gamma=pg, gamma=gm, quantize=True)
+        zs = exts["proj"].fp8_matmul(codes, scales, q2.codes, q2.scales)
+    assert torch.equal(hs, h)
+    n = codes.float() * scales.float().repeat_interleave(128, 1)
+    ref = n.double().cpu() @ _value64(w2, 128, E4).t()
+    _near(zs, ref, n.double().cpu().abs() @ _value64(w2, 128, E4).abs().t(), D, "bf16 z")
+    # the two runs differ by n's rounding to bf16 before it is quantised: a code moves by a
+    # step (2^-3 of it) at most, and moves for few
+    assert (zs.float() - z.float()).norm() <= 2.0 ** -3 * z.float().norm()
+
+
+def test_run_captured_with_eager_work_between(dev):
+    """Forward and backward of the run in a graph, three replays with eager runs of
+    the same leaves between them."""
+    T, D = 130, 256
+    x, h0 = _rand((T, D), torch.bfloat16, dev, 1), _rand((T, D), torch.bfloat16, dev, 2)
+    w1, w2 = _rand((D, D), torch.bfloat16, dev, 3, 0.05), _rand((D, D), torch.bfloat16, dev, 4, 0.05)
+    pg, gm = _rand((D,), torch.bfloat16, dev, 5, 0.1), _rand((D,), torch.bfloat16, dev, 6, 0.1)
+    leaves = (x, h0, w1, w2, pg, gm)
+
+    def step():
+        h, z = _run(*leaves)
+        return [h, z, *torch.autograd.grad([h, z], leaves, [torch.ones_like(h), torch.ones_like(z)])]
+
+    eager = [t.detach().clone() for t in step()]  # no eager graph of the leaves outlives this line
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        for t in got:
+            t.detach().fill_(7.0)
+        graph.replay()
+        again = [t.detach() for t in step()]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager)) and all(torch.equal(a, b) for a, b in zip(again, eager))
+
+
+def test_capture_beside_an_eager_graph_is_refused(dev):
+    """A backward pass that would wait for another stream's gradient accumulators
+    inside a capture is refused before autograd does."""
+    x = _rand((16, 256), torch.bfloat16, dev, 1)
+    gm = _rand((256,), torch.bfloat16, dev, 2)
+    w = _rand((128, 256), torch.bfloat16, dev, 3)
+    for f, leaves in ((lambda: block_norm(x, gamma=gm)[1], (x, gm)), (lambda: fp8_linear(x, w), (x, w))):
+        kept = f()  # its graph lives
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager autograd graph"):
+            with torch.cuda.graph(graph, stream=side):
+                y = f()
+                torch.autograd.grad(y, leaves, torch.ones_like(y))
+        torch.cuda.synchronize()
+        y = None
+        torch.autograd.grad(kept, leaves, torch.ones_like(kept))  # the eager graph is as it was
+        kept = None
+    torch.cuda.synchronize()
+
+
+def test_two_streams_at_once(exts, dev):
+    """Calls on two streams share nothing."""
+    x = [_rand((500, 2048), torch.bfloat16, dev, s, grad=False) for s in (1, 2)]
+    gm = _rand((2048,), torch.bfloat16, dev, 3, grad=False)
+    w = Fp8Weight(_rand((1000, 2048), torch.bfloat16, dev, 4, 0.05, grad=False))
+
+    def run(t):
+        h, n, c, s = exts["rmsnorm"].block_norm(t, residual=t, gamma=gm, quantize=True)
+        return h, exts["proj"].fp8_matmul(c, s, w.codes, w.scales)
+
+    want = [run(t) for t in x]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in x]
+    for _ in range(5):
+        got = []
+        for t, s in zip(x, streams):
+            with torch.cuda.stream(s):
+                got.append(run(t))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w_ in zip(got, want) for a, b in zip(g, w_))
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda e, t: e["rmsnorm"].block_norm(t, residual=t[:2]), "residual must have y's shape"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, gate=t.float()), "gate must have"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, gate=t[:3]), "gate must have y's shape"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, gamma=t[0, :8]), "gamma must be D"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, gamma=t[0], post_gamma=t[0].float()), "one type"),
+    (lambda e, t: e["rmsnorm"].block_norm(t.half()), "bfloat16 or float32"),
+    (lambda e, t: e["rmsnorm"].block_norm(t.t()), "adjacent elements"),
+    (lambda e, t: e["rmsnorm"].block_norm(t[None].expand(3, 4, 256)), "one stride|overlap"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, act="relu"), "act must be"),
+    (lambda e, t: e["rmsnorm"].block_norm(t.float(), residual=t), "unsupported"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, store_h=False), "nothing to write"),
+    (lambda e, t: e["rmsnorm"].block_norm(t, inplace=True), "inplace"),
+    (lambda e, t: e["rmsnorm"].block_norm_backward(None, None, t), "dh or dn"),
+    (lambda e, t: e["rmsnorm"].block_norm_backward(t, None, t, post_gamma=t[0]), "rstd_y"),
+    (lambda e, t: e["rmsnorm"].block_norm_backward(t.float(), None, t), "h's type"),
+    (lambda e, t: e["rmsnorm"].block_norm_backward(None, t, t), "dn needs gamma"),
+    (lambda e, t: e["proj"].fp8_quantize(t, block_rows=64), "1 or 128"),
+    (lambda e, t: e["proj"].fp8_quantize(t, dtype=torch.float16), "float8"),
+    (lambda e, t: e["proj"].fp8_quantize(t, rows=False), "neither"),
+    (lambda e, t: e["proj"].fp8_quantize(t.t()), "adjacent"),
+    (lambda e, t: e["proj"].fp8_quantize(t[None]), r"\[M, K\]"),
+    (lambda e, t: e["proj"].fp8_matmul(t, t, t, t), "float8"),
+])
+def test_binding_refusals(exts, dev, call, match):
+    t = torch.zeros(4, 256, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match=match):
+        call(exts, t)
+
+
+def test_product_binding_refusals(exts, dev):
+    t = torch.zeros(4, 256, dtype=torch.bfloat16, device=dev)
+    a, s = exts["proj"].fp8_quantize(t)
+    f = exts["proj"].fp8_matmul
+    for args, match in (((a, s, a[:, :128], s), "K"), ((a[:, :64], s, a[:, :64], s), "multiple of 128"), ((a, s.float(), a, s), "a_scale"),
+                        ((a, s[:2], a, s), "a_scale"), ((a, s, a, s[:2]), "b_scale"), ((a, s, a, s.half()), "b_scale"),
+                        ((a, s, a, s, torch.float16), "out_dtype"), ((a, s, a.cpu(), s.cpu()), "one device")):
+        with pytest.raises(RuntimeError, match=match):
+            f(*args)
