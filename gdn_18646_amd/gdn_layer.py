@@ -148,8 +148,12 @@ class GDNLayerCustom:
         return self.exts['rmsnorm'].forward(x2d.contiguous(), self.w['norm_gamma'], 1e-6, 256, 2)
 
     @torch.no_grad()
-    def forward(self, x, mask=None, return_state=False, state=None, cu_seqlens=None):
+    def forward(self, x, mask=None, return_state=False, state=None, cu_seqlens=None, xn=None):
         """x [B, T, D] bf16 -> y [B, T, D] bf16.
+
+        ``xn`` (x's shape): the input norm's result where the caller has it
+        already (a stack's block norms make it with the residual, see stack.py);
+        x is then not read and may be None.
 
         mask [B, T] fp32 (1 keep, 0 masked; default all ones).  With
         ``return_state`` also returns the decode-state dict after the last
@@ -168,12 +172,13 @@ class GDNLayerCustom:
         if self.dt_bias_scalar is None:
             raise ValueError("prefill takes a scalar dt_bias (as the reference kernel)")
         if cu_seqlens is not None:
-            return self._forward_packed(x, cu_seqlens, mask, return_state, state)
+            return self._forward_packed(x, cu_seqlens, mask, return_state, state, xn)
+        x = xn if xn is not None else x
         B, T, _ = x.shape
         Dd, Hh, dk, dv = self.D, self.H, self.DK, self.DV
         if mask is None:  # empty = every token kept (no fill kernel)
             mask = torch.empty(0, dtype=torch.float32, device=x.device)
-        xn = self._rmsnorm(x.reshape(B * T, Dd)).reshape(B, T, Dd)
+        xn = xn.contiguous() if xn is not None else self._rmsnorm(x.reshape(B * T, Dd)).reshape(B, T, Dd)
         st = state or {}
         outs = self._layer.in_proj(xn, self.W_qkvab, self.conv_qkv, Hh, dk, dv,
                                    st.get('conv_q'), st.get('conv_k'), st.get('conv_v'), bool(return_state))
@@ -199,13 +204,14 @@ class GDNLayerCustom:
             xn_hist = torch.cat([prev[:, T:], xn], 1)
         return y, dict(recurrent=S, conv_q=outs[5], conv_k=outs[6], conv_v=outs[7], xn=xn_hist.contiguous())
 
-    def _forward_packed(self, x, cu_seqlens, mask, return_state, state):
+    def _forward_packed(self, x, cu_seqlens, mask, return_state, state, xn):
+        x = xn if xn is not None else x
         Dd, Hh, dk, dv = self.D, self.H, self.DK, self.DV
         cu = torch.as_tensor(cu_seqlens, dtype=torch.int32).cpu().contiguous()
         Tt = x.shape[-2]
         if x.shape[-1] != Dd or x.numel() != Tt * Dd:
             raise ValueError(f"packed x must be [1, T_total, D] or [T_total, D], got {tuple(x.shape)}")
-        xn = self._rmsnorm(x.reshape(Tt, Dd))
+        xn = xn.reshape(Tt, Dd).contiguous() if xn is not None else self._rmsnorm(x.reshape(Tt, Dd))
         st = state or {}
         outs = self._layer.in_proj_varlen(xn, self.W_qkvab, self.conv_qkv, Hh, dk, dv, cu, st.get('conv_q'),
                                           st.get('conv_k'), st.get('conv_v'), bool(return_state))
