@@ -26,7 +26,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
     __shared__ float sums[2][2][LPR > 64 ? LPR / 64 : 1];
     const int tid = threadIdx.x, lane = tid % LPR;
     const int D = p.D;
-    auto inside = [&](int u, int e) { return VEC ? 8 * (lane + LPR * u) < D : 8 * (lane + LPR * u) + e < D; };
+    auto inside = [&](int u, int e) { return own<VEC>(8 * (lane + LPR * u), e, D); };
 
     struct Row {
         Oct<TY> y[NV], g[NV];
@@ -85,8 +85,8 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
             cur.y[u].get(h[u]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                h[u][e] = inside(u, e) ? h[u][e] : 0.f;
-                ss = fmaf(h[u][e], h[u][e], ss);
+                if (VEC && !inside(u, e)) h[u][e] = 0.f;
+                if (VEC || inside(u, e)) ss = fmaf(h[u][e], h[u][e], ss);
             }
         }
         float inv = 1.f;
@@ -115,8 +115,9 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                h[u][e] = inside(u, e) ? fmaf(a[e], h[u][e], t[e]) : 0.f;
-                ss = fmaf(h[u][e], h[u][e], ss);
+                h[u][e] = fmaf(a[e], h[u][e], t[e]);
+                if (VEC && !inside(u, e)) h[u][e] = 0.f;
+                if (VEC || inside(u, e)) ss = fmaf(h[u][e], h[u][e], ss);
             }
             if (p.h && live) store8<TR, VEC>(p.h, r * p.ldh, 8 * (lane + LPR * u), D, h[u]);
         }
@@ -130,10 +131,14 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
             const int c = 8 * (lane + LPR * u);
             if (p.gamma) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[u][e] = inside(u, e) ? h[u][e] * inv * gm[u][e] : 0.f;
+                for (int e = 0; e < 8; ++e) {
+                    h[u][e] = h[u][e] * inv * gm[u][e];
+                    if (VEC && !inside(u, e)) h[u][e] = 0.f;
+                }
             }
             if (p.n && live) store8<TY, VEC>(p.n, r * p.ldn, c, D, h[u]);
             if (p.codes) {
+                if constexpr (!VEC) to_natural(h[u], c - vector_at(c, D), D);
                 const uint32_t s = Fp8<GDN_E4M3>::scale_byte(max16(amax8(h[u])));
                 const u32x2 w = Fp8<GDN_E4M3>::codes8(h[u], Fp8<GDN_E4M3>::inverse(s), s == 0xffu);
                 if (live && c / kBlk * kBlk < D) {  // a ragged last block is filled up with zero codes

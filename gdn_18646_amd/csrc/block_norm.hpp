@@ -6,6 +6,13 @@
 // lane l's vector u is columns 8 (l + LPR u) .. + 7, so 16 neighbouring lanes
 // hold 128 adjacent columns.  Rows are read once and stay in registers between
 // their sums and what is written from them.
+//
+// Where 16-byte accesses do not fit (VEC false: D no multiple of 8, or rows at
+// odd addresses) the lane with the row's end holds its last 8 columns instead,
+// some of which the lane before it holds too: both compute and write the same
+// there, and the sums take each column once.  So every lane's loads are whole
+// and all under way at once; taking the end element by element made that wave
+// wait for each tensor in turn (figures at the kernels).
 #pragma once
 
 #include "gdn_common.hpp"
@@ -50,15 +57,23 @@ using namespace gdn;
 using gdn_block::NormBwdParams;
 using gdn_block::NormParams;
 
+// The first of the 8 columns that the lane of columns c .. c + 7 holds, without VEC.
+__device__ __forceinline__ int vector_at(int c, int D) { return max(min(c, D - 8), 0); }
+// Whether the lane's element e is one of its own columns c .. c + 7, and inside the row.
+template <bool VEC>
+__device__ __forceinline__ bool own(int c, int e, int D) {
+    const int at = vector_at(c, D);
+    return VEC ? c < D : e >= c - at && at + e < D;
+}
+
 // Eight elements of a row as they lie in memory.
 template <class T>
 struct Oct {
     u32x4 w[sizeof(T) / 2];
 
-    // Columns c .. c + 7 of the row at `row` of D columns; columns past the end
-    // repeat one inside it (the callers drop them).  VEC: rows lie at multiples of
-    // 16 bytes and D is one of 8; else the lane with the row's end takes it element
-    // by element.
+    // The lane's 8 columns (vector_at(c, D) .. + 7) of the row at element `row`.
+    // Lanes past the end read some of the row's; the callers drop them, and the
+    // repeated elements of a row of fewer than 8.
     template <bool VEC>
     __device__ __forceinline__ static Oct load(const void* base, long long row, int c, int D) {
         const T* p = static_cast<const T*>(base) + row;
@@ -67,12 +82,12 @@ struct Oct {
             const u32x4* q = reinterpret_cast<const u32x4*>(p + (c < D ? c : 0));
 #pragma unroll
             for (unsigned i = 0; i < sizeof(T) / 2; ++i) o.w[i] = q[i];
-        } else if (c + 8 <= D) {
-            __builtin_memcpy(o.w, p + c, 8 * sizeof(T));  // 16-byte loads at any address
+        } else if (D >= 8) {
+            __builtin_memcpy(o.w, p + vector_at(c, D), 8 * sizeof(T));  // 16-byte loads at any address
         } else {
             T e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = p[min(c + i, D - 1)];
+            for (int i = 0; i < 8; ++i) e[i] = p[min(i, D - 1)];
             __builtin_memcpy(o.w, e, 8 * sizeof(T));
         }
         return o;
@@ -97,17 +112,31 @@ __device__ __forceinline__ void store8(void* base, long long row, int c, int D, 
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(f[i]);
     }
+    if (c >= D) return;
     if constexpr (VEC) {
-        if (c >= D) return;
         u32x4* q = reinterpret_cast<u32x4*>(p + c);
 #pragma unroll
         for (unsigned i = 0; i < sizeof(T) / 2; ++i) q[i] = w[i];
-    } else if (c + 8 <= D) {
-        __builtin_memcpy(p + c, w, 8 * sizeof(T));
+    } else if (D >= 8) {
+        __builtin_memcpy(p + vector_at(c, D), w, 8 * sizeof(T));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < D) p[c + i] = static_cast<T>(f[i]);
+            if (i < D) p[i] = static_cast<T>(f[i]);
+    }
+}
+
+// The values of columns vector_at .. + 7 moved down by `shift` to those of c .. c + 7, zeros past the row's end.
+__device__ __forceinline__ void to_natural(float* f, int shift, int D) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = e < D ? f[e] : 0.f;
+#pragma unroll
+    for (int o = 4; o; o >>= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = shift & o ? (e + o < 8 ? f[e + o] : 0.f) : f[e];
+    if (shift >= 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 0.f;
     }
 }
 

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
     const long long first = static_cast<long long>(group) * p.group_rows;
     const int end = static_cast<int>(min(first + p.group_rows, static_cast<long long>(p.R)));
     const long long step = static_cast<long long>(p.chunks) * SLOTS;
-    auto inside = [&](int u, int e) { return VEC ? 8 * (lane + LPR * u) < D : 8 * (lane + LPR * u) + e < D; };
+    auto inside = [&](int u, int e) { return own<VEC>(8 * (lane + LPR * u), e, D); };
 
     struct Row {
         Oct<TY> y[NV], dn[NV], g[NV];
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
             }
             cur.y[u].get(yn[u]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) yn[u][e] = inside(u, e) ? yn[u][e] * cur.ry : 0.f;
+            for (int e = 0; e < 8; ++e) yn[u][e] = !VEC || inside(u, e) ? yn[u][e] * cur.ry : 0.f;
             if (p.dh) {
                 cur.dh[u].get(dH[u]);
             } else {
@@ -214,14 +214,11 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
     float* const out = p.part + static_cast<size_t>(blockIdx.x) * 2 * D;
     if constexpr (!kShared) {
 #pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (inside(u, e)) {
-                    const int c = 8 * (lane + LPR * u) + e;
-                    out[c] = kLds ? cols[(u * LPR + lane) * 8 + e] : se[kLds ? 0 : u][e];
-                    out[D + c] = kLds ? cols[((NV + u) * LPR + lane) * 8 + e] : sg[kLds ? 0 : u][e];
-                }
+        for (int u = 0; u < NV; ++u) {
+            const int c = 8 * (lane + LPR * u);
+            store8<float, VEC>(out, 0, c, D, kLds ? cols + (u * LPR + lane) * 8 : se[kLds ? 0 : u]);
+            store8<float, VEC>(out, D, c, D, kLds ? cols + ((NV + u) * LPR + lane) * 8 : sg[kLds ? 0 : u]);
+        }
     } else {
         constexpr int kC = LPR * NV * 8;
 #pragma unroll
@@ -239,7 +236,8 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
                 for (int u = 0; u < NV; ++u)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int c = 8 * (lane + LPR * u) + e;
+                        const int at = 8 * (lane + LPR * u), c = (VEC ? at : vector_at(at, D)) + e;
+                        if (!VEC && !inside(u, e)) continue;
                         cols[c] = w == 0 ? se[u][e] : cols[c] + se[u][e];
                         cols[kC + c] = w == 0 ? sg[u][e] : cols[kC + c] + sg[u][e];
                     }
@@ -313,9 +311,12 @@ __global__ __launch_bounds__(1024) void gdn_block_norm_sum_kernel(SumParams p) {
 }
 
 // How R rows with a gate row each `per` are split over workgroups: 512 of them in
-// all, two a CU, or 256 for rows of over 2048 columns, while each has a row for
-// every one of its slots (16384 x 2048: 123 us with 512, 172 with 256, 138 with
-// 1024; 8192 x 4096: 131 with 256, 138 with 512).
+// all, two a CU, while each has a row for every one of its slots (16384 x 2048:
+// 118 us with 512, 171 with 256, 134 with 1024).  Rows of over 2048 columns have
+// workgroups of eight waves and more, 256 of them (8192 x 4096: 129 us, 134 with
+// 512); rows of 513 to 1024 have two waves, and 1024 workgroups if each walks
+// four rows at least (bf16, 16384 x 1024: 67 us, 99 with 512; 1500 rows: 20.8,
+// 19.2 with 512; fp32, 8192 x 1024: 63.5 against 59).
 struct Plan {
     long long groups;
     int group_rows, chunks;
@@ -327,7 +328,7 @@ Plan plan_rows(long long R, long long D, long long per) {
     Plan q;
     q.group_rows = static_cast<int>(rows);
     q.groups = shared ? (R + rows - 1) / rows : 1;
-    const long long all = D <= 2048 ? 512 : 256, most = (all + q.groups - 1) / q.groups, need = (rows + slots - 1) / slots;
+    const long long all = D > 2048 ? 256 : D > 512 && D <= 1024 && R >= 4096 ? 1024 : 512, most = (all + q.groups - 1) / q.groups, need = (rows + slots - 1) / slots;
     q.chunks = static_cast<int>(need < most ? need : most);
     return q;
 }

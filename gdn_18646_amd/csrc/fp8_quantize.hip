@@ -45,6 +45,7 @@ __global__ __launch_bounds__(512) void gdn_fp8_quantize_kernel(QuantParams p) {
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         o[i].get(f[i]);
+        if (!p.vec) to_natural(f[i], c - vector_at(c, p.K), p.K);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[i][j] = r0 + i < p.M && c + j < p.K ? f[i][j] : 0.f;
     }

@@ -12,6 +12,8 @@ relative to the sum of the magnitudes that enter a value covers it.
 import pytest
 import torch
 
+from tests.test_fp8_gpu import _quantize64
+
 pytestmark = pytest.mark.gpu
 
 EPS = 1e-6
@@ -126,6 +128,30 @@ def test_quantized_output(exts, dev, shape, pre, types):
     big = torch.nn.functional.pad(what, (0, Dp - D)).reshape(R, -1, 128).abs().amax(-1)
     s = scales.double().cpu()
     assert (big <= 448 * s * (1 + 1e-5)).all() and (big > 224 * s * (1 - 1e-5)).all()
+
+
+@pytest.mark.parametrize("D", [*range(2, 10), *range(121, 137), *range(1017, 1025)])
+def test_every_remainder_of_columns(exts, dev, D):
+    """Rows that end at each place of a lane's eight columns, both directions;
+    the codes are those of the fp32 n that a call without them writes."""
+    f = exts["rmsnorm"].block_norm
+    for types in ("bf16", "fp32"):
+        v = _inputs((2, 5, D), types, "sequence", seed=D)
+        h, n, _, _ = f(**v, act="silu", eps=EPS)
+        r, h64, n64, mag = _reference(v, 1.0, "silu")
+        _close(h, h64, mag, "h")
+        rms = (h64.pow(2).mean(-1, keepdim=True) + EPS).sqrt()
+        _close(n, n64, mag / rms * r["gamma"].abs(), "n")
+        h2, _, codes, scales = f(**v, act="silu", eps=EPS, quantize=True)
+        assert torch.equal(h2, h)
+        if types == "fp32":
+            rc, rs = _quantize64(n.reshape(-1, D), 1, torch.float8_e4m3fn)
+            assert torch.equal(scales.view(torch.uint8).cpu(), rs)
+            got = codes.view(torch.uint8).cpu()
+            assert ((got == rc) | ((got & 0x7f == 0) & (rc & 0x7f == 0))).all()
+        g = torch.Generator().manual_seed(9)
+        dh, dn = (torch.randn(h.shape, generator=g).to(h.dtype).to(dev) for _ in range(2))
+        _check_grads(_run_backward(exts, v, 1.0, "silu", dh, dn), _grads64(v, 1.0, "silu", dh, dn)[0], 10)
 
 
 def test_store_h_and_inplace(exts, dev):

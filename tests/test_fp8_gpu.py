@@ -68,6 +68,18 @@ def test_quantize(exts, dev, M, K, dtype, block, fmt):
         assert len(alone) == 2 and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(alone, pair))
 
 
+@pytest.mark.parametrize("K", [*range(2, 10), *range(121, 137)])
+def test_quantize_every_remainder_of_columns(exts, dev, K):
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(5, K, generator=torch.Generator().manual_seed(K)).to(dtype)
+        got = exts["proj"].fp8_quantize(x.to(dev), rows=True, columns=True)
+        for (codes, scales), t in ((got[:2], x), (got[2:], x.t())):
+            rc, rs = _quantize64(t, 1, E4)
+            assert torch.equal(scales.view(torch.uint8).cpu(), rs)
+            got_c = codes.view(torch.uint8).cpu()
+            assert ((got_c == rc) | ((got_c & 0x7f == 0) & (rc & 0x7f == 0))).all()
+
+
 @pytest.mark.parametrize("block", [1, 128])
 def test_quantize_not_finite(exts, dev, block):
     x = torch.randn(200, 300, generator=torch.Generator().manual_seed(1))
