@@ -2,6 +2,7 @@
 //   rmsnorm.block_norm, rmsnorm.block_norm_backward, proj.fp8_quantize, proj.fp8_matmul
 // Errors surface as RuntimeError; launches go to torch's current HIP stream of
 // the tensors' device.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -138,8 +139,14 @@ std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gat
                             const Opt& scale, double residual_scale, const std::string& act, double eps, bool quantize,
                             bool store_h, bool stats, bool inplace) {
     const Operands o = operands(y, residual, gate, post_gamma, gamma, scale);
+    const int a = act_of(act);
     TORCH_CHECK(store_h || quantize || given(gamma), "block_norm: store_h=False leaves nothing to write");
     TORCH_CHECK(!inplace || (given(residual) && store_h), "block_norm: inplace writes h over residual");
+    if (inplace) {  // a row of an operand may be written only by the workgroup that reads it
+        at::assert_no_partial_overlap(*residual, y);
+        for (const Opt* t : {&gate, &post_gamma, &gamma, &scale})
+            if (given(*t)) at::assert_no_partial_overlap(*residual, **t);
+    }
     const c10::DeviceGuard guard(y.device());
     std::vector<Opt> out(stats ? 6 : 4);
     Rows h, n;
@@ -168,7 +175,7 @@ std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gat
     }
     if (o.R == 0) return out;
     check_status(gdn_block_norm_hip(o.y.ptr, o.y.ld, o.residual.ptr, o.residual.ld, o.gate.ptr, o.gate.ld, o.rows_per_gate,
-                                    o.post_gamma, o.gamma, o.scale, static_cast<float>(residual_scale), act_of(act),
+                                    o.post_gamma, o.gamma, o.scale, static_cast<float>(residual_scale), a,
                                     static_cast<float>(eps), h.ptr, h.ld, n.ptr, n.ld, codes, ldc, scales, lds, ry, rh, o.R, o.D,
                                     o.ty, o.tr, o.tp, stream_of(y)),
                  "block_norm");
@@ -179,6 +186,7 @@ std::vector<Opt> block_norm_backward(const Opt& dh, const Opt& dn, const Tensor&
                                      const Opt& post_gamma, const Opt& gamma, const Opt& scale, double residual_scale,
                                      const std::string& act, const Opt& rstd_y, const Opt& rstd_h) {
     const Operands o = operands(y, residual, gate, post_gamma, gamma, scale);
+    const int a = act_of(act);
     TORCH_CHECK(given(dh) || given(dn), "block_norm_backward: dh or dn is needed");
     Rows rdh, rdn;
     if (given(dh)) {
@@ -222,7 +230,7 @@ std::vector<Opt> block_norm_backward(const Opt& dh, const Opt& dn, const Tensor&
     auto ptr = [&](int i) { return given(out[i]) ? out[i]->data_ptr() : nullptr; };
     check_status(gdn_block_norm_bwd_hip(rdh.ptr, rdh.ld, rdn.ptr, rdn.ld, o.y.ptr, o.y.ld, o.residual.ptr, o.residual.ld,
                                         o.gate.ptr, o.gate.ld, o.rows_per_gate, o.post_gamma, normed ? o.gamma : nullptr, o.scale,
-                                        static_cast<float>(residual_scale), act_of(act), ry, rh, ptr(0), ptr(1), ptr(2), ptr(3),
+                                        static_cast<float>(residual_scale), a, ry, rh, ptr(0), ptr(1), ptr(2), ptr(3),
                                         normed ? ptr(4) : nullptr, ptr(5), o.R, o.D, o.ty, o.tr, o.tp,
                                         bytes ? ws.data_ptr() : nullptr, bytes, stream_of(y)),
                  "block_norm_backward");

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
                 if (VEC && !inside(u, e)) h[u][e] = 0.f;
                 if (VEC || inside(u, e)) ss = fmaf(h[u][e], h[u][e], ss);
             }
-            if (p.h && live) store8<TR, VEC>(p.h, r * p.ldh, 8 * (lane + LPR * u), D, h[u]);
+            if (p.h && live) store8<TR, VEC, false>(p.h, r * p.ldh, 8 * (lane + LPR * u), D, h[u]);
         }
         inv = 1.f;
         if (p.gamma) {
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
                     if (VEC && !inside(u, e)) h[u][e] = 0.f;
                 }
             }
-            if (p.n && live) store8<TY, VEC>(p.n, r * p.ldn, c, D, h[u]);
+            if (p.n && live) store8<TY, VEC, false>(p.n, r * p.ldn, c, D, h[u]);
             if (p.codes) {
                 if constexpr (!VEC) to_natural(h[u], c - vector_at(c, D), D);
                 const uint32_t s = Fp8<GDN_E4M3>::scale_byte(max16(amax8(h[u])));
@@ -172,7 +172,7 @@ extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residu
     if (!types_ok(type_y, type_r, type_p))
         return fail(GDN_ERR_UNSUPPORTED, "block_norm: types %d, %d, %d of y, residual and parameters", type_y, type_r, type_p);
     if (act < GDN_ACT_NONE || act > GDN_ACT_TANH) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: act=%d", act);
-    if (!y || (!h && !n && !codes)) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: y or every output is null");
+    if ((R > 0 && !y) || (!h && !n && !codes)) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: y or every output is null");
     if (!gamma && (n || rstd_h)) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: n and rstd_h need gamma");
     if (!post_gamma && rstd_y) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rstd_y needs post_gamma");
     if (gate && rows_per_gate <= 0) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rows_per_gate=%lld", (long long)rows_per_gate);
@@ -198,7 +198,8 @@ extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residu
     return with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
         return with_row_shape<false>(p.D, vec, [&](auto lpr, auto nv, auto v) {
             constexpr int LPR = decltype(lpr)::value, threads = LPR <= 64 ? 256 : LPR;
-            const int all = (p.R + slots_of(LPR) - 1) / slots_of(LPR);
+            const int all = static_cast<int>((R + slots_of(LPR) - 1) / slots_of(LPR));
+            if (!gdn_host::grid_fits(all, threads)) return fail(GDN_ERR_UNSUPPORTED, "block_norm: R=%lld rows of %lld are too many for a launch", (long long)R, (long long)D);
             const dim3 grid(LPR == 1024 && all > 256 ? 256 : all), block(threads);
             hipLaunchKernelGGL((gdn_block_norm_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
                                grid, block, 0, static_cast<hipStream_t>(stream), p);

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
         }
         if (p.dresidual && live) {
 #pragma unroll
-            for (int u = 0; u < NV; ++u) store8<TR, VEC>(p.dresidual, r * D, 8 * (lane + LPR * u), D, dH[u]);
+            for (int u = 0; u < NV; ++u) store8<TR, VEC, true>(p.dresidual, r * D, 8 * (lane + LPR * u), D, dH[u]);
         }
 
         // dgate, the column sums, and z (which takes dH's place)
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
                 if (inside(u, e)) q = fmaf(dH[u][e], yn[u][e], q);
             }
             add(0, u, ea);
-            if (p.dgate && live) store8<TY, VEC>(p.dgate, r * D, 8 * (lane + LPR * u), D, dg);
+            if (p.dgate && live) store8<TY, VEC, true>(p.dgate, r * D, 8 * (lane + LPR * u), D, dg);
         }
         if (p.rstd_y) {
             q = row_sum<LPR>(q, sums[parity][1]) * p.inv_D;
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
         }
         if (live) {
 #pragma unroll
-            for (int u = 0; u < NV; ++u) store8<TY, VEC>(p.dy, r * D, 8 * (lane + LPR * u), D, dH[u]);
+            for (int u = 0; u < NV; ++u) store8<TY, VEC, true>(p.dy, r * D, 8 * (lane + LPR * u), D, dH[u]);
         }
         if (!more) break;
         base += step;
@@ -216,8 +216,8 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             const int c = 8 * (lane + LPR * u);
-            store8<float, VEC>(out, 0, c, D, kLds ? cols + (u * LPR + lane) * 8 : se[kLds ? 0 : u]);
-            store8<float, VEC>(out, D, c, D, kLds ? cols + ((NV + u) * LPR + lane) * 8 : sg[kLds ? 0 : u]);
+            store8<float, VEC, true>(out, 0, c, D, kLds ? cols + (u * LPR + lane) * 8 : se[kLds ? 0 : u]);
+            store8<float, VEC, true>(out, D, c, D, kLds ? cols + ((NV + u) * LPR + lane) * 8 : sg[kLds ? 0 : u]);
         }
     } else {
         constexpr int kC = LPR * NV * 8;

@@ -191,6 +191,8 @@ __device__ __forceinline__ void wait_vm() {
 namespace gdn_host {
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int check_launch(const char* kernel);
+// Whether a launch of that many workgroups has fewer than 2^32 threads, what one can have.
+inline bool grid_fits(long long groups, int threads) { return groups <= 0xffffffffLL / threads; }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 // Argument checks of gdn_decode_hip (defined in decode.hip): GDN_OK when the
 // call would launch (or, for B == 0, do nothing), else the error status.

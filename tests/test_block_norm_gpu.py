@@ -165,6 +165,37 @@ def test_store_h_and_inplace(exts, dev):
     assert h3.data_ptr() == keep["residual"].data_ptr() and torch.equal(h3, h) and torch.equal(n3, n)
 
 
+@pytest.mark.parametrize("D", [513, 517, 1001, 2049])
+def test_inplace_where_lanes_share_columns(exts, dev, D):
+    """The row's last lane reads columns of the lane before it, which here may lie
+    in another wave and have h written already."""
+    for post in (True, False):
+        v = _inputs((700, D), post=post)
+        f = exts["rmsnorm"].block_norm
+        h, n, _, _ = f(**v, act="silu")
+        keep = dict(v, residual=v["residual"].clone())
+        h2, n2, _, _ = f(**keep, act="silu", inplace=True)
+        assert torch.equal(h2, h) and torch.equal(n2, n)
+
+
+def test_inplace_overlap(exts, dev):
+    """The residual itself as another operand is read before it is written; parts
+    of it in other rows' places are refused."""
+    f = exts["rmsnorm"].block_norm
+    v = _inputs((6, 300))
+    h, n, _, _ = f(v["y"], residual=v["y"], gamma=v["gamma"])
+    y = v["y"].clone()
+    h2, n2, _, _ = f(y, residual=y, gamma=v["gamma"], inplace=True)
+    assert h2.data_ptr() == y.data_ptr() and torch.equal(h2, h) and torch.equal(n2, n)
+    buf = torch.zeros(7, 300, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="memory location"):
+        f(buf[:6], residual=buf[1:], inplace=True)
+    with pytest.raises(RuntimeError, match="memory location"):
+        f(v["y"], residual=buf[:6], gamma=buf[2], inplace=True)
+    with pytest.raises(RuntimeError, match="act must be"):
+        f(buf[:0], act="gelu")
+
+
 def test_strided_rows(exts, dev):
     """Operands that are column slices of a wider buffer, 16-byte aligned or not."""
     for off, D in ((64, 256), (3, 256), (64, 250)):
