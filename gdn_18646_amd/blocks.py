@@ -98,12 +98,18 @@ class Fp8Weight:
         self.codes_t, self.scales_t = out[2:] if transposed else (None, None)
 
 
+def _as_rows(x, K):
+    """x [..., K] as rows for the quantisation; expanded and transposed ones are copied."""
+    x = x.reshape(-1, K)
+    return x if x.stride(1) == 1 and x.stride(0) >= K else x.contiguous()
+
+
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, record):
         proj = compile_kernels()["proj"]
         need_x, need_w = (record and need for need in ctx.needs_input_grad[:2])
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _as_rows(x, x.shape[-1])
         q = proj.fp8_quantize(x2, rows=True, columns=need_w)
         w = weight if isinstance(weight, Fp8Weight) else Fp8Weight(weight, transposed=need_x)
         if need_x and w.codes_t is None:
@@ -121,7 +127,7 @@ class _Fp8Linear(torch.autograd.Function):
         xt, xts, wt, wts = ctx.saved_tensors
         N, K = ctx.sizes
         need_x, need_w = ctx.needs_input_grad[:2]
-        d = proj.fp8_quantize(dy.reshape(-1, N), dtype=torch.float8_e5m2, rows=need_x, columns=need_w)
+        d = proj.fp8_quantize(_as_rows(dy, N), dtype=torch.float8_e5m2, rows=need_x, columns=need_w)
         dx = dw = None
         if need_x:
             dx = proj.fp8_matmul(d[0], d[1], wt, wts, out_dtype=ctx.dtypes[0]).reshape(ctx.shape)
@@ -142,6 +148,6 @@ def fp8_linear(x, weight):
     results.  In the backward pass the incoming gradient is quantised to e5m2 in
     blocks of 1 x 128 along each product's own sum, x along its tokens.
     """
-    if x.shape[-1] != weight.shape[1]:
+    if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"fp8_linear: x [..., {x.shape[-1]}] and weight {tuple(weight.shape)}")
     return _Fp8Linear.apply(x, weight, torch.is_grad_enabled())

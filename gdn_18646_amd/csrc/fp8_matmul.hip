@@ -123,6 +123,7 @@ int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t str
     if (p.M <= 4 || (p.M <= 16 && p.N <= 4096)) {
         const auto few = [&](auto out32, auto waves) {
             constexpr int W = decltype(waves)::value;
+            if (!gdn_host::grid_fits((p.N + 15) / 16, 64 * W)) return gdn_host::fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: N=%d is too large for a launch", p.N);
             hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, scales);
             return gdn_host::check_launch("gdn_fp8_few_kernel");
         };

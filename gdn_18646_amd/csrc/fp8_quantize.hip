@@ -140,7 +140,7 @@ extern "C" int gdn_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int6
     if (type_x != GDN_BF16 && type_x != GDN_F32) return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: type %d of x", type_x);
     if (format != GDN_E4M3 && format != GDN_E5M2) return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: format %d", format);
     const int64_t MB = (M + kBlk - 1) / kBlk, KB = (K + kBlk - 1) / kBlk;
-    if (M > 0x7fffffffLL - kBlk || K > 0x7fffffffLL - kBlk || MB * KB > 0x7fffffffLL)
+    if (M > 0x7fffffffLL - kBlk || K > 0x7fffffffLL - kBlk || MB * KB > 0x7fffffffLL || !gdn_host::grid_fits(MB * KB, 512))
         return fail(GDN_ERR_UNSUPPORTED, "fp8_quantize: problem too large");
     if (!codes && !codes_t) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_quantize: no output");
     if (M == 0 || K == 0) return GDN_OK;

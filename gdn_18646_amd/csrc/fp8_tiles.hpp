@@ -561,6 +561,8 @@ int launch_scaled(const MatmulParams& p, hipStream_t stream) {
     const int n_tok = (p.M + TL::toks - 1) / TL::toks, n_col = (p.N + TL::cols - 1) / TL::cols;
     const unsigned tiles = static_cast<unsigned>(n_tok) * n_col;
     const dim3 grid(TL::PHASED && tiles > 256 ? 256 : tiles);  // phased: a workgroup a CU
+    if (!gdn_host::grid_fits(grid.x, TL::waves * 64))
+        return gdn_host::fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: M=%d N=%d are too large for a launch", p.M, p.N);
     hipLaunchKernelGGL((gdn_fp8_matmul_kernel<TL, FA, FB, SB, OUT32>), grid, dim3(TL::waves * 64), 0, stream, p, n_tok, n_col);
     return gdn_host::check_launch("gdn_fp8_matmul_kernel");
 }

@@ -22,7 +22,7 @@ class GDNStack:
     post_gammas, scales: a tensor [D] or None for each layer (None: none at all).
     """
 
-    def __init__(self, layers, final_gamma=None, post_gammas=None, scales=None, residual_scale=1.0, eps=1e-6, exts=None):
+    def __init__(self, layers, final_gamma=None, post_gammas=None, scales=None, residual_scale=1.0, exts=None):
         if not layers:
             raise ValueError("a stack needs a layer")
         self.layers = list(layers)
@@ -33,13 +33,17 @@ class GDNStack:
             raise ValueError(f"{n} layers, {len(self.post_gammas)} post_gammas and {len(self.scales)} scales")
         if any(layer.D != self.layers[0].D for layer in self.layers):
             raise ValueError("the layers differ in D")
-        self.final_gamma, self.residual_scale, self.eps = final_gamma, float(residual_scale), eps
+        self.final_gamma, self.residual_scale = final_gamma, float(residual_scale)
         self._norm = (exts if exts is not None else compile_kernels())["rmsnorm"]
+
+    def _check_states(self, states):
+        if states is not None and len(states) != len(self.layers):
+            raise ValueError(f"{len(self.layers)} layers and {len(states)} states")
 
     def _join(self, i, y, h, gamma, **kw):
         """(h, n) after layer i."""
         h, n, _, _ = self._norm.block_norm(y, residual=h, post_gamma=self.post_gammas[i], gamma=gamma, scale=self.scales[i],
-                                           residual_scale=self.residual_scale, eps=self.eps, **kw)
+                                           residual_scale=self.residual_scale, eps=1e-6, **kw)  # the layers' own
         return h, n
 
     @torch.no_grad()
@@ -47,6 +51,7 @@ class GDNStack:
         """x [B, T, D] bf16 -> out [B, T, D]; with ``return_state`` also a list of
         the layers' decode states.  The other arguments are the layer's, ``states``
         a state for each layer."""
+        self._check_states(states)
         h, xn, new = x.contiguous(), None, []
         for i, layer in enumerate(self.layers):
             y = layer.forward(h if xn is None else None, mask=mask, return_state=return_state,
@@ -67,6 +72,9 @@ class GDNStack:
     def decode(self, x, states, inplace=False):
         """One token: x [B, 1, D] -> (out [B, 1, D], states).  The layers' own steps
         norm their inputs, so between them only the residual is joined."""
+        if states is None:
+            raise ValueError("decode needs a state for each layer")
+        self._check_states(states)
         h, n, new = x.contiguous(), None, []
         for i, layer in enumerate(self.layers):
             y, state = layer.decode(h, states[i], inplace=inplace)

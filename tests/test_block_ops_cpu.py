@@ -22,7 +22,7 @@ def _norm(**k):
 
 @pytest.mark.parametrize("bad,match", [
     (dict(R=-1), "INVALID_ARGUMENT"), (dict(D=0), "INVALID_ARGUMENT"), (dict(D=16385), "UNSUPPORTED.*16384"),
-    (dict(R=1 << 31), "UNSUPPORTED"), (dict(ty=F32), "UNSUPPORTED.*types"), (dict(tp=3), "UNSUPPORTED.*types"),
+    (dict(R=1 << 31), "UNSUPPORTED"), (dict(R=(1 << 31) - 1), "too many"), (dict(ty=F32), "UNSUPPORTED.*types"), (dict(tp=3), "UNSUPPORTED.*types"),
     (dict(tr=F32), "UNSUPPORTED.*types"), (dict(act=4), "act=4"), (dict(y=None), "null"), (dict(h=None, n=None), "null"),
     (dict(gamma=None), "need gamma"), (dict(gamma=None, n=None, rh=FAKE), "need gamma"), (dict(post=None, ry=FAKE), "needs post_gamma"),
     (dict(rpg=0), "rows_per_gate"), (dict(codes=FAKE), "codes"), (dict(codes=FAKE, scales=FAKE, ldc=128, lds=4), "codes"),
@@ -35,6 +35,7 @@ def test_block_norm_refusals(bad, match):
 
 def test_no_rows_is_no_call():
     _norm(R=0, residual=None)
+    _norm(R=0, y=None)
 
 
 def _bwd(**k):
@@ -108,7 +109,7 @@ def _mm(**k):
     (dict(out=None), "null"), (dict(a=FAKE + 8), "16-byte"), (dict(ldb=240), "16-byte"), (dict(ldb=264), "16-byte"),
     (dict(ldas=32), "a's scales"), (dict(ldas=40), "a's scales"), (dict(sa=FAKE + 4), "a's scales"), (dict(ldbs=1), "b's scales"),
     (dict(brows=1, ldbs=96), "b's scales"), (dict(brows=1, ldbs=104), "b's scales"), (dict(tsb=F32, sb=FAKE + 2), "b's scales"),
-    (dict(ldo=99), "ldo"), (dict(out=FAKE + 1), "unaligned")])
+    (dict(ldo=99), "ldo"), (dict(M=1, N=1 << 30, ldo=1 << 30), "N=.*too large for a launch"), (dict(out=FAKE + 1), "unaligned")])
 def test_product_refusals(bad, match):
     with pytest.raises(GdnError, match=match):
         _mm(**bad)

@@ -71,6 +71,20 @@ def test_fp8_linear_partial_gradients(dev):
     assert y.shape == (0, 128) and dx.shape == (0, 256) and (dw == 0).all()
 
 
+def test_fp8_linear_of_expanded_and_transposed(dev):
+    """Layouts that autograd and views make: a sum's expanded gradient, expanded and
+    transposed inputs give what their copies give."""
+    x, w = _rand((40, 256), torch.bfloat16, dev, 1), _rand((128, 256), torch.bfloat16, dev, 2, 0.05)
+    y = fp8_linear(x, w)
+    got = torch.autograd.grad(y.sum(), (x, w))
+    want = torch.autograd.grad(fp8_linear(x, w), (x, w), torch.ones_like(y))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for t in (x.detach()[:1].expand(40, 256), x.detach().t().contiguous().t(), x.detach()[:, :1].expand(40, 256)):
+        assert torch.equal(fp8_linear(t, w), fp8_linear(t.contiguous(), w))
+    with pytest.raises(ValueError, match="weight"):
+        fp8_linear(x, w[0])
+
+
 def test_block_norm_gradients_through_autograd(dev):
     """Expanded, missing and accumulated gradients reach the kernel as they should."""
     D = 512

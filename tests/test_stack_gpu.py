@@ -90,3 +90,12 @@ def test_refusals(layers, dev):
         GDNStack([])
     with pytest.raises(ValueError, match="post_gammas"):
         GDNStack(layers, post_gammas=[None])
+    stack = GDNStack(layers)
+    states = stack.init_decode_state(1)
+    x = _x((1, 1, D), dev)
+    for call in (lambda s: stack.decode(x, s, inplace=True), lambda s: stack.forward(x, states=s)):
+        with pytest.raises(ValueError, match="2 states"):
+            call(states[:2])
+    with pytest.raises(ValueError, match="state for each layer"):
+        stack.decode(x, None)
+    assert all((t == 0).all() for s in states for t in s.values())
