@@ -8,7 +8,11 @@
 //
 // What bounds it: HBM for many rows (each input read once, each output written
 // once, two row sums between them that never leave the registers), the one
-// chain of loads, sums and stores for a few.  Rows of up to 4096 columns have a
+// chain of loads, sums and stores for a few (16384 x 2048, three inputs and two
+// outputs in bf16: 63 us, 5.3 TB/s; 24000 x 256, a gated head norm: 10.6 us;
+// 1 x 2048: 3.1 us).  Non-temporal stores take 3-13% off the kernel and give it
+// back to whoever reads n next (16384 x 2048 with a reader: 85.4 us, 86.4 with
+// them).  Rows of up to 4096 columns have a
 // workgroup each or share one; rows above that keep sixteen waves busy alone, and
 // a workgroup a CU walks them, the next row's loads under way while a row is
 // worked on (4096 x 8192: 78 us against 102 with a workgroup a row; walking rows

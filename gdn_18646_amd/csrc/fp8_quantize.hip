@@ -8,7 +8,9 @@
 // transposed codes pass through LDS so that both layouts leave in whole
 // 128-byte lines.  What bounds it: HBM (2 bytes read, 1 or 2 written a value)
 // above some 1000 tiles, below that a tile's chain of loads, maxima and stores,
-// which is why eight waves share one.
+// which is why eight waves share one (8224 x 2048 by blocks both ways: 11.6 us,
+// 5.7 TB/s, 14.1 with four waves and conflicting transposition; 1500 x 2048 along
+// its rows: 3.7 us).
 #include "block_norm.hpp"
 #include "fp8_blocks.hpp"
 

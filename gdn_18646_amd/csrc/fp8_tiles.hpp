@@ -2,14 +2,26 @@
 //   out[m, n] = sum over blocks kb of a_scale[m, kb] b_scale[n, kb] sum_k a[m, k] b[n, k]
 // with fp32 sums, one rounding where out is written.
 //
-// In tiles of columns x tokens (W = b, x = a).  A stage is one block of 128 k: 128-byte rows, which reach LDS by DMA
-// in a ring, every 8 lanes of a copy one whole line, placed with an XOR swizzle
-// that keeps the fragment reads at linear-read speed; the stage's scales come
-// with it.  bf16 results: one MFMA 16x16x128 takes a block: e8m0 scales are its
+// In tiles of columns x tokens (W = b, x = a).  A stage is one block of 128 k:
+// 128-byte rows, which reach LDS by DMA in a ring, every 8 lanes of a copy one
+// whole line, placed with an XOR swizzle that keeps the fragment reads at
+// linear-read speed; the stage's scales come with it.  bf16 results: one MFMA 16x16x128 takes a block: e8m0 scales are its
 // own scale operands and cost nothing; fp32 scales multiply its result on the
 // VALU, into the accumulator.  fp32 results: codes become bf16 in registers,
 // times their e8m0 scale, and the block takes four MFMA 16x16x32, whose sums
 // keep every bit that fp32 has.
+//
+// What bounds it: the matrix cores for large products, and there the card's
+// power: 8192 x 8192 x 8192 takes 413 us (2.66 PFLOP/s) with random codes and 345
+// with zeros.  Waves of 128 x 128 (half the LDS reads a product) changed nothing
+// for that reason.  A 256 x 256 tile takes 1.2-1.5 us a block of K and some 6.6
+// to begin, fill the ring and store, of which a persistent workgroup hides the
+// filling behind the stores before it: 16384 x 6176 x 2048, 193 us.  Running the
+// stages on over tile borders (8192 x 8192 x 8192: 420 us), non-temporal stores
+// (213 against 185 us at 16384 x 6144 x 2048) and staggered starts were slower or
+// no faster.  Products of one round of tiles are bound by how many of the 256 CUs
+// have one (1500 x 8224 x 2048: 198 tiles, 28 us, 1.8 PFLOP/s), small ones by a
+// tile's chain of copies, which groups of waves on different blocks shorten.
 #pragma once
 
 #include "fp8_matmul.hpp"
