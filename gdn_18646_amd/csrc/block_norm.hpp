@@ -213,22 +213,17 @@ __device__ __forceinline__ float row_sum(float v, float* slot) {
 // Lanes a row and vectors a lane for rows of D: f(LPR, NV).  Up to 512 columns a
 // part of a wave or a wave, above that a workgroup, one vector a lane as far as
 // that goes (the backward pass, which holds three times as much, has two a lane
-// from 4096 columns on, sixteen waves having too few registers).  Rows that
-// 16-byte accesses do not fit run on some of these forms.
+// from 4096 columns on, sixteen waves having too few registers).
 template <bool BWD, class F>
 int with_row_shape(int D, bool vec, F&& f) {
     using std::integral_constant;
     const auto shape = [&](auto v) {
-        if constexpr (decltype(v)::value) {
-            if (D <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, v);
-            if (D <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, v);
-        }
+        if (D <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, v);
+        if (D <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, v);
         if (D <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, v);
         if (D <= 1024) return f(integral_constant<int, 128>{}, integral_constant<int, 1>{}, v);
         if (D <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, v);
-        if constexpr (decltype(v)::value) {
-            if (D <= 4096) return f(integral_constant<int, 512>{}, integral_constant<int, 1>{}, v);
-        }
+        if (D <= 4096) return f(integral_constant<int, 512>{}, integral_constant<int, 1>{}, v);
         if constexpr (BWD) {
             if (D <= 8192) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{}, v);
         } else {

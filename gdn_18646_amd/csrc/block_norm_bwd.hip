@@ -258,12 +258,14 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) __attribute__((amdgpu_waves_
     }
 }
 
-// Adds the sums of `chunks` workgroups of each group (blockIdx.y), 16 columns a
-// workgroup, 64 at a time, and writes what follows from them: the gradient of a
-// shared gate row, and either the parameters' gradients (one group) or the
-// group's part of them (part2).
+// Adds the sums of `chunks` workgroups of each of `groups` groups (one, at
+// blockIdx.y, where there are more than kGroups), 16 columns a workgroup, 64 rows
+// of sums at a time, and writes what follows from them: the gradient of a shared
+// gate row, and the parameters' gradients or (part2) the group's part of them.
+constexpr int kGroups = 32;
 struct SumParams {
     const float* part;
+    int groups, share;  // share: the 64 rows' part for a group, 64 / (groups up to a power of two)
     int chunks, D;
     float rs;
     const void *gate, *post_gamma, *scale;
@@ -276,13 +278,13 @@ struct SumParams {
 template <class TY, class TP>
 __global__ __launch_bounds__(1024) void gdn_block_norm_sum_kernel(SumParams p) {
     __shared__ float lds[2][64][17];
-    const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, d = blockIdx.x * 16 + col, D = p.D;
-    const long long g = blockIdx.y;
+    const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, d = blockIdx.x * 16 + col, D = p.D, S = p.share;
+    const long long first = blockIdx.y;
     float e = 0.f, s = 0.f;
-    if (d < D) {
-        const float* src = p.part + static_cast<size_t>(g) * p.chunks * 2 * D + d;
+    if (d < D && lane / S < p.groups) {
+        const float* src = p.part + static_cast<size_t>(first + lane / S) * p.chunks * 2 * D + d;
 #pragma unroll 4
-        for (int i = lane; i < p.chunks; i += 64) {
+        for (int i = lane % S; i < p.chunks; i += S) {
             e += src[static_cast<size_t>(i) * 2 * D];
             s += src[static_cast<size_t>(i) * 2 * D + D];
         }
@@ -290,26 +292,37 @@ __global__ __launch_bounds__(1024) void gdn_block_norm_sum_kernel(SumParams p) {
     lds[0][lane][col] = e;
     lds[1][lane][col] = s;
     __syncthreads();
-    if (threadIdx.x >= 32) return;
-    float sum = 0.f;  // threads 0 .. 15 of e, 16 .. 31 of s
+    const float pg = d < D && p.post_gamma ? static_cast<float>(static_cast<const TP*>(p.post_gamma)[d]) : 1.f;
+    const float sc = d < D && p.scale ? static_cast<float>(static_cast<const TP*>(p.scale)[d]) : 1.f;
+    // Of group lane / 2, the sum of e (even lanes; then what it makes for the gate) or of s.
+    const int g = lane >> 1, which = lane & 1;
+    float sum = 0.f;
+    if (g < p.groups) {
+        for (int i = 0; i < S; ++i) sum += lds[which][g * S + i][col];
+        if (which == 0) {
+            sum *= p.rs;
+            if (p.gate && d < D) {
+                float x[8], a[8], da[8];
 #pragma unroll
-    for (int i = 0; i < 64; ++i) sum += lds[threadIdx.x >> 4][i][col];
-    s = __shfl(sum, 16 + col);
+                for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<const TY*>(p.gate)[(first + g) * p.ldg + d]);
+                act8<true>(x, p.act, a, da);
+                if (p.dgate) static_cast<TY*>(p.dgate)[(first + g) * D + d] = static_cast<TY>(sum * pg * sc * da[0]);
+                sum *= a[0];
+            }
+        }
+    }
+    __syncthreads();
+    lds[which][g][col] = sum;
+    __syncthreads();
     if (threadIdx.x >= 16 || d >= D) return;
-    e = sum * p.rs;
-    const float pg = p.post_gamma ? static_cast<float>(static_cast<const TP*>(p.post_gamma)[d]) : 1.f;
-    const float sc = p.scale ? static_cast<float>(static_cast<const TP*>(p.scale)[d]) : 1.f;
-    if (p.gate) {
-        float x[8], a[8], da[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<const TY*>(p.gate)[g * p.ldg + d]);
-        act8<true>(x, p.act, a, da);
-        if (p.dgate) static_cast<TY*>(p.dgate)[g * D + d] = static_cast<TY>(e * pg * sc * da[0]);
-        e *= a[0];
+    e = s = 0.f;
+    for (int i = 0; i < p.groups; ++i) {
+        e += lds[0][i][col];
+        s += lds[1][i][col];
     }
     if (p.part2) {
-        p.part2[static_cast<size_t>(g) * 2 * D + d] = e;
-        p.part2[static_cast<size_t>(g) * 2 * D + D + d] = s;
+        p.part2[static_cast<size_t>(first) * 2 * D + d] = e;
+        p.part2[static_cast<size_t>(first) * 2 * D + D + d] = s;
         return;
     }
     if (p.dpost_gamma) static_cast<TP*>(p.dpost_gamma)[d] = static_cast<TP>(e * sc);
@@ -345,7 +358,7 @@ Plan plan_rows(long long R, long long D, long long per) {
 extern "C" size_t gdn_block_norm_bwd_workspace_bytes(int64_t R, int64_t D, int64_t rows_per_gate) {
     if (R <= 0 || D <= 0) return 0;
     const Plan q = plan_rows(R, D, rows_per_gate);
-    return static_cast<size_t>(q.groups) * (q.chunks + (q.groups > 1 ? 1 : 0)) * 2 * D * sizeof(float);
+    return static_cast<size_t>(q.groups) * (q.chunks + (q.groups > kGroups ? 1 : 0)) * 2 * D * sizeof(float);
 }
 
 extern "C" int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* dn, int64_t lddn, const void* y, int64_t ldy,
@@ -419,16 +432,20 @@ extern "C" int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* 
     t.part = part, t.chunks = R > 0 ? q.chunks : 0, t.D = static_cast<int>(D);
     t.post_gamma = post_gamma, t.scale = scale, t.act = act, t.dpost_gamma = dpost_gamma, t.dscale = dscale, t.dgamma = dgamma;
     if (shared && R > 0) t.gate = gate, t.ldg = ldg, t.dgate = dgate;
-    float* const part2 = q.groups > 1 ? part + static_cast<size_t>(q.groups) * q.chunks * 2 * D : nullptr;
-    t.part2 = part2;
+    // Up to kGroups groups in one launch; more in one that sums each and one that adds them.
+    const bool apart = q.groups > kGroups;
+    float* const part2 = apart ? part + static_cast<size_t>(q.groups) * q.chunks * 2 * D : nullptr;
+    t.part2 = part2, t.groups = apart ? 1 : static_cast<int>(q.groups);
+    t.share = 64;
+    while (t.share * t.groups > 64) t.share /= 2;
     return with_types(type_y, type_r, type_p, [&](auto ty, auto, auto tp) {
-        const auto launch = [&](long long groups) {
-            hipLaunchKernelGGL((gdn_block_norm_sum_kernel<decltype(ty), decltype(tp)>), dim3((t.D + 15) / 16, static_cast<unsigned>(groups)),
+        const auto launch = [&](long long count) {
+            hipLaunchKernelGGL((gdn_block_norm_sum_kernel<decltype(ty), decltype(tp)>), dim3((t.D + 15) / 16, static_cast<unsigned>(count)),
                                dim3(1024), 0, s, t);
             return gdn_host::check_launch("gdn_block_norm_sum_kernel");
         };
-        const int st = launch(q.groups);
-        if (st != GDN_OK || !part2) return st;
+        const int st = launch(apart ? q.groups : 1);
+        if (st != GDN_OK || !apart) return st;
         t.part = part2, t.chunks = static_cast<int>(q.groups), t.part2 = nullptr, t.rs = 1.f, t.gate = nullptr, t.dgate = nullptr;
         return launch(1);
     });

@@ -190,7 +190,6 @@ extern "C" int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, c
     p.a = a, p.b = b, p.a_scale = a_scale, p.b_scale = b_scale, p.out = out;
     p.lda = lda, p.ldb = ldb, p.lda_s = lda_s, p.ldb_s = ldb_s, p.ldo = ldo;
     p.M = static_cast<int>(M), p.N = static_cast<int>(N), p.K = static_cast<int>(K);
-    p.wide = aligned(out, 16) && ldo * static_cast<int64_t>(bo) % 16 == 0;
     const int scales = type_b_scale == GDN_F32 ? (b_block_rows == 1 ? gdn_fp8::kF32Row : gdn_fp8::kF32Block)
                                                : (b_block_rows == 1 ? gdn_fp8::kE8Row : gdn_fp8::kE8Block);
     const auto s = static_cast<hipStream_t>(stream);

@@ -14,7 +14,6 @@ struct MatmulParams {
     void* out;                   // [M, ldo] bf16 or fp32
     long long lda, ldb, lda_s, ldb_s, ldo;
     int M, N, K;
-    int wide;  // 16-byte stores fit
 };
 
 // b's scales: e8m0 or fp32, one a 128 x 128 block [ceil(N / 128)][ldb_s >= K / 128]
@@ -91,11 +90,11 @@ __device__ __forceinline__ void store_cols(const gdn_fp8::MatmulParams& p, long 
     using T = std::conditional_t<F32, float, bf16>;
     typedef T vec __attribute__((ext_vector_type(NC)));
     T* const o = static_cast<T*>(p.out) + static_cast<size_t>(row) * p.ldo + col;
-    if (p.wide && col + NC <= p.N) {
+    if (col + NC <= p.N) {
         vec w;
 #pragma unroll
         for (int i = 0; i < NC; ++i) w[i] = static_cast<T>(v[i]);
-        *reinterpret_cast<vec*>(o) = w;
+        __builtin_memcpy(o, &w, sizeof(w));  // at any address: odd rows too leave in whole stores
         return;
     }
 #pragma unroll

@@ -311,6 +311,16 @@ def test_backward_without(exts, dev, gate, absent):
     _check_grads(_run_backward(exts, v, 1.0, act, dh, dn), ref, 111)
 
 
+@pytest.mark.parametrize("B,T,D", [(2, 300, 136), (5, 41, 700), (17, 3, 64), (31, 2, 130), (32, 9, 96), (33, 9, 96), (70, 2, 40)])
+def test_backward_of_shared_gates(exts, dev, B, T, D):
+    """Gates a sequence, around the number of them that one launch sums."""
+    for types in ("bf16", "fp32"):
+        v = _inputs((B, T, D), types, "sequence", seed=B)
+        g = torch.Generator().manual_seed(9)
+        dh, dn = (torch.randn((B, T, D), generator=g).to(v["y"].dtype).to(dev) for _ in range(2))
+        _check_grads(_run_backward(exts, v, 0.7, "tanh", dh, dn), _grads64(v, 0.7, "tanh", dh, dn)[0], B * T)
+
+
 def test_backward_against_differences(exts, dev):
     """Directional differences of the forward kernel itself, in fp32."""
     shape, act = (2, 5, 384), "silu"

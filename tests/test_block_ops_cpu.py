@@ -61,12 +61,13 @@ def test_block_norm_backward_refusals(bad, match):
 
 def test_backward_workspace_covers_the_launch():
     """Two fp32 sums a column for each workgroup, at most 512 of them and one a
-    row group; one set more a gate row where rows share gate rows."""
+    row group; one set more a gate row where rows share over 32 gate rows."""
     f = abi.load().gdn_block_norm_bwd_workspace_bytes
     assert f(0, 256, 1) == 0
     assert f(16384, 2048, 1) == 512 * 2 * 2048 * 4
     assert f(3, 2048, 1) == 3 * 2 * 2048 * 4
-    assert f(16384, 2048, 4096) == (512 + 4) * 2 * 2048 * 4
+    assert f(16384, 2048, 4096) == 512 * 2 * 2048 * 4
+    assert f(16384, 2048, 256) == (512 + 64) * 2 * 2048 * 4
     assert f(100, 128, 100) == 7 * 2 * 128 * 4
 
 
