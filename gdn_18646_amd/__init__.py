@@ -4,14 +4,15 @@ Native pieces (built in-tree by ``gdn_18646_amd._build``):
 
 * ``libgdn_amd.so`` — hand-written HIP kernels behind the C ABI declared in
   ``include/gdn_amd.h`` (decode, chunked prefill, varlen prefill, RMSNorm,
-  projection + conv + SiLU);
+  projection + conv + SiLU, block norms, 8-bit quantisation and products);
 * ``_gdn_ext`` — a thin torch binding that re-exports the reference project's
   module API over that ABI.
 
 ``compile_kernels()`` returns the same ``dict(rmsnorm, proj, prefill,
 decode)`` of modules that the reference's ``bench_gdn.compile_kernels()``
 returns (``bench_gdn.py:25-45``), so callers written against the reference
-work unchanged.  There is no fallback: if the native code is missing, these
+work unchanged.  ``blocks`` has the differentiable block norms and 8-bit linear
+layers on them, ``stack`` layers on a residual stream.  There is no fallback: if the native code is missing, these
 functions raise.
 """
 
