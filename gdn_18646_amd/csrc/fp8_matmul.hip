@@ -61,23 +61,27 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
 
 // What a call on a tile takes, us: c + rounds (a + b blocks of K), rounds of 256
 // workgroups, or, where two share a CU, of 512, and of up to 256 alone.  Fitted
-// to 114 products, 17 to 16384 tokens, N 512 to 8192, K 1024 to 4096 (kernels
-// back to back): the tile that the fit picks takes at most 1.16 times the best
-// one's time and 1.01 on average; 24 tiles were timed, those here are the ones
-// whose absence costs.
+// to 184 products, 17 to 16384 tokens, N 512 to 8192, K 800 to 4096 (kernels
+// back to back): the tile that the fit picks takes at most 1.02 times the best
+// one's time (fp32 results: 114 products, 1.16, 1.01 on average); 26 tiles were
+// timed, those here are the ones whose absence costs: 256 x 160 and 128 x 192 up
+// to 9%, where they make one round of what others make two of or a half (1500 x
+// 6176 x 2048: 22.7 us on 256 x 160, 24.3 on 256 x 192).
 struct TileCost {
     int tile, cols, toks, per_cu;
     float c, a1, b1, a2, b2;  // per_cu 2: alone (1) and two (2)
 };
 constexpr TileCost kBf16[] = {
-    {gdn_fp8::k256x256, 256, 256, 1, 0.f, 6.58f, 1.211f, 0.f, 0.f},
-    {gdn_fp8::k256x192, 256, 192, 1, 0.f, 5.86f, 1.081f, 0.f, 0.f},
-    {gdn_fp8::k256x128, 256, 128, 1, 0.f, 4.88f, 0.776f, 0.f, 0.f},
-    {gdn_fp8::k128x128, 128, 128, 1, 0.46f, 3.33f, 0.539f, 0.f, 0.f},
-    {gdn_fp8::k64x128, 64, 128, 1, 0.86f, 3.31f, 0.333f, 0.f, 0.f},
-    {gdn_fp8::k64x64, 64, 64, 1, 1.04f, 2.76f, 0.236f, 0.f, 0.f},
-    {gdn_fp8::k64x32, 64, 32, 1, 1.15f, 2.49f, 0.150f, 0.f, 0.f},
-    {gdn_fp8::k32x32, 32, 32, 2, 1.86f, 1.20f, 0.123f, 1.80f, 0.192f},
+    {gdn_fp8::k256x256, 256, 256, 1, 0.f, 6.93f, 1.177f, 0.f, 0.f},
+    {gdn_fp8::k256x192, 256, 192, 1, 0.f, 6.20f, 1.042f, 0.f, 0.f},
+    {gdn_fp8::k256x160, 256, 160, 1, 0.f, 5.69f, 0.921f, 0.f, 0.f},
+    {gdn_fp8::k256x128, 256, 128, 1, 0.f, 5.34f, 0.753f, 0.f, 0.f},
+    {gdn_fp8::k128x192, 128, 192, 1, 0.48f, 4.14f, 0.702f, 0.f, 0.f},
+    {gdn_fp8::k128x128, 128, 128, 1, 0.60f, 3.45f, 0.518f, 0.f, 0.f},
+    {gdn_fp8::k64x128, 64, 128, 1, 0.85f, 3.44f, 0.328f, 0.f, 0.f},
+    {gdn_fp8::k64x64, 64, 64, 1, 0.94f, 2.77f, 0.231f, 0.f, 0.f},
+    {gdn_fp8::k64x32, 64, 32, 1, 1.13f, 2.53f, 0.148f, 0.f, 0.f},
+    {gdn_fp8::k32x32, 32, 32, 2, 1.84f, 1.18f, 0.120f, 1.75f, 0.197f},
 };
 constexpr TileCost kF32[] = {
     {gdn_fp8::k128x128, 128, 128, 2, 0.85f, 2.61f, 0.957f, 4.54f, 1.676f},

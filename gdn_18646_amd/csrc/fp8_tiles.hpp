@@ -560,7 +560,9 @@ namespace gdn_fp8 {
 
 using Tile256x256 = Fp8Tile<4, 2, 4, 8, 2, 1, 1, true>;
 using Tile256x192 = Fp8Tile<4, 2, 4, 6, 2, 1, 1, true>;
+using Tile256x160 = Fp8Tile<4, 2, 4, 5, 2, 1, 1, true>;
 using Tile256x128 = Fp8Tile<4, 2, 4, 4, 3, 1, 1, true>;
+using Tile128x192 = Fp8Tile<2, 4, 4, 3, 3, 1, 1, true>;
 using Tile128x128 = Fp8Tile<2, 4, 4, 2, 4, 1>;
 using Tile128x128Pair = Fp8Tile<2, 4, 4, 2, 2, 2>;  // fp32 results: two workgroups a CU, one converts while the other multiplies
 using Tile64x128 = Fp8Tile<1, 4, 4, 2, 3, 1, 2>;
@@ -605,7 +607,9 @@ int launch_tile(int tile, int scales, bool f32, const MatmulParams& p, hipStream
     switch (tile) {
         case k256x256: return launch_tiled<Tile256x256, FA, FB, false>(scales, p, stream);
         case k256x192: return launch_tiled<Tile256x192, FA, FB, false>(scales, p, stream);
+        case k256x160: return launch_tiled<Tile256x160, FA, FB, false>(scales, p, stream);
         case k256x128: return launch_tiled<Tile256x128, FA, FB, false>(scales, p, stream);
+        case k128x192: return launch_tiled<Tile128x192, FA, FB, false>(scales, p, stream);
         default: return small(std::false_type{});
     }
 }

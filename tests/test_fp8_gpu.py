@@ -170,6 +170,15 @@ def test_product_in_two_launches(exts, dev, M, N, K, out, bscale, rows):
     _check(exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out), a, sa, b, sb)
 
 
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
+@pytest.mark.parametrize("fa,fb", [(E4, E4), (E5, E4)], ids=["e4e4", "e5e4"])
+@pytest.mark.parametrize("M,N,K", [(2499, 4090, 256), (2600, 2040, 384)])
+def test_product_of_one_round_of_tiles(exts, dev, M, N, K, fa, fb, bscale, rows):
+    """Sizes that tiles of 160 and of 192 tokens fit."""
+    a, sa, b, sb = _operands(M, N, K, fa, fb, bscale, rows, dev)
+    _check(exts["proj"].fp8_matmul(a, sa, b, sb), a, sa, b, sb)
+
+
 @pytest.mark.parametrize("M,N,K", [(3, 200, 256), (150, 300, 256)])
 def test_product_strides_and_scale_layouts(exts, dev, M, N, K):
     """Codes in wider rows, scales in any layout: the same bits."""

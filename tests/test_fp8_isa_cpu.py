@@ -14,7 +14,8 @@ import pytest
 from tests.test_isa_cpu import _assembly, _events, _function
 
 # columns: waves along columns, tokens, MFMA tiles of a wave along each, stages
-PHASED = {"256x256": (4, 2, 4, 8, 2), "256x192": (4, 2, 4, 6, 2), "256x128": (4, 2, 4, 4, 3)}
+PHASED = {"256x256": (4, 2, 4, 8, 2), "256x192": (4, 2, 4, 6, 2), "256x160": (4, 2, 4, 5, 2), "256x128": (4, 2, 4, 4, 3),
+          "128x192": (2, 4, 4, 3, 3)}
 ROW_SCALES = 1
 
 
@@ -29,7 +30,7 @@ def _kernels(asm, tile="", scales=r"\d"):
 
 def test_no_tile_spills(asm):
     names = _kernels(asm)
-    assert len(names) == 4 * (8 + 5), names  # layouts of b's scales x tiles of bf16 and of fp32 results
+    assert len(names) == 4 * (10 + 5), names  # layouts of b's scales x tiles of bf16 and of fp32 results
     for name in names:
         assert not any("scratch_" in ln for ln in _function(asm, name)), name
 
