@@ -172,10 +172,20 @@ def test_product_in_two_launches(exts, dev, M, N, K, out, bscale, rows):
 
 @pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
 @pytest.mark.parametrize("fa,fb", [(E4, E4), (E5, E4)], ids=["e4e4", "e5e4"])
-@pytest.mark.parametrize("M,N,K", [(2499, 4090, 256), (2600, 2040, 384)])
+@pytest.mark.parametrize("M,N,K", [(2499, 4090, 256), (2600, 2040, 384), (2590, 4090, 128), (1594, 4090, 128), (2756, 1500, 128),
+                                   (2092, 450, 256), (2092, 450, 128), (2341, 200, 128), (2756, 130, 128), (1677, 130, 256)])
 def test_product_of_one_round_of_tiles(exts, dev, M, N, K, fa, fb, bscale, rows):
-    """Sizes that tiles of 160 and of 192 tokens fit."""
+    """Sizes that the tiles fit, each of them."""
     a, sa, b, sb = _operands(M, N, K, fa, fb, bscale, rows, dev)
+    for out in (torch.bfloat16, torch.float32):
+        _check(exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out), a, sa, b, sb)
+
+
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("fp32", 128), ("e8m0", 1)])
+@pytest.mark.parametrize("M,N", [(2100, 4400), (4200, 4400), (300, 1030), (1300, 1300)])
+def test_product_long_bf16(exts, dev, M, N, bscale, rows):
+    """The same on the bf16 results' tiles, and on several tiles a workgroup."""
+    a, sa, b, sb = _operands(M, N, 8448, E4, E5, bscale, rows, dev)
     _check(exts["proj"].fp8_matmul(a, sa, b, sb), a, sa, b, sb)
 
 
