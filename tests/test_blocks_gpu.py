@@ -263,3 +263,43 @@ def test_product_binding_refusals(exts, dev):
                         ((a, s, a, s, torch.float16), "out_dtype"), ((a, s, a.cpu(), s.cpu()), "one device")):
         with pytest.raises(RuntimeError, match=match):
             f(*args)
+
+
+def test_offsets_past_32_bits(exts, dev):
+    """The last rows of operands of more than 2^31 elements, against calls on those
+    rows alone (a norm's row, a code and a product's row depend on nothing else)."""
+    R, D, N, last = (1 << 20) + 3001, 2048, 1100, 700
+    g = torch.Generator(device=dev).manual_seed(1)
+    y = torch.empty(R, D, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    r = torch.empty_like(y).normal_(generator=g)
+    gm = torch.randn(D, generator=g, device=dev).to(torch.bfloat16)
+    f, b = exts["rmsnorm"].block_norm, exts["rmsnorm"].block_norm_backward
+    kw = dict(gate=r, post_gamma=gm, gamma=gm, act="silu")
+    end = {k: v[-last:] if v is r else v for k, v in kw.items()}
+    whole, part = f(y, residual=r, stats=True, **kw), f(y[-last:], residual=r[-last:], stats=True, **end)
+    for a, c in zip(whole, part):
+        assert (a is None and c is None) or torch.equal(a[-last:], c)
+    ga = b(None, r, y, residual=r, rstd_y=whole[4], rstd_h=whole[5], **kw)
+    gc = b(None, r[-last:], y[-last:], residual=r[-last:], rstd_y=part[4], rstd_h=part[5], **end)
+    for a, c in zip(ga[:3], gc[:3]):
+        assert torch.equal(a[-last:], c)
+    del whole, ga
+    q = f(y, residual=r, quantize=True, store_h=False, **kw)[2:]
+    q2 = f(y[-last:], residual=r[-last:], quantize=True, store_h=False, **end)[2:]
+    assert all(torch.equal(a[-last:].view(torch.uint8), c.view(torch.uint8)) for a, c in zip(q, q2))
+    del r, kw, end, q2
+    codes, scales, codes_t, scales_t = exts["proj"].fp8_quantize(y, rows=True, columns=True)
+    c2, s2 = exts["proj"].fp8_quantize(y[-last:])
+    assert torch.equal(codes[-last:].view(torch.uint8), c2.view(torch.uint8))
+    assert torch.equal(scales[-last:].view(torch.uint8), s2.view(torch.uint8))
+    at = R // 128 * 128 - 512  # whole blocks of 128 rows, along the columns
+    t2, ts2 = exts["proj"].fp8_quantize(y[at:], rows=False, columns=True)
+    assert torch.equal(codes_t[:, at:].view(torch.uint8), t2.view(torch.uint8))
+    assert torch.equal(scales_t[:, at // 128:].view(torch.uint8), ts2.view(torch.uint8))
+    del y, codes_t, scales_t, t2, ts2
+    w = exts["proj"].fp8_quantize(torch.randn(N, D, generator=g, device=dev), block_rows=128)
+    out = exts["proj"].fp8_matmul(codes, scales, *w)
+    ref = (c2.double() * s2.float().double().repeat_interleave(128, 1)) @ (w[0].double() * w[1].float().double().repeat_interleave(
+        128, 0)[:N].repeat_interleave(128, 1)).t()
+    # half a step of bf16, and 2^-10 of the sum of 2048 terms' magnitudes, some 2048 * 0.64 for values of unit size
+    assert out.shape == (R, N) and ((out[-last:].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * 1400).all()
