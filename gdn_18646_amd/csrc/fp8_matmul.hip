@@ -1,21 +1,25 @@
 // Entry point of the fp8 block-scaled product, and its kernel for a few tokens.
 //
 // gdn_fp8_few_kernel (a decode step's tokens): what counts is the weights' bytes.
-// A workgroup owns 16 columns; each of its waves takes every WAVES-th block of K
-// straight from memory into MFMA fragments (no LDS: nothing is used twice), and
-// the waves' sums meet in LDS.  One token, us (GB/s of weights): N 2048, K 2048 3.5
-// (launch bound), 8224 x 2048 5.4, 8192 x 8192 12.0 (5.6 TB/s).
+// A workgroup owns 16 columns and 16 tokens; each of its waves takes every
+// WAVES-th block of K straight from memory into MFMA fragments (no LDS: nothing is
+// used twice), and the waves' sums meet in LDS.  The workgroups of an XCD begin at
+// different blocks: 16 rows at a stride of a power of two lie in one or two of its
+// L2's channels, and in step they would all wait for the same ones (one token,
+// 4096 x 4096: 5.0 us against 6.2).  One token: 2048 x 2048 4.0 us (launch bound),
+// 8224 x 2048 5.5, 8192 x 8192 11.6 (5.8 TB/s of weights).  More loads under way a
+// wave (four blocks' at once, 110 registers) made it slower: 2048 x 8192 7.0 -> 7.7.
 #include "fp8_matmul.hpp"
 
 namespace {
 
 template <int FA, int FB, bool OUT32, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::MatmulParams p, int scales) {
+__global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::MatmulParams p, int scales, int rot_mask) {
     __shared__ f32x4 sums[WAVES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
-    const int n0 = blockIdx.x * 16, nslices = p.K / 128;
-    const int row = min(n0 + r16, p.N - 1), tok = min(r16, p.M - 1);
+    const int n0 = blockIdx.x * 16, t0 = blockIdx.y * 16, nslices = p.K / 128;
+    const int row = min(n0 + r16, p.N - 1), tok = min(t0 + r16, p.M - 1);
     const uint8_t* const w = p.b + static_cast<size_t>(row) * p.ldb + 16 * g4;
     const uint8_t* const x = p.a + static_cast<size_t>(tok) * p.lda + 16 * g4;
     const bool rows = scales == gdn_fp8::kE8Row || scales == gdn_fp8::kF32Row;
@@ -23,8 +27,10 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
     // the scale of the lane's row of b, its accumulator's column
     const size_t sstep = rows ? p.ldb_s : 1, sat = rows ? row : static_cast<size_t>(row / 128) * p.ldb_s;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int rot = static_cast<int>(blockIdx.x >> 3) & rot_mask;
 #pragma unroll 4
-    for (int kb = wave; kb < nslices; kb += WAVES) {
+    for (int i = wave; i < nslices; i += WAVES) {
+        const int kb = i + rot < nslices ? i + rot : i + rot - nslices;
         const u32x4* const wp = reinterpret_cast<const u32x4*>(w + static_cast<size_t>(kb) * 128);
         const u32x4* const xp = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(kb) * 128);
         const int sx = p.a_scale[kb * p.lda_s + tok];
@@ -55,7 +61,7 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float v[1] = {acc[i]};
-        if (4 * g4 + i < p.M) store_cols<OUT32>(p, 4 * g4 + i, n0 + r16, v);
+        if (t0 + 4 * g4 + i < p.M) store_cols<OUT32>(p, t0 + 4 * g4 + i, n0 + r16, v);
     }
 }
 
@@ -119,20 +125,26 @@ Choice choose_tile(long long M, long long N, int K, bool f32) {
 
 template <int FA, int FB>
 int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t stream) {
-    // Few tokens.  Above four the tokens' own codes, which every workgroup reads,
-    // begin to count, and more so the more workgroups: 16 tokens of K = 2048 take
-    // 4.0 us (tiles 4.8) at N = 2048, 7.4 (5.6) at 8224.  Many columns give every
-    // CU enough waves with four a workgroup (8224: 5.4 us against 5.8 with eight),
-    // few do not (2048, K = 4096: 5.0 against 4.4).
-    if (p.M <= 4 || (p.M <= 16 && p.N <= 4096)) {
+    // Few workgroups of 16 x 16 results (up to one a CU), where a tile's chain of
+    // copies would be longer than the sum itself: us here and on tiles, 32 x 2048 x
+    // 8192 9.6 and 13.4, 64 x 1024 x 4096 5.9 and 6.4, 48 x 2048 x 4096 (384 of
+    // them) 9.6 and 6.5.  Few tokens on more columns too: 4 x 8224 x 2048 6.2 and
+    // 6.6, 8 x 6176 x 2048 5.5 and 6.3, 16 x 8224 x 2048 7.7 and 6.7.  Up to one
+    // workgroup a CU eight waves share a sum (2048 x 4096: 4.8 us, 5.9 with four),
+    // above that four (8224 x 2048: 5.6, 5.8 with eight).
+    const long long few_groups = (p.M + 15LL) / 16 * ((p.N + 15LL) / 16);
+    if (p.M <= 4 || few_groups <= (p.M <= 8 ? 400 : 256)) {
+        int mask = 1;
+        while (2 * mask <= p.K / 128) mask *= 2;
         const auto few = [&](auto out32, auto waves) {
             constexpr int W = decltype(waves)::value;
             if (!gdn_host::grid_fits((p.N + 15) / 16, 64 * W)) return gdn_host::fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: N=%d is too large for a launch", p.N);
-            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, scales);
+            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16, (p.M + 15) / 16), dim3(64 * W), 0, stream, p,
+                               scales, mask - 1);
             return gdn_host::check_launch("gdn_fp8_few_kernel");
         };
         const auto of_n = [&](auto out32) {
-            return p.N <= 4096 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
+            return few_groups <= 256 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
         };
         return f32 ? of_n(std::true_type{}) : of_n(std::false_type{});
     }
