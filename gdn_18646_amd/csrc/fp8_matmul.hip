@@ -1,14 +1,15 @@
-// Entry point of the fp8 block-scaled product, and its kernel for a few tokens.
+// Entry point of the fp8 block-scaled product, the rule that picks its kernel, and
+// the kernel for one token or two.
 //
-// gdn_fp8_few_kernel (a decode step's tokens): what counts is the weights' bytes.
-// A workgroup owns 16 columns and 16 tokens; each of its waves takes every
-// WAVES-th block of K straight from memory into MFMA fragments (no LDS: nothing is
-// used twice), and the waves' sums meet in LDS.  The workgroups of an XCD begin at
-// different blocks: 16 rows at a stride of a power of two lie in one or two of its
-// L2's channels, and in step they would all wait for the same ones (one token,
-// 4096 x 4096: 5.0 us against 6.2).  One token: 2048 x 2048 4.0 us (launch bound),
-// 8224 x 2048 5.5, 8192 x 8192 11.6 (5.8 TB/s of weights).  More loads under way a
-// wave (four blocks' at once, 110 registers) made it slower: 2048 x 8192 7.0 -> 7.7.
+// gdn_fp8_few_kernel (a decode step's token): what counts is the weights' bytes. A
+// workgroup owns 16 columns; each of its waves takes every WAVES-th block of K
+// straight from memory into MFMA fragments (no LDS: nothing is used twice), and
+// the waves' sums meet in LDS.  The workgroups of an XCD begin at different
+// blocks: 16 rows at a stride of a power of two lie in one or two of its L2's
+// channels, and in step they would all wait for the same ones (one token, 4096 x
+// 4096: 5.0 us against 6.2).  One token: 2048 x 2048 4.0 us (launch bound), 8224 x
+// 2048 5.5, 8192 x 8192 11.6 (5.8 TB/s of weights).  More loads under way a wave
+// (four blocks' at once, 110 registers) made it slower: 2048 x 8192 7.0 -> 7.7.
 #include "fp8_matmul.hpp"
 
 namespace {
@@ -18,8 +19,8 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
     __shared__ f32x4 sums[WAVES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
-    const int n0 = blockIdx.x * 16, t0 = blockIdx.y * 16, nslices = p.K / 128;
-    const int row = min(n0 + r16, p.N - 1), tok = min(t0 + r16, p.M - 1);
+    const int n0 = blockIdx.x * 16, nslices = p.K / 128;
+    const int row = min(n0 + r16, p.N - 1), tok = min(r16, p.M - 1);
     const uint8_t* const w = p.b + static_cast<size_t>(row) * p.ldb + 16 * g4;
     const uint8_t* const x = p.a + static_cast<size_t>(tok) * p.lda + 16 * g4;
     const bool rows = scales == gdn_fp8::kE8Row || scales == gdn_fp8::kF32Row;
@@ -61,40 +62,50 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float v[1] = {acc[i]};
-        if (t0 + 4 * g4 + i < p.M) store_cols<OUT32>(p, t0 + 4 * g4 + i, n0 + r16, v);
+        if (4 * g4 + i < p.M) store_cols<OUT32>(p, 4 * g4 + i, n0 + r16, v);
     }
 }
 
-// What a call on a tile takes, us: c + rounds (a + b blocks of K), rounds of 256
-// workgroups, or, where two share a CU, of 512, and of up to 256 alone.  Fitted
-// to 184 products, 17 to 16384 tokens, N 512 to 8192, K 800 to 4096 (kernels
-// back to back): the tile that the fit picks takes at most 1.02 times the best
-// one's time (fp32 results: 114 products, 1.16, 1.01 on average); 26 tiles were
-// timed, those here are the ones whose absence costs: 256 x 160 and 128 x 192 up
-// to 9%, where they make one round of what others make two of or a half (1500 x
-// 6176 x 2048: 22.7 us on 256 x 160, 24.3 on 256 x 192).
+// What a call on a tile takes, us: c + rounds (a + b blocks of K), a round being
+// 256 workgroups, or, where a CU holds per_cu of them, up to per_cu times 256,
+// with a and b between a1, b1 (one a CU) and a2, b2 (per_cu).  Fitted to 336
+// products (fp32 results: 336), 1 to 8192 tokens, N 200 to 8224, K 512 to 8192,
+// kernels back to back on operands that the L2s do not hold: the tile that the fit
+// picks takes at most 1.12 times the best one's time (fp32 1.05) and 1.003 times on
+// average; 39 tiles were timed, those here are the ones whose absence costs.
+// Small products are bound by how fast a CU takes in its rows, some 45 GB/s, so
+// the small tiles spread them over the CUs, split K over groups of waves and keep
+// several stages under way: 16 x 2048 x 8192 takes 6.8 us on 16 x 16 with eight
+// groups and four stages (a workgroup a CU), 8.6 with two stages, 10.5 on 32 x 32;
+// 16 x 8224 x 2048 6.2 on 16 x 16 with three a CU, 6.8 on 64 x 32.  256 x 160 and 128
+// x 192 are up to 9% faster where they make one round of what others make two of
+// or a half (1500 x 6176 x 2048: 22.7 us on 256 x 160, 24.3 on 256 x 192).
 struct TileCost {
     int tile, cols, toks, per_cu;
-    float c, a1, b1, a2, b2;  // per_cu 2: alone (1) and two (2)
+    float c, a1, b1, a2, b2;  // per_cu above 1: alone (1) and with per_cu on each CU (2)
 };
 constexpr TileCost kBf16[] = {
-    {gdn_fp8::k256x256, 256, 256, 1, 0.f, 6.93f, 1.177f, 0.f, 0.f},
-    {gdn_fp8::k256x192, 256, 192, 1, 0.f, 6.20f, 1.042f, 0.f, 0.f},
-    {gdn_fp8::k256x160, 256, 160, 1, 0.f, 5.69f, 0.921f, 0.f, 0.f},
-    {gdn_fp8::k256x128, 256, 128, 1, 0.f, 5.34f, 0.753f, 0.f, 0.f},
-    {gdn_fp8::k128x192, 128, 192, 1, 0.48f, 4.14f, 0.702f, 0.f, 0.f},
-    {gdn_fp8::k128x128, 128, 128, 1, 0.60f, 3.45f, 0.518f, 0.f, 0.f},
-    {gdn_fp8::k64x128, 64, 128, 1, 0.85f, 3.44f, 0.328f, 0.f, 0.f},
-    {gdn_fp8::k64x64, 64, 64, 1, 0.94f, 2.77f, 0.231f, 0.f, 0.f},
-    {gdn_fp8::k64x32, 64, 32, 1, 1.13f, 2.53f, 0.148f, 0.f, 0.f},
-    {gdn_fp8::k32x32, 32, 32, 2, 1.84f, 1.18f, 0.120f, 1.75f, 0.197f},
+    {gdn_fp8::k256x256, 256, 256, 1, 0.f, 6.75f, 1.135f, 0.f, 0.f},
+    {gdn_fp8::k256x192, 256, 192, 1, 0.f, 6.22f, 1.012f, 0.f, 0.f},
+    {gdn_fp8::k256x160, 256, 160, 1, 0.f, 5.75f, 0.904f, 0.f, 0.f},
+    {gdn_fp8::k256x128, 256, 128, 1, 0.f, 5.56f, 0.725f, 0.f, 0.f},
+    {gdn_fp8::k128x192, 128, 192, 1, 0.f, 4.78f, 0.688f, 0.f, 0.f},
+    {gdn_fp8::k128x128, 128, 128, 1, 0.f, 4.28f, 0.511f, 0.f, 0.f},
+    {gdn_fp8::k64x128, 64, 128, 1, 0.40f, 4.22f, 0.315f, 0.f, 0.f},
+    {gdn_fp8::k64x64, 64, 64, 1, 0.92f, 3.20f, 0.222f, 0.f, 0.f},
+    {gdn_fp8::k64x32, 64, 32, 1, 1.26f, 2.73f, 0.144f, 0.f, 0.f},
+    {gdn_fp8::k32x32, 32, 32, 1, 1.48f, 2.16f, 0.106f, 0.f, 0.f},
+    {gdn_fp8::k16x16Alone, 16, 16, 1, 1.64f, 1.78f, 0.054f, 0.f, 0.f},
+    {gdn_fp8::k16x16, 16, 16, 3, 2.60f, 0.70f, 0.064f, 1.37f, 0.112f},
 };
 constexpr TileCost kF32[] = {
-    {gdn_fp8::k128x128, 128, 128, 2, 0.85f, 2.61f, 0.957f, 4.54f, 1.676f},
-    {gdn_fp8::k64x128, 64, 128, 1, 0.77f, 3.24f, 0.538f, 0.f, 0.f},
-    {gdn_fp8::k64x64, 64, 64, 1, 1.09f, 2.65f, 0.361f, 0.f, 0.f},
-    {gdn_fp8::k64x32, 64, 32, 1, 1.26f, 2.56f, 0.213f, 0.f, 0.f},
-    {gdn_fp8::k32x32, 32, 32, 2, 2.16f, 1.02f, 0.156f, 1.97f, 0.228f},
+    {gdn_fp8::k128x128, 128, 128, 2, 1.01f, 3.08f, 0.915f, 8.07f, 1.556f},
+    {gdn_fp8::k64x128, 64, 128, 1, 0.11f, 4.40f, 0.525f, 0.f, 0.f},
+    {gdn_fp8::k64x64, 64, 64, 1, 0.76f, 3.32f, 0.346f, 0.f, 0.f},
+    {gdn_fp8::k64x32, 64, 32, 1, 1.09f, 3.09f, 0.200f, 0.f, 0.f},
+    {gdn_fp8::k32x32, 32, 32, 1, 1.34f, 2.25f, 0.150f, 0.f, 0.f},
+    {gdn_fp8::k16x16Alone, 16, 16, 1, 1.63f, 1.84f, 0.064f, 0.f, 0.f},
+    {gdn_fp8::k16x16, 16, 16, 3, 2.61f, 0.70f, 0.081f, 1.53f, 0.123f},
 };
 
 struct Choice {
@@ -110,13 +121,14 @@ Choice choose_tile(long long M, long long N, int K, bool f32) {
     for (int i = 0; i < n; ++i) {
         const TileCost& t = table[i];
         const long long tiles = (M + t.toks - 1) / t.toks * ((N + t.cols - 1) / t.cols);
+        const float alone = t.a1 + t.b1 * nk, full = t.a2 + t.b2 * nk;
         float us = t.c;
         if (t.per_cu == 1) {
-            us += static_cast<float>((tiles + kCUs - 1) / kCUs) * (t.a1 + t.b1 * nk);
+            us += static_cast<float>((tiles + kCUs - 1) / kCUs) * alone;
         } else {
-            const long long rest = tiles % (2 * kCUs);
-            us += static_cast<float>(tiles / (2 * kCUs) + (rest > kCUs ? 1 : 0)) * (t.a2 + t.b2 * nk);
-            if (rest > 0 && rest <= kCUs) us += t.a1 + t.b1 * nk;
+            const long long round = kCUs * t.per_cu, each = (tiles % round + kCUs - 1) / kCUs;  // workgroups a CU in the last one
+            us += static_cast<float>(tiles / round) * full;
+            if (each > 0) us += alone + static_cast<float>(each - 1) / static_cast<float>(t.per_cu - 1) * (full - alone);
         }
         if (i == 0 || us < best.us) best = {t.tile, us};
     }
@@ -125,26 +137,23 @@ Choice choose_tile(long long M, long long N, int K, bool f32) {
 
 template <int FA, int FB>
 int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t stream) {
-    // Few workgroups of 16 x 16 results (up to one a CU), where a tile's chain of
-    // copies would be longer than the sum itself: us here and on tiles, 32 x 2048 x
-    // 8192 9.6 and 13.4, 64 x 1024 x 4096 5.9 and 6.4, 48 x 2048 x 4096 (384 of
-    // them) 9.6 and 6.5.  Few tokens on more columns too: 4 x 8224 x 2048 6.2 and
-    // 6.6, 8 x 6176 x 2048 5.5 and 6.3, 16 x 8224 x 2048 7.7 and 6.7.  Up to one
-    // workgroup a CU eight waves share a sum (2048 x 4096: 4.8 us, 5.9 with four),
+    // One token, us here and on tiles: 4096 x 4096 5.0 and 5.8, 4096 x 8192 7.1 and
+    // 8.0, 8224 x 2048 5.6 and 6.0, but 2048 x 8192 7.0 and 6.4, 6176 x 4096 7.0 and
+    // 6.6; three tokens: 8224 x 2048 6.0 and 6.1, 6176 x 4096 7.5 and 6.8.  Eight
+    // waves share a sum up to a workgroup a CU (2048 x 4096: 4.8 us, 5.9 with four),
     // above that four (8224 x 2048: 5.6, 5.8 with eight).
-    const long long few_groups = (p.M + 15LL) / 16 * ((p.N + 15LL) / 16);
-    if (p.M <= 4 || few_groups <= (p.M <= 8 ? 400 : 256)) {
+    if (p.M <= 2) {
         int mask = 1;
         while (2 * mask <= p.K / 128) mask *= 2;
         const auto few = [&](auto out32, auto waves) {
             constexpr int W = decltype(waves)::value;
             if (!gdn_host::grid_fits((p.N + 15) / 16, 64 * W)) return gdn_host::fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: N=%d is too large for a launch", p.N);
-            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16, (p.M + 15) / 16), dim3(64 * W), 0, stream, p,
+            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p,
                                scales, mask - 1);
             return gdn_host::check_launch("gdn_fp8_few_kernel");
         };
         const auto of_n = [&](auto out32) {
-            return few_groups <= 256 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
+            return p.N <= 4096 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
         };
         return f32 ? of_n(std::true_type{}) : of_n(std::false_type{});
     }

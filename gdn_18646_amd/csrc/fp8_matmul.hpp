@@ -22,7 +22,7 @@ enum Scales { kE8Block = 0, kE8Row = 1, kF32Block = 2, kF32Row = 3 };
 
 // Tiles of the tiled kernel (columns x tokens), largest first; those before
 // k128x128 for bf16 results alone.
-enum Tile { k256x256 = 0, k256x192, k256x160, k256x128, k128x192, k128x128, k64x128, k64x64, k64x32, k32x32, kTiles };
+enum Tile { k256x256 = 0, k256x192, k256x160, k256x128, k128x192, k128x128, k64x128, k64x64, k64x32, k32x32, k16x16Alone, k16x16 };
 
 // Defined in fp8_mm_*.hip for each pair of formats (of a, of b).  f32: out is
 // fp32 (and the products are summed in full, see fp8_tiles.hpp), else bf16.

@@ -568,7 +568,9 @@ using Tile128x128Pair = Fp8Tile<2, 4, 4, 2, 2, 2>;  // fp32 results: two workgro
 using Tile64x128 = Fp8Tile<1, 4, 4, 2, 3, 1, 2>;
 using Tile64x64 = Fp8Tile<2, 2, 2, 2, 3, 1, 2>;
 using Tile64x32 = Fp8Tile<1, 2, 4, 1, 3, 1, 4>;
-using Tile32x32 = Fp8Tile<1, 2, 2, 1, 2, 2, 4>;
+using Tile32x32 = Fp8Tile<1, 2, 2, 1, 3, 1, 4>;
+using Tile16x16Alone = Fp8Tile<1, 1, 1, 1, 4, 1, 8>;
+using Tile16x16 = Fp8Tile<1, 1, 1, 1, 3, 3, 4>;
 
 template <class TL, int FA, int FB, int SB, bool OUT32>
 int launch_scaled(const MatmulParams& p, hipStream_t stream) {
@@ -600,6 +602,8 @@ int launch_tile(int tile, int scales, bool f32, const MatmulParams& p, hipStream
             case k64x64: return launch_tiled<Tile64x64, FA, FB, O>(scales, p, stream);
             case k64x32: return launch_tiled<Tile64x32, FA, FB, O>(scales, p, stream);
             case k32x32: return launch_tiled<Tile32x32, FA, FB, O>(scales, p, stream);
+            case k16x16Alone: return launch_tiled<Tile16x16Alone, FA, FB, O>(scales, p, stream);
+            case k16x16: return launch_tiled<Tile16x16, FA, FB, O>(scales, p, stream);
             default: return launch_tiled<std::conditional_t<O, Tile128x128Pair, Tile128x128>, FA, FB, O>(scales, p, stream);
         }
     };

@@ -30,7 +30,7 @@ def _kernels(asm, tile="", scales=r"\d"):
 
 def test_no_tile_spills(asm):
     names = _kernels(asm)
-    assert len(names) == 4 * (10 + 5), names  # layouts of b's scales x tiles of bf16 and of fp32 results
+    assert len(names) == 4 * (12 + 7), names  # layouts of b's scales x tiles of bf16 and of fp32 results
     for name in names:
         assert not any("scratch_" in ln for ln in _function(asm, name)), name
 
