@@ -20,8 +20,9 @@
 // stages on over tile borders (8192 x 8192 x 8192: 420 us), non-temporal stores
 // (213 against 185 us at 16384 x 6144 x 2048) and staggered starts were slower or
 // no faster.  Products of one round of tiles are bound by how many of the 256 CUs
-// have one (1500 x 8224 x 2048: 198 tiles, 28 us, 1.8 PFLOP/s), small ones by a
-// tile's chain of copies, which groups of waves on different blocks shorten.
+// have one (1500 x 8224 x 2048: 198 tiles, 28 us, 1.8 PFLOP/s), small ones by
+// how fast a CU takes in its rows, which more, smaller tiles with K over groups of
+// waves spread over the CUs (fp8_matmul.hip has the figures).
 #pragma once
 
 #include "fp8_matmul.hpp"
