@@ -17,6 +17,11 @@
 // a workgroup a CU walks them, the next row's loads under way while a row is
 // worked on (4096 x 8192: 78 us against 102 with a workgroup a row; walking rows
 // of 2048 columns instead took 70 against 64).
+#include <stdlib.h>
+
+#include <algorithm>
+#include <numeric>
+
 #include "block_norm.hpp"
 #include "fp8_blocks.hpp"
 
@@ -160,6 +165,28 @@ __global__ __launch_bounds__(LPR <= 64 ? 256 : LPR) void gdn_block_norm_kernel(N
     }
 }
 
+// Rows as they lie in memory: how many, the bytes of one and from one to the next.
+struct Span {
+    const void* at;
+    long long rows, bytes, step;
+    long long first() const { return static_cast<long long>(reinterpret_cast<uintptr_t>(at)); }
+    long long low() const { return first() + std::min(0LL, (rows - 1) * step); }
+    long long high() const { return first() + std::max(0LL, (rows - 1) * step) + bytes; }
+};
+
+// Whether rows of h may be written while those of an input are read.  A row of an
+// input that is a row of h itself has each value read by the lane that writes it,
+// before it does; anything else has to lie apart from h for certain: in another
+// range of memory, or in other columns of a common step.
+bool may_share(const Span& h, const Span& in) {
+    if (!h.at || !in.at || h.high() <= in.low() || in.high() <= h.low()) return true;
+    if (h.at == in.at && h.rows == in.rows && h.bytes == in.bytes && (h.rows == 1 || h.step == in.step)) return true;
+    const long long step = std::gcd(h.rows > 1 ? llabs(h.step) : 0, in.rows > 1 ? llabs(in.step) : 0);
+    if (step == 0) return false;
+    const long long at = ((in.first() - h.first()) % step + step) % step;
+    return at >= h.bytes && at + in.bytes <= step;
+}
+
 }  // namespace
 
 extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residual, int64_t ldr, const void* gate,
@@ -199,11 +226,26 @@ extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residu
     p.codes = codes, p.scales = scales, p.ldc = ldc, p.lds = lds;
     p.rstd_y = rstd_y, p.rstd_h = rstd_h;
     p.R = static_cast<int>(R), p.D = static_cast<int>(D), p.inv_D = 1.f / static_cast<float>(D);
+    const auto span = [&](const void* at, long long rows, long long ld, size_t size) {
+        return Span{at, rows, D * static_cast<long long>(size), ld * static_cast<long long>(size)};
+    };
+    const Span written = span(h, R, ldh, br);
+    const char* shared = nullptr;  // the input that h would be written over
+    const auto check = [&](const char* name, const Span& in) {
+        if (!may_share(written, in)) shared = name;
+    };
+    check("y", span(y, R, ldy, by));
+    check("residual", span(residual, R, ldr, br));
+    if (gate) check("gate", span(gate, R / rows_per_gate + (R % rows_per_gate != 0), ldg, by));
+    check("post_gamma", span(post_gamma, 1, 0, bp));
+    check("gamma", span(gamma, 1, 0, bp));
+    check("scale", span(scale, 1, 0, bp));
     return with_types(type_y, type_r, type_p, [&](auto ty, auto tr, auto tp) {
         return with_row_shape<false>(p.D, vec, [&](auto lpr, auto nv, auto v) {
             constexpr int LPR = decltype(lpr)::value, threads = LPR <= 64 ? 256 : LPR;
             const int all = static_cast<int>((R + slots_of(LPR) - 1) / slots_of(LPR));
             if (!gdn_host::grid_fits(all, threads)) return fail(GDN_ERR_UNSUPPORTED, "block_norm: R=%lld rows of %lld are too many for a launch", (long long)R, (long long)D);
+            if (shared) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: h would be written to memory locations of %s other than its own row's", shared);
             const dim3 grid(LPR == 1024 && all > 256 ? 256 : all), block(threads);
             hipLaunchKernelGGL((gdn_block_norm_kernel<decltype(ty), decltype(tr), decltype(tp), LPR, decltype(nv)::value, decltype(v)::value>),
                                grid, block, 0, static_cast<hipStream_t>(stream), p);

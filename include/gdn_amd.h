@@ -375,8 +375,10 @@ enum { GDN_ACT_NONE = 0, GDN_ACT_SIGMOID = 1, GDN_ACT_SILU = 2, GDN_ACT_TANH = 3
  *   one for all), n [R, D]: type_y; residual, h [R, D]: type_r;
  *   post_gamma, gamma, scale [D]: type_p.  Inputs but y may be NULL, outputs
  *   too.  Types (y, r, p): bf16 bf16 bf16, bf16 bf16 fp32, bf16 fp32 fp32,
- *   fp32 fp32 fp32.  ld*: elements from a row to the next.  h may be residual
- *   itself (same stride).
+ *   fp32 fp32 fp32.  ld*: elements from a row to the next.  h may be written
+ *   over the rows of residual, y or a gate a token (same address, type and
+ *   stride); a call whose h is not apart from an input otherwise, by its range
+ *   of memory or by columns within a common stride, is refused.
  *   codes [R, ldc >= D padded to 128] and scales [ceil(D / 128), lds >= R]: n
  *   (h without gamma), unrounded, as e4m3 codes in blocks of 128 columns (see
  *   gdn_fp8_quantize_hip); codes 16-byte aligned, ldc % 16 == 0.

@@ -196,6 +196,33 @@ def test_inplace_overlap(exts, dev):
         f(buf[:0], act="gelu")
 
 
+def test_inplace_strided(exts, dev):
+    """Rows of a wider buffer: columns beside the residual's are taken, views that
+    share columns with it are refused."""
+    f = exts["rmsnorm"].block_norm
+    g = torch.Generator().manual_seed(3)
+    for D, at in ((256, 0), (600, 8), (1001, 5)):
+        wide = torch.randn(9, 3 * D + 24, generator=g).to(torch.bfloat16).to(dev)
+        gm, gate = (torch.randn(9, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+        y, r = wide[:, at:at + D], wide[:, at + D:at + 2 * D]
+        kw = dict(gamma=wide[4, at + 2 * D:at + 3 * D], gate=gate, act="silu")
+        h, n, _, _ = f(y, residual=r, **kw)
+        keep = wide.clone()
+        h2, n2, _, _ = f(y, residual=r, inplace=True, **kw)
+        assert h2.data_ptr() == r.data_ptr() and torch.equal(r, h) and torch.equal(n2, n)
+        keep[:, at + D:at + 2 * D] = h
+        assert torch.equal(wide, keep)  # the other columns are as they were
+        h3 = f(wide[1:, at:at + D], residual=r[:8])[0]  # other rows' columns beside it are apart as well
+        assert torch.equal(f(wide[1:, at:at + D], residual=r[:8], inplace=True)[0], h3)
+        for t in (wide[:8, at + D - 8:at + 2 * D - 8], wide[1:, at + D:at + 2 * D]):
+            with pytest.raises(RuntimeError, match="memory locations of y"):
+                f(t, residual=r[:8], inplace=True)
+        with pytest.raises(RuntimeError, match="memory locations of gamma"):
+            f(y, residual=r, gamma=r[3], inplace=True)
+        with pytest.raises(RuntimeError, match="memory locations of gate"):
+            f(gate[:8], residual=r[:8], gate=r[1:], inplace=True)
+
+
 def test_strided_rows(exts, dev):
     """Operands that are column slices of a wider buffer, 16-byte aligned or not."""
     for off, D in ((64, 256), (3, 256), (64, 250)):

@@ -33,6 +33,26 @@ def test_block_norm_refusals(bad, match):
         _norm(**bad)
 
 
+@pytest.mark.parametrize("over,name", [
+    (dict(y=FAKE + 1024), "y"),                          # rows of one buffer, a row on (rows 1024 bytes apart)
+    (dict(y=FAKE - 1024), "y"),
+    (dict(y=FAKE + 256), "y"),                           # columns of the same rows, half a row on
+    (dict(y=FAKE + 768), "y"),                           # past the row's end into the next one
+    (dict(y=FAKE + 512, ldy=320), "y"),                  # steps that have 128 bytes in common
+    (dict(y=FAKE, ldy=256), "y"),                        # the same place, another step
+    (dict(residual=FAKE + 1024), "residual"),
+    (dict(gate=FAKE + 2048), "gate"),
+    (dict(gate=FAKE, rpg=2), "gate"),                    # rows 0 and 1 are read by others
+    (dict(gate=FAKE, rpg=4), "gate"),
+    (dict(post=FAKE), "post_gamma"), (dict(gamma=FAKE + 3072), "gamma"), (dict(scale=FAKE + 1500), "scale")])
+def test_block_norm_refuses_h_over_what_others_read(over, name):
+    """h in every second 512 bytes of a buffer, at FAKE; the other operands elsewhere."""
+    far = dict(y=1 << 20, residual=FAKE, ldr=512, ldy=512, ldg=512, gate=2 << 20, post=3 << 20, gamma=3 << 20, scale=3 << 20, h=FAKE, ldh=512,
+               n=4 << 20)
+    with pytest.raises(GdnError, match=f"INVALID_ARGUMENT.*memory locations of {name} "):
+        _norm(**{**far, **over})
+
+
 def test_no_rows_is_no_call():
     _norm(R=0, residual=None)
     _norm(R=0, y=None)
