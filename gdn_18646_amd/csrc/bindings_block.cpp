@@ -137,6 +137,8 @@ Tensor down_columns(int64_t M, int64_t KB, at::ScalarType type, const Tensor& t)
 std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gate, const Opt& post_gamma, const Opt& gamma,
                             const Opt& scale, double residual_scale, const std::string& act, double eps, bool quantize,
                             bool store_h, bool stats, bool inplace) {
+    TORCH_CHECK(!inplace || !given(residual) || !at::GradMode::is_enabled() || !residual->requires_grad(),
+                "block_norm: inplace would write over a residual that requires grad (no gradients are recorded here)");
     const Operands o = operands(y, residual, gate, post_gamma, gamma, scale);
     const int a = act_of(act);
     TORCH_CHECK(store_h || quantize || given(gamma), "block_norm: store_h=False leaves nothing to write");
@@ -173,6 +175,7 @@ std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gat
                                     static_cast<float>(eps), h.ptr, h.ld, n.ptr, n.ld, codes, ldc, scales, lds, ry, rh, o.R, o.D,
                                     o.ty, o.tr, o.tp, stream_of(y)),
                  "block_norm");
+    if (inplace && !residual->is_inference()) residual->unsafeGetTensorImpl()->bump_version();  // a graph that saved it raises
     return out;
 }
 
@@ -350,7 +353,8 @@ void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11
                 "post_gamma, gamma, scale [D]; what is None is left out.  Returns [h, n, codes, scales] "
                 "(+ [rstd_y, rstd_h] with stats, for block_norm_backward), None where not made: quantize gives n (h without "
                 "gamma) as e4m3 codes [R, D padded to 128] with e8m0 scales [R, blocks] instead of n; store_h=False leaves h "
-                "out, inplace writes it over residual.",
+                "out, inplace writes it over residual (as an in-place operation: a graph that saved the residual can no longer "
+                "run backward; one that requires grad is refused while gradients are recorded).",
                 py::arg("y"), py::arg("residual") = none, py::arg("gate") = none, py::arg("post_gamma") = none,
                 py::arg("gamma") = none, py::arg("scale") = none, py::arg("residual_scale") = 1.0, py::arg("act") = "none",
                 py::arg("eps") = 1e-6, py::arg("quantize") = false, py::arg("store_h") = true, py::arg("stats") = false,

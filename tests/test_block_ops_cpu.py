@@ -152,3 +152,14 @@ def test_binding_refusals_on_the_host():
         e["proj"].fp8_quantize(y)
     with pytest.raises(RuntimeError, match="GPU tensors"):
         e["proj"].fp8_matmul(y, y, y, y)
+
+
+def test_inplace_over_a_residual_that_requires_grad_is_refused():
+    f = compile_kernels()["rmsnorm"].block_norm
+    y = torch.zeros(4, 256, dtype=torch.bfloat16)
+    leaf = torch.zeros(4, 256, dtype=torch.bfloat16, requires_grad=True)
+    for r in (leaf, leaf * 2, leaf[:]):
+        with pytest.raises(RuntimeError, match="requires grad"):
+            f(y, residual=r, inplace=True)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU tensor"):  # past that check
+            f(y, residual=r, inplace=True)

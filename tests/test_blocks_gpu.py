@@ -112,6 +112,26 @@ def test_block_norm_gradients_through_autograd(dev):
     assert torch.isfinite(only).all()
 
 
+def test_backward_over_an_overwritten_residual_raises(exts, dev):
+    """An in-place call counts as one for autograd: a graph that saved the residual
+    does not compute gradients from what was written over it."""
+    D = 256
+    y, gm = _rand((6, D), torch.bfloat16, dev, 1), _rand((D,), torch.bfloat16, dev, 2)
+    r = _rand((6, D), torch.bfloat16, dev, 3, grad=False)
+    for view in (False, True):  # a view written over is a write to its base
+        _, n = block_norm(y, residual=r, gamma=gm)
+        torch.autograd.grad(n.sum(), y, retain_graph=True)
+        before = r._version
+        exts["rmsnorm"].block_norm(y.detach()[:3] if view else y.detach(), residual=r[:3] if view else r, gamma=gm, inplace=True)
+        assert r._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(n.sum(), y)
+    with torch.inference_mode():
+        s = _rand((6, D), torch.bfloat16, dev, 3, grad=False).clone()
+        h, _, _, _ = exts["rmsnorm"].block_norm(y.detach(), residual=s, gamma=gm, inplace=True)
+        assert h.data_ptr() == s.data_ptr()
+
+
 def _run(x, h0, w1, w2, pg, gm):
     """A block's tail and the next block's head: project, join the residual
     stream, norm, project."""
