@@ -19,6 +19,7 @@ on) take the same operands without recording gradients.
 """
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import compile_kernels, native_extension
@@ -73,10 +74,13 @@ def block_norm(y, residual=None, gate=None, post_gamma=None, gamma=None, scale=N
 
     residual: y's shape.  gate: y's shape, [B, D] (a gate a sequence of
     y [B, ..., D]) or [D]; act: none, sigmoid, silu or tanh.  post_gamma, gamma,
-    scale: [D].  What is None is left out.  Differentiable in every tensor.
+    scale: [D].  What is None is left out.  Differentiable in every tensor, in
+    reverse mode; an operand with a forward-mode tangent raises.
     """
     tensors = (y, residual, gate, post_gamma, gamma, scale)
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
+    there = [t for t in tensors if t is not None]
+    recorded = torch.is_grad_enabled() and any(t.requires_grad for t in there)
+    if not recorded and all(forward_ad.unpack_dual(t).tangent is None for t in there):
         h, n, _, _ = compile_kernels()["rmsnorm"].block_norm(
             y, residual=residual, gate=gate, post_gamma=post_gamma, gamma=gamma, scale=scale,
             residual_scale=residual_scale, act=act, eps=eps)
