@@ -29,17 +29,17 @@ __all__ = ["block_norm", "fp8_linear", "Fp8Weight"]
 BLOCK = 128
 
 
-def _check_capture(ctx):
-    """Refuses a backward pass that is being captured into a graph while a graph of
-    eager work on the same leaves lives: their gradient accumulators belong to the
-    eager work's stream, which autograd would wait for inside the capture, and that
-    ends the process."""
+def _check_capture():
+    """Refuses a backward pass that is being captured into a graph and has yet to
+    reach nodes of eager work, such as the gradient accumulators of leaves that an
+    eager graph keeps alive: they belong to the eager work's stream, which autograd
+    would draw into the capture, and that ends the process."""
     if not torch.cuda.is_current_stream_capturing():
         return
-    leaves = [f.variable for f, _ in ctx.next_functions if f is not None and hasattr(f, "variable")]
-    if native_extension()._leaves_of_another_stream(leaves):
+    outside = sorted({name for name, out in native_extension()._backward_nodes() if out})
+    if outside:
         raise RuntimeError("a backward pass is captured while an eager autograd graph of the same leaves is alive: "
-                           "drop (or detach) the eager results before the capture")
+                           f"drop (or detach) the eager results before the capture ({', '.join(outside)})")
 
 
 class _BlockNorm(torch.autograd.Function):
@@ -56,7 +56,7 @@ class _BlockNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dn):
-        _check_capture(ctx)
+        _check_capture()
         y, residual, gate, post_gamma, gamma, scale, rstd_y, rstd_h = ctx.saved_tensors
         if dh is None and dn is None:
             return (None,) * 9
@@ -126,7 +126,7 @@ class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _check_capture(ctx)
+        _check_capture()
         proj = compile_kernels()["proj"]
         xt, xts, wt, wts = ctx.saved_tensors
         N, K = ctx.sizes

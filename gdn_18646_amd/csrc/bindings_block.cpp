@@ -5,6 +5,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include "../../include/gdn_amd.h"
@@ -329,23 +330,43 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     return out;
 }
 
-// Whether a gradient accumulator of one of these leaves lives that belongs to
-// another stream than the current one of the leaf's device.
-bool leaves_of_another_stream(const std::vector<Tensor>& leaves) {
-    for (const auto& t : leaves) {
-        if (!t.is_cuda()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-        const auto stream = node ? node->stream() : std::nullopt;
-        if (stream.has_value() && stream->id() != c10::hip::getCurrentHIPStream(t.get_device()).id()) return true;
+// Whether a node's stream is one that a capture on the current stream must not
+// wait for or write to: another than the current one, and not part of a capture.
+bool outside_capture(const c10::Stream& s) {
+    if (s.id() == c10::hip::getCurrentHIPStream(s.device_index()).id()) return false;
+    if (s.id() == 0) return true;  // the default stream cannot be captured (nor asked while another is)
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const c10::hip::HIPStream stream(c10::hip::HIPStream::UNCHECKED, s);
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return true;
     }
-    return false;
+    return status != hipStreamCaptureStatusActive;
+}
+
+// The nodes that the running backward pass has to run (empty outside of one), by
+// name, and whether each belongs to a stream outside of the current capture.
+std::vector<std::pair<std::string, bool>> backward_nodes() {
+    std::vector<std::pair<std::string, bool>> out;
+    const auto* const nodes = torch::autograd::get_current_graph_task_nodes_in_graph();
+    if (!nodes) return out;
+    const auto* const wanted = torch::autograd::get_current_graph_task_exec_info();  // empty: all of them
+    for (auto* const node : *nodes) {
+        if (wanted && !wanted->empty()) {
+            const auto it = wanted->find(node);
+            if (it == wanted->end() || !it->second.should_execute()) continue;
+        }
+        const auto stream = node->stream();
+        out.emplace_back(node->name(), stream.has_value() && outside_capture(*stream));
+    }
+    return out;
 }
 
 }  // namespace
 
 void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11::module_& proj) {
     namespace py = pybind11;
-    top.def("_leaves_of_another_stream", &leaves_of_another_stream);
+    top.def("_backward_nodes", &backward_nodes);
     const py::object none = py::none();
     rmsnorm.def("block_norm", &block_norm,
                 "u = RMSNorm(y) post_gamma; h = residual + residual_scale scale act(gate) u; n = RMSNorm(h) gamma.\n"

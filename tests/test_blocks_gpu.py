@@ -222,6 +222,46 @@ def test_capture_beside_an_eager_graph_is_refused(dev):
     torch.cuda.synchronize()
 
 
+def test_capture_beside_an_eager_graph_behind_other_operations(dev):
+    """The same where views, casts or whole eager results lie between the operator
+    and the leaves; leaves that no gradient is asked of do not matter."""
+    x = _rand((8, 512), torch.bfloat16, dev, 1)
+    gm = _rand((256,), torch.float32, dev, 2)
+    w = _rand((128, 256), torch.bfloat16, dev, 3)
+
+    def view():
+        return block_norm(x.view(16, 256), gamma=gm.to(torch.bfloat16))[1]
+
+    def project():
+        return fp8_linear(x.view(16, 256), w * 2)
+
+    eager = view()
+    for f, leaves in ((view, (x, gm)), (view, (gm,)), (project, (w,)), (lambda: fp8_linear(eager, w.detach()), (x,))):
+        kept = f()  # its graph lives
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with pytest.raises(RuntimeError, match="eager autograd graph.*AccumulateGrad"):
+            with torch.cuda.graph(graph, stream=side):
+                y = f()
+                torch.autograd.grad(y, leaves, torch.ones_like(y))
+        torch.cuda.synchronize()
+        y = None
+        torch.autograd.grad(kept, leaves, torch.ones_like(kept), retain_graph=True)  # the eager graph is as it was
+        kept = None
+    # eager (alive) holds x's and gm's accumulators, not w's
+    want = [t.clone() for t in torch.autograd.grad(fp8_linear(x.view(16, 256), w), (w,), torch.ones(16, 128, dtype=torch.bfloat16, device=dev))]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        y = fp8_linear(x.view(16, 256), w)
+        got = torch.autograd.grad(y, (w,), torch.ones_like(y))
+    for _ in range(3):
+        got[0].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0])
+
+
 def test_two_streams_at_once(exts, dev):
     """Calls on two streams share nothing."""
     x = [_rand((500, 2048), torch.bfloat16, dev, s, grad=False) for s in (1, 2)]
