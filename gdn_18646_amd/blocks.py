@@ -88,6 +88,12 @@ def block_norm(y, residual=None, gate=None, post_gamma=None, gamma=None, scale=N
     return _BlockNorm.apply(*tensors, float(residual_scale), act, float(eps))
 
 
+def _adjacent(x):
+    """x [M, K] with a row's elements adjacent, as the quantisation reads them;
+    expanded and transposed ones are copied."""
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
 class Fp8Weight:
     """A weight [N, K] (bf16 or fp32) as e4m3 codes with a scale for each 128 x 128
     block: ``codes`` / ``scales`` for x W^T and, with ``transposed``, ``codes_t`` /
@@ -97,15 +103,9 @@ class Fp8Weight:
         if weight.dim() != 2:
             raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
         self.shape = tuple(weight.shape)
-        out = compile_kernels()["proj"].fp8_quantize(weight.detach(), block_rows=BLOCK, rows=True, columns=transposed)
+        out = compile_kernels()["proj"].fp8_quantize(_adjacent(weight.detach()), block_rows=BLOCK, rows=True, columns=transposed)
         self.codes, self.scales = out[:2]
         self.codes_t, self.scales_t = out[2:] if transposed else (None, None)
-
-
-def _as_rows(x, K):
-    """x [..., K] as rows for the quantisation; expanded and transposed ones are copied."""
-    x = x.reshape(-1, K)
-    return x if x.stride(1) == 1 and x.stride(0) >= K else x.contiguous()
 
 
 class _Fp8Linear(torch.autograd.Function):
@@ -113,7 +113,7 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, record):
         proj = compile_kernels()["proj"]
         need_x, need_w = (record and need for need in ctx.needs_input_grad[:2])
-        x2 = _as_rows(x, x.shape[-1])
+        x2 = _adjacent(x.reshape(-1, x.shape[-1]))
         q = proj.fp8_quantize(x2, rows=True, columns=need_w)
         w = weight if isinstance(weight, Fp8Weight) else Fp8Weight(weight, transposed=need_x)
         if need_x and w.codes_t is None:
@@ -131,7 +131,7 @@ class _Fp8Linear(torch.autograd.Function):
         xt, xts, wt, wts = ctx.saved_tensors
         N, K = ctx.sizes
         need_x, need_w = ctx.needs_input_grad[:2]
-        d = proj.fp8_quantize(_as_rows(dy, N), dtype=torch.float8_e5m2, rows=need_x, columns=need_w)
+        d = proj.fp8_quantize(_adjacent(dy.reshape(-1, N)), dtype=torch.float8_e5m2, rows=need_x, columns=need_w)
         dx = dw = None
         if need_x:
             dx = proj.fp8_matmul(d[0], d[1], wt, wts, out_dtype=ctx.dtypes[0]).reshape(ctx.shape)

@@ -85,6 +85,23 @@ def test_fp8_linear_of_expanded_and_transposed(dev):
         fp8_linear(x, w[0])
 
 
+def test_fp8_linear_of_weights_that_are_views(dev):
+    """Transposed, expanded and sliced weights give what their copies give, and get
+    the same gradients."""
+    x = _rand((40, 256), torch.bfloat16, dev, 1)
+    base = _rand((256, 400), torch.bfloat16, dev, 2, 0.05)
+    dy = _rand((40, 400), torch.bfloat16, dev, 3, grad=False)
+    for view in (lambda b: b.t(), lambda b: b.t()[:1].expand(400, 256), lambda b: b.t()[:, :1].expand(400, 256),
+                 lambda b: b.t()[::2], lambda b: b[:, :256].contiguous()[:, ::2].repeat(1, 2)[:, :256]):
+        w = view(base)
+        n = w.shape[0]
+        copy = w.detach().clone(memory_format=torch.contiguous_format).requires_grad_()
+        y, z = fp8_linear(x, w), fp8_linear(x, copy)
+        assert torch.equal(y, z) and torch.equal(fp8_linear(x, Fp8Weight(w, transposed=True)), z)
+        got = torch.autograd.grad(y, (x, w), dy[:, :n])
+        assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(z, (x, copy), dy[:, :n])))
+
+
 def test_block_norm_gradients_through_autograd(dev):
     """Expanded, missing and accumulated gradients reach the kernel as they should."""
     D = 512
