@@ -72,9 +72,16 @@ __global__ __launch_bounds__(512) void gdn_fp8_quantize_kernel(QuantParams p) {
     } else if (p.codes) {
 #pragma unroll
         for (int i = 0; i < RT; ++i) rowb[i] = Fp8<FMT>::scale_byte(max16(amax8(f[i])));
-        if (cg == 0 && r0 < p.lds)
-            *reinterpret_cast<uint32_t*>(p.scales + static_cast<long long>(k0 / kBlk) * p.lds + r0) =
-                rowb[0] | rowb[1] << 8 | rowb[2] << 16 | rowb[3] << 24;
+        if (cg == 0) {
+            uint8_t* const at = p.scales + static_cast<long long>(k0 / kBlk) * p.lds + r0;
+            if (r0 + RT <= p.M) {
+                *reinterpret_cast<uint32_t*>(at) = rowb[0] | rowb[1] << 8 | rowb[2] << 16 | rowb[3] << 24;
+            } else {  // what lies past the last row is the caller's
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    if (r0 + i < p.M) at[i] = static_cast<uint8_t>(rowb[i]);
+            }
+        }
     }
     if (p.codes) {
 #pragma unroll

@@ -425,7 +425,8 @@ int gdn_block_norm_bwd_hip(const void* dh, int64_t lddh, const void* dn, int64_t
  * [ceil(M / 128), lds >= ceil(K / 128)] (128).  Along the columns, the same of
  * x^T: codes_t [K, ldt], columns M up to the next multiple of 128 zero; scales_t
  * [ceil(M / 128), ldst >= K] or [ceil(K / 128), ldst >= ceil(M / 128)].  Either
- * pair may be NULL.  Code rows 16-byte aligned.
+ * pair may be NULL.  Code rows 16-byte aligned.  What lies behind these in
+ * wider buffers is left as it is.
  */
 int gdn_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, int block_rows, int format,
                          uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, uint8_t* codes_t, int64_t ldt,

@@ -14,6 +14,8 @@ block's largest codes and scales.
 import pytest
 import torch
 
+from gdn_18646_amd import abi
+
 pytestmark = pytest.mark.gpu
 
 E4, E5, E8 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
@@ -96,6 +98,31 @@ def test_quantize_strided_rows(exts, dev):
         a = exts["proj"].fp8_quantize(wide[:, lo:hi], rows=True, columns=True)
         b = exts["proj"].fp8_quantize(wide[:, lo:hi].contiguous(), rows=True, columns=True)
         assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("M,K", [(1, 200), (97, 130), (126, 300), (130, 257)])
+def test_quantize_leaves_what_lies_behind(dev, M, K, block):
+    """Through the C ABI, into buffers that are wider and longer than the results."""
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(torch.bfloat16).to(dev)
+    Mp, Kp = _up(M, 128), _up(K, 128)
+    ldc, ldt, lds, ldst = Kp + 32, Mp + 48, _up(M, 16) + 144, _up(K, 16) + 144
+    codes, scales, codes_t, scales_t = (torch.full(s, 0x55, dtype=torch.uint8, device=dev)
+                                        for s in ((M + 2, ldc), (Kp // 128 + 1, lds), (K + 2, ldt), (Mp // 128 + 1, ldst)))
+    if block == 128:
+        scales, scales_t = scales.view(lds, -1), scales_t.view(ldst, -1)
+    abi.call("gdn_fp8_quantize_hip", x.data_ptr(), K, 0, M, K, block, 0, codes.data_ptr(), ldc, scales.data_ptr(), scales.stride(0),
+             codes_t.data_ptr(), ldt, scales_t.data_ptr(), scales_t.stride(0), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for got_c, got_s, t in ((codes, scales, x.cpu()), (codes_t, scales_t, x.t().cpu())):
+        rc, rs = _quantize64(t, block, E4)
+        want_c, want_s = torch.full(got_c.shape, 0x55, dtype=torch.uint8), torch.full(got_s.shape, 0x55, dtype=torch.uint8)
+        want_c[:rc.shape[0], :rc.shape[1]] = rc
+        rs = rs.t() if block == 1 else rs
+        want_s[:rs.shape[0], :rs.shape[1]] = rs
+        assert torch.equal(got_s.cpu(), want_s)
+        c = got_c.cpu()
+        assert ((c == want_c) | ((c & 0x7f == 0) & (want_c & 0x7f == 0))).all()
 
 
 # ---------------------------------------------------------------------------
