@@ -201,6 +201,8 @@ extern "C" int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, c
     constexpr int64_t kMost = int64_t{1} << 22, kRows = 0x7fffff00LL;
     if (lda > kMost || ldb > kMost || M > kRows || N > kRows || (M + 31) / 32 * ((N + 31) / 32) > 0x7fffffffLL)
         return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: problem too large (rows of at most 2^22 codes)");
+    if (b_block_rows == 1 && type_b_scale == GDN_F32 && N > int64_t{1} << 30)  // 32-bit byte offsets within a row of scales
+        return fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: problem too large (at most 2^30 columns with an fp32 scale each)");
     if (M == 0 || N == 0) return GDN_OK;
     if (!a || !a_scale || !b || !b_scale || !out) return fail(GDN_ERR_INVALID_ARGUMENT, "fp8_matmul: null pointer argument");
     if (!aligned(a, 16) || !aligned(b, 16) || lda % 16 != 0 || ldb % 16 != 0 || lda < K || ldb < K)

@@ -136,6 +136,16 @@ def test_product_refusals(bad, match):
         _mm(**bad)
 
 
+def test_product_refuses_scales_past_32_bit_offsets():
+    N = (1 << 30) + 16
+    wide = dict(brows=1, tsb=F32, M=3, N=N, ldbs=N, ldo=N)
+    with pytest.raises(GdnError, match="UNSUPPORTED.*2.30 columns"):
+        _mm(**wide)
+    for other in (dict(N=1 << 30), dict(tsb=E8), dict(brows=128, ldbs=2)):  # these are told of another fault
+        with pytest.raises(GdnError, match="null"):
+            _mm(**{**wide, **other, "a": None})
+
+
 def test_product_of_nothing():
     _mm(M=0)
     _mm(N=0)
