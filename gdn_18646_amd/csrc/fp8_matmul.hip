@@ -14,7 +14,7 @@
 
 namespace {
 
-template <int FA, int FB, bool OUT32, int WAVES>
+template <int FA, int FB, bool OUT32, bool F32, int WAVES>  // F32: b's scales are fp32
 __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::MatmulParams p, int scales, int rot_mask) {
     __shared__ f32x4 sums[WAVES][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -24,7 +24,6 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
     const uint8_t* const w = p.b + static_cast<size_t>(row) * p.ldb + 16 * g4;
     const uint8_t* const x = p.a + static_cast<size_t>(tok) * p.lda + 16 * g4;
     const bool rows = scales == gdn_fp8::kE8Row || scales == gdn_fp8::kF32Row;
-    const bool f32 = scales == gdn_fp8::kF32Block || scales == gdn_fp8::kF32Row;
     // the scale of the lane's row of b, its accumulator's column
     const size_t sstep = rows ? p.ldb_s : 1, sat = rows ? row : static_cast<size_t>(row / 128) * p.ldb_s;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -35,23 +34,32 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
         const u32x4* const wp = reinterpret_cast<const u32x4*>(w + static_cast<size_t>(kb) * 128);
         const u32x4* const xp = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(kb) * 128);
         const int sx = p.a_scale[kb * p.lda_s + tok];
-        int sw = 127;
+        uint32_t sw;  // b's scale as a power of two, and what is left of an fp32 one
         float fw = 1.f;
-        if (f32)
-            fw = static_cast<const float*>(p.b_scale)[sat + kb * sstep];
-        else
+        if constexpr (F32) {
+            const uint32_t bits = static_cast<const uint32_t*>(p.b_scale)[sat + kb * sstep];
+            sw = scale_byte_of(bits);
+            fw = scale_rest(bits, sw);
+        } else {
             sw = static_cast<const uint8_t*>(p.b_scale)[sat + kb * sstep];
+        }
         const i32x8 wc = join(wp[0], wp[4]), xc = join(xp[0], xp[4]);
         f32x4 t = {0.f, 0.f, 0.f, 0.f};
         if constexpr (OUT32) {
+            const int cx = nearby(sx), cw = nearby(static_cast<int>(sw));
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                t = mfma16x16x32(codes_to_bf16<FA>(xc[2 * q], xc[2 * q + 1], sx), codes_to_bf16<FB>(wc[2 * q], wc[2 * q + 1], sw), t);
-        } else {
-            t = mfma_fp8<FA, FB, 0, 0>(xc, wc, t, sx, sw);
-        }
+                t = mfma16x16x32(codes_to_bf16<FA>(xc[2 * q], xc[2 * q + 1], cx), codes_to_bf16<FB>(wc[2 * q], wc[2 * q + 1], cw), t);
+            // the tokens of accumulators 0 and 1; there are no others
+            const int left = sx - cx, left0 = __builtin_amdgcn_readlane(left, 0), left1 = __builtin_amdgcn_readlane(left, 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = fmaf(fw, t[i], acc[i]);
+            for (int i = 0; i < 2; ++i)
+                acc[i] += __builtin_amdgcn_ldexpf(fw * t[i], (i == 0 ? left0 : left1) + static_cast<int>(sw) - cw);
+        } else {
+            t = mfma_fp8<FA, FB, 0, 0>(xc, wc, t, sx, static_cast<int>(sw));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(fw, t[i], acc[i]);
+        }
     }
     sums[wave][lane] = acc;
     __syncthreads();
@@ -145,17 +153,20 @@ int launch(const gdn_fp8::MatmulParams& p, int scales, bool f32, hipStream_t str
     if (p.M <= 2) {
         int mask = 1;
         while (2 * mask <= p.K / 128) mask *= 2;
-        const auto few = [&](auto out32, auto waves) {
+        const auto few = [&](auto out32, auto f32_scales, auto waves) {
             constexpr int W = decltype(waves)::value;
             if (!gdn_host::grid_fits((p.N + 15) / 16, 64 * W)) return gdn_host::fail(GDN_ERR_UNSUPPORTED, "fp8_matmul: N=%d is too large for a launch", p.N);
-            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p,
+            hipLaunchKernelGGL((gdn_fp8_few_kernel<FA, FB, decltype(out32)::value, decltype(f32_scales)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p,
                                scales, mask - 1);
             return gdn_host::check_launch("gdn_fp8_few_kernel");
         };
-        const auto of_n = [&](auto out32) {
-            return p.N <= 4096 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
+        const auto of_n = [&](auto out32, auto f32_scales) {
+            return p.N <= 4096 ? few(out32, f32_scales, std::integral_constant<int, 8>{}) : few(out32, f32_scales, std::integral_constant<int, 4>{});
         };
-        return f32 ? of_n(std::true_type{}) : of_n(std::false_type{});
+        const auto of_scales = [&](auto out32) {
+            return scales == gdn_fp8::kF32Block || scales == gdn_fp8::kF32Row ? of_n(out32, std::true_type{}) : of_n(out32, std::false_type{});
+        };
+        return f32 ? of_scales(std::true_type{}) : of_scales(std::false_type{});
     }
     // The last columns past a multiple of 256 in a launch of their own, on a tile
     // of their size, where the fit says that this is faster than a column of

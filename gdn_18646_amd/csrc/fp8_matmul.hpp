@@ -59,9 +59,25 @@ __device__ __forceinline__ f32x4 mfma_fp8(const i32x8 x, const i32x8 w, const f3
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, c, FX, FW, SX, sx, SW, sw);
 }
 
-// Eight codes times a power of two as bf16, exactly (but where it leaves bf16's
-// range): an e8m0 scale byte s as the fp32 bits s << 23, 255 giving NaN.  Their
-// products are exact in fp32 and the bf16 MFMA sums them in fp32.
+// An fp32 scale as a power of two, which the instruction takes together with the
+// other operand's scale (a product of the two alone may leave fp32's range where the
+// result does not), and the rest, 1 to 2 in magnitude (0, infinite or NaN as the
+// scale is).
+__device__ __forceinline__ uint32_t scale_byte_of(uint32_t bits) { return min(bits >> 23 & 0xffu, 254u); }
+__device__ __forceinline__ float scale_rest(uint32_t bits, uint32_t byte) {
+    return __builtin_amdgcn_ldexpf(__uint_as_float(bits), 127 - static_cast<int>(byte));
+}
+
+// codes_to_bf16 is exact while code times scale lies in bf16's normal range: for
+// e8m0 bytes 64 to 191 (`near`, in bit 7 of each byte of a word) in any case, and
+// sums of 128 products stay in fp32's.  Others are converted with a byte nearby,
+// and the powers of two that this leaves, `s - nearby(s)`, are applied to the sums.
+__device__ __forceinline__ uint32_t near_bits(uint32_t bytes) { return bytes ^ bytes << 1; }
+__device__ __forceinline__ int nearby(int s) { return s == 255 ? 255 : min(max(s, 96), 159); }
+
+// Eight codes times a power of two as bf16: an e8m0 scale byte s as the fp32 bits
+// s << 23, 255 giving NaN.  Their products are exact in fp32 and the bf16 MFMA sums
+// them in fp32.
 template <int F>
 __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi, uint32_t scale_byte) {
     const float s = __uint_as_float(scale_byte << 23);

@@ -5,11 +5,16 @@
 // In tiles of columns x tokens (W = b, x = a).  A stage is one block of 128 k:
 // 128-byte rows, which reach LDS by DMA in a ring, every 8 lanes of a copy one
 // whole line, placed with an XOR swizzle that keeps the fragment reads at
-// linear-read speed; the stage's scales come with it.  bf16 results: one MFMA 16x16x128 takes a block: e8m0 scales are its
-// own scale operands and cost nothing; fp32 scales multiply its result on the
-// VALU, into the accumulator.  fp32 results: codes become bf16 in registers,
-// times their e8m0 scale, and the block takes four MFMA 16x16x32, whose sums
-// keep every bit that fp32 has.
+// linear-read speed; the stage's scales come with it.  bf16 results: one MFMA
+// 16x16x128 takes a block: e8m0 scales are its own scale operands and cost nothing;
+// of fp32 scales it takes the powers of two so, and the rest multiplies its result
+// on the VALU, into the accumulator.  fp32 results: codes become bf16 in registers,
+// times their e8m0 scale, and the block takes four MFMA 16x16x32, whose sums keep
+// every bit that fp32 has.  Codes times scales far from 1 leave bf16's range: a
+// workgroup that met one computes its tile again, block after block, for the rows
+// and columns that have such scales (2048 x 2048 x 2688 27.3 us, 27.5 with the
+// question; asking it before each block's product made the block wait for its
+// scales, 30.4 us).
 //
 // What bounds it: the matrix cores for large products, and there the card's
 // power: 8192 x 8192 x 8192 takes 413 us (2.66 PFLOP/s) with random codes and 345
@@ -251,33 +256,42 @@ __global__ __launch_bounds__(TL::waves * 64)
     };
 
     auto half = [&](const lds_u8* at, int h) { return *reinterpret_cast<const lds_u32x4*>(at + rd[h]); };
-    // W's scales of a staged block: WMT bytes of neighbouring columns in a word,
-    // the block's byte in each, or WMT floats.
-    auto w_bytes = [&](const lds_u8* st, int slice) -> uint32_t {
-        if constexpr (SB == gdn_fp8::kE8Block) {
-            return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wscale), slice & 63)) * 0x01010101u;
-        } else if constexpr (SB == gdn_fp8::kE8Row) {
+    // W's scales of a staged block: WMT bytes of neighbouring columns in a word, the
+    // block's byte in each, or WMT floats, whose powers of two the fp8 instruction
+    // takes as bytes (split_w; the bf16 instruction's sums are in range without).
+    auto read_sw = [&](const lds_u8* st, int slice, uint32_t (&sw)[WMT], float (&fw)[WMT]) {
+        if constexpr (kF32) {
+            const __attribute__((address_space(3))) float* const at = reinterpret_cast<const lds_f32*>(st + ST::off_ws) + 16 * WMT * wm + WMT * r16;
+#pragma unroll
+            for (int mt = 0; mt < WMT; ++mt) {
+                sw[mt] = 127u;
+                if constexpr (SB == gdn_fp8::kF32Row)
+                    fw[mt] = at[mt];
+                else
+                    fw[mt] = __int_as_float(__builtin_amdgcn_readlane(static_cast<int>(wscale), slice & 63));
+            }
+        } else if constexpr (SB == gdn_fp8::kE8Block) {
+            sw[0] = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wscale), slice & 63)) * 0x01010101u;
+        } else {
             const lds_u8* const at = st + ST::off_ws + 16 * WMT * wm + WMT * r16;
             if constexpr (WMT == 4)
-                return *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(at);
+                sw[0] = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(at);
             else if constexpr (WMT == 2)
-                return *reinterpret_cast<const lds_u16*>(at);
+                sw[0] = *reinterpret_cast<const lds_u16*>(at);
             else
-                return *at;
-        } else {
-            return 0x7f7f7f7fu;
+                sw[0] = *at;
         }
     };
-    auto w_floats = [&](const lds_u8* st, int slice, float (&f)[WMT]) {
-        const __attribute__((address_space(3))) float* const at = reinterpret_cast<const lds_f32*>(st + ST::off_ws) + 16 * WMT * wm + WMT * r16;
-#pragma unroll
-        for (int mt = 0; mt < WMT; ++mt) {
-            if constexpr (SB == gdn_fp8::kF32Row)
-                f[mt] = at[mt];
-            else
-                f[mt] = __int_as_float(__builtin_amdgcn_readlane(static_cast<int>(wscale), slice & 63));
+    auto split_w = [&](auto MT, uint32_t (&sw)[WMT], float (&fw)[WMT]) {
+        constexpr int mt = decltype(MT)::value;
+        if constexpr (kF32) {
+            const uint32_t bits = __float_as_uint(fw[mt]);
+            sw[mt] = scale_byte_of(bits);
+            fw[mt] = scale_rest(bits, sw[mt]);
         }
     };
+    // Column mt's byte.
+    auto byte_w = [&](int mt, const uint32_t (&sw)[WMT]) { return kF32 ? sw[mt] : sw[0] >> (8 * mt) & 0xffu; };
     // x's scales of a staged block, WNT bytes of neighbouring tokens: in words
     // where WNT is a power of two, else a register each.
     constexpr bool kWords = (WNT & (WNT - 1)) == 0;
@@ -299,15 +313,15 @@ __global__ __launch_bounds__(TL::waves * 64)
     };
 
     // One block's product of operands mt and nt into the accumulator.
-    auto multiply = [&](auto MT, auto NT, const i32x8& x, const i32x8& w, const uint32_t (&sx)[NSX], uint32_t sw, const float (&fw)[WMT]) {
+    auto multiply = [&](auto MT, auto NT, const i32x8& x, const i32x8& w, const uint32_t (&sx)[NSX], const uint32_t (&sw)[WMT], const float (&fw)[WMT]) {
         constexpr int mt = decltype(MT)::value, nt = decltype(NT)::value, bx = kWords ? nt % 4 : 0;
         const int s = static_cast<int>(sx[kWords ? nt / 4 : nt]);
         if constexpr (kF32) {
-            const f32x4 t = mfma_fp8<FA, FB, bx, mt>(x, w, f32x4{0.f, 0.f, 0.f, 0.f}, s, static_cast<int>(sw));
+            const f32x4 t = mfma_fp8<FA, FB, bx, 0>(x, w, f32x4{0.f, 0.f, 0.f, 0.f}, s, static_cast<int>(sw[mt]));
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[mt][nt][i] = fmaf(fw[mt], t[i], acc[mt][nt][i]);
         } else {
-            acc[mt][nt] = mfma_fp8<FA, FB, bx, mt>(x, w, acc[mt][nt], s, static_cast<int>(sw));
+            acc[mt][nt] = mfma_fp8<FA, FB, bx, mt>(x, w, acc[mt][nt], s, static_cast<int>(sw[0]));
         }
     };
 
@@ -315,6 +329,8 @@ __global__ __launch_bounds__(TL::waves * 64)
     int tile = static_cast<int>(blockIdx.x) >> 3;
     set_tile(tile);
     load_block_scales(0);
+    uint32_t x_near = ~0u, w_near = ~0u;  // the AND of the near_bits of the scales that the lane met
+
     if constexpr (TL::PHASED) {
         // Two groups of four waves, one wave of each on every SIMD, take turns:
         // while one multiplies, the other reads its next fragments and issues its
@@ -330,7 +346,7 @@ __global__ __launch_bounds__(TL::waves * 64)
         static_assert(!OUT32, "fp32 results run on the ring");
         i32x8 w0[TL::M0n], w1[TL::M1n], xf[TL::X0n];
         uint32_t sx[NSX];
-        uint32_t sw = 0;
+        uint32_t sw[WMT];
         float fw[WMT];
         constexpr int cX0 = TL::ncopy(0) + ST::scale_copies, cW1 = TL::ncopy(2), cX1 = TL::ncopy(3), cAll = ST::copies;
         auto frag = [&](const lds_u8* at) { return join(half(at, 0), half(at, 1)); };
@@ -350,9 +366,10 @@ __global__ __launch_bounds__(TL::waves * 64)
                     static_for<0, TL::M0n>([&](auto I) { w0[decltype(I)::value] = frag(stw + 16 * decltype(I)::value * kRowB); });
                     static_for<0, TL::X0n>([&](auto I) { xf[decltype(I)::value] = frag(stx + 16 * decltype(I)::value * kRowB); });
                     read_sx(st, sx);
-                    sw = w_bytes(st, kt);
-                    if constexpr (kF32) w_floats(st, kt, fw);
+                    read_sw(st, kt, sw, fw);
+                    static_for<0, TL::M0n>([&](auto I) { split_w(I, sw, fw); });
                 } else if constexpr (ph == 1) {
+                    static_for<TL::M0n, WMT>([&](auto I) { split_w(I, sw, fw); });
                     static_for<0, TL::M1n>([&](auto I) { w1[decltype(I)::value] = frag(stw + 16 * (TL::M0n + decltype(I)::value) * kRowB); });
                 } else if constexpr (ph == 2) {
                     static_for<0, TL::X1n>([&](auto I) { xf[decltype(I)::value] = frag(stx + 16 * (TL::X0n + decltype(I)::value) * kRowB); });
@@ -473,10 +490,11 @@ __global__ __launch_bounds__(TL::waves * 64)
                 const lds_u8* const stw = st + 16 * WMT * wm * kRowB;
                 uint32_t sx[NSX];
                 read_sx(st, sx);
-                const uint32_t sw = w_bytes(st, slice);
+                uint32_t sw[WMT];
                 float fw[WMT];
-                if constexpr (kF32) w_floats(st, slice, fw);
+                read_sw(st, slice, sw, fw);
                 if constexpr (!OUT32) {
+                    static_for<0, WMT>([&](auto MT) { split_w(MT, sw, fw); });
                     i32x8 x[WNT];
                     static_for<0, WNT>([&](auto NT) {
                         constexpr int nt = decltype(NT)::value;
@@ -488,6 +506,8 @@ __global__ __launch_bounds__(TL::waves * 64)
                         static_for<0, WNT>([&](auto NT) { multiply(MT, NT, x[decltype(NT)::value], w, sx, sw, fw); });
                     });
                 } else {
+                    x_near &= near_bits(sx[0]);
+                    if constexpr (!kF32) w_near &= near_bits(sw[0]);
                     f32x4 block[kF32 ? WMT : 1][kF32 ? WNT : 1];  // fp32 scales: this block's sums
                     if constexpr (kF32) {
 #pragma unroll
@@ -511,7 +531,7 @@ __global__ __launch_bounds__(TL::waves * 64)
                             });
                             static_for<0, WMT>([&](auto MT) {
                                 constexpr int mt = decltype(MT)::value;
-                                const bf16x8 w = codes_to_bf16<FB>(wc[mt][2 * q], wc[mt][2 * q + 1], sw >> (8 * mt) & 0xffu);
+                                const bf16x8 w = codes_to_bf16<FB>(wc[mt][2 * q], wc[mt][2 * q + 1], byte_w(mt, sw));
                                 static_for<0, WNT>([&](auto NT) {
                                     constexpr int nt = decltype(NT)::value;
                                     f32x4& c = kF32 ? block[kF32 ? mt : 0][kF32 ? nt : 0] : acc[mt][nt];
@@ -535,24 +555,120 @@ __global__ __launch_bounds__(TL::waves * 64)
         }
     }
 
+    // fp32 results: whether a wave met a scale that is not near, in any row but those
+    // past the last one, which may have any.
+    __shared__ uint32_t met_far[TL::waves];
+    if constexpr (OUT32) {
+        constexpr uint32_t x_top = 0x80808080u >> (8 * (4 - WNT)), w_top = 0x80808080u >> (8 * (4 - WMT));
+#pragma unroll
+        for (int nt = 0; nt < WNT; ++nt)
+            if (f0 + 16 * WNT * wn + WNT * r16 + nt >= p.M) x_near |= 0x80u << (8 * nt);
+        if constexpr (kRow) {
+#pragma unroll
+            for (int mt = 0; mt < WMT; ++mt)
+                if (c0 + 16 * WMT * wm + WMT * r16 + mt >= p.N) w_near |= 0x80u << (8 * mt);
+        }
+        met_far[wave] = __builtin_amdgcn_ballot_w64((~x_near & x_top) != 0 || (~w_near & w_top) != 0) != 0;
+    }
+    if constexpr (KS > 1 || OUT32) lds_barrier();  // every wave is past its last stage read
+    auto any_far = [&]() {
+        if constexpr (OUT32) return __builtin_amdgcn_ballot_w64(met_far[lane % TL::waves] != 0) != 0;
+        return false;
+    };
+    const auto part = [&](int k, int i) {
+        return reinterpret_cast<lds_f32x4*>(smem + (((k - 1) * TL::gwaves + gw) * WMT * WNT + i) * 1024 + 16 * lane);
+    };
     if constexpr (KS > 1) {
-        lds_barrier();  // every wave is past its last stage read
-        const auto part = [&](int k, int i) {
-            return reinterpret_cast<lds_f32x4*>(smem + (((k - 1) * TL::gwaves + gw) * WMT * WNT + i) * 1024 + 16 * lane);
-        };
         if (ks > 0) {
 #pragma unroll
             for (int i = 0; i < WMT * WNT; ++i) *part(ks, i) = acc[i / WNT][i % WNT];
         }
         lds_barrier();
-        if (ks > 0) return;
-#pragma unroll
-        for (int k = 1; k < KS; ++k)
-#pragma unroll
-            for (int i = 0; i < WMT * WNT; ++i) acc[i / WNT][i % WNT] += *part(k, i);
+        if (ks > 0 && !any_far()) return;
     }
-
-    store_tile(f0, c0);
+    if (KS == 1 || ks == 0) {
+        if constexpr (KS > 1) {
+#pragma unroll
+            for (int k = 1; k < KS; ++k)
+#pragma unroll
+                for (int i = 0; i < WMT * WNT; ++i) acc[i / WNT][i % WNT] += *part(k, i);
+        }
+        store_tile(f0, c0);
+    }
+    if constexpr (OUT32) {
+        if ((KS == 1 || ks == 0) && !any_far()) return;
+        // The tile once more, block after block, for the rows and columns that have a
+        // scale which is not near: with scales nearby, and the powers of two that are
+        // left on each block's sums.  Results of other rows and columns stay as they
+        // are, so that they do not depend on their neighbours.  K's first group of waves
+        // does it, the others keep to the barriers.
+        clear();
+        uint32_t far_tok = 0, far_col = 0;  // bit 4 nt + i: of accumulator (., nt)[i]'s token; bit mt: of (mt, .)'s column
+        for (int slice = 0; slice < nslices; ++slice) {
+            int lane = tid & 63;
+            asm volatile("" : "+v"(lane));  // nothing of this is kept over the loop above
+            const int r16 = lane & 15, g4 = lane >> 4;
+            lds_barrier();  // the last block's rows, or the groups' sums, are read
+            if (!kRow && slice % 64 == 0) load_block_scales(slice);
+            if (KS == 1 || ks == 0) {
+                issue_rows(0, slice);
+                issue_scales(0, slice);
+            }
+            wait_vm<0>();
+            lds_barrier();
+            if (KS > 1 && ks > 0) continue;
+            const lds_u8* const stx = smem + (TL::cols + 16 * WNT * wn) * kRowB;
+            const lds_u8* const stw = smem + 16 * WMT * wm * kRowB;
+            uint32_t sx[NSX], sw[WMT];
+            float fw[WMT];
+            read_sx(smem, sx);
+            read_sw(smem, slice, sw, fw);
+            static_for<0, WNT>([&](auto NT) {
+                constexpr int nt = decltype(NT)::value;
+                const int x = static_cast<int>(sx[0] >> (8 * nt) & 0xffu);
+                int s[4];  // the accumulators' tokens' scales
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[i] = smem[ST::off_xs + 16 * WNT * wn + WNT * (4 * g4 + i) + nt];
+                    far_tok |= (~near_bits(s[i]) >> 7 & 1u) << (4 * nt + i);
+                }
+                static_for<0, WMT>([&](auto MT) {
+                    constexpr int mt = decltype(MT)::value;
+                    const int w = static_cast<int>(byte_w(mt, sw));
+                    if (nt == 0) far_col |= (~near_bits(w) >> 7 & 1u) << mt;
+                    f32x4 sums = {0.f, 0.f, 0.f, 0.f};
+                    static_for<0, 2>([&](auto H) {
+                        const u32x4 xc = half(stx + 16 * nt * kRowB, decltype(H)::value), wc = half(stw + 16 * mt * kRowB, decltype(H)::value);
+                        __builtin_amdgcn_sched_barrier(0);  // one after the other, in few registers
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            sums = mfma16x16x32(codes_to_bf16<FA>(xc[2 * q], xc[2 * q + 1], nearby(x)),
+                                                codes_to_bf16<FB>(wc[2 * q], wc[2 * q + 1], nearby(w)), sums);
+                    });
+                    int left = w - nearby(w);
+                    float rest = 1.f;
+                    if constexpr (kF32) {
+                        const uint32_t bits = __float_as_uint(fw[mt]), byte = scale_byte_of(bits);
+                        left = static_cast<int>(byte) - 127;
+                        rest = scale_rest(bits, byte);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[mt][nt][i] += __builtin_amdgcn_ldexpf(rest * sums[i], s[i] - nearby(s[i]) + left);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            });
+        }
+        if (KS > 1 && ks > 0) return;
+        static_for<0, 4 * WNT>([&](auto J) {
+            constexpr int i = decltype(J)::value / WNT, nt = decltype(J)::value % WNT;
+            const int row = f0 + 16 * WNT * wn + WNT * (4 * g4 + i) + nt, col = c0 + 16 * WMT * wm + WMT * r16;
+#pragma unroll
+            for (int mt = 0; mt < WMT; ++mt) {
+                const float v[1] = {acc[mt][nt][i]};
+                if (row < p.M && col + mt < p.N && ((far_tok >> (4 * nt + i) | far_col >> mt) & 1u)) store_cols<OUT32>(p, row, col + mt, v);
+            }
+        });
+    }
 }
 
 }  // namespace

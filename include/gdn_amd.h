@@ -441,8 +441,10 @@ int gdn_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int6
  *   b_scale e8m0 or fp32 (type_b_scale), a 128 x 128 block each
  *   [ceil(N / 128), ldb_s >= K / 128] (b_block_rows 128) or a row and block
  *   each [K / 128, ldb_s >= N], 16-byte aligned, ldb_s % 16 == 0 (1).
- * K % 128 == 0 (zero codes pad), any M and N.  A row's sums do not depend on
- * other rows' values; their order follows M, N, K and the column.
+ * K % 128 == 0 (zero codes pad), any M, any N (up to 2^30 with an fp32 scale a
+ * row and block).  Scales may be anything that the types hold; only the product of
+ * the two has to be in fp32's range.  A row's sums do not depend on other rows'
+ * values; their order follows M, N, K and the column.
  */
 int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_t* a_scale, int64_t lda_s,
                        const uint8_t* b, int64_t ldb, int format_b, const void* b_scale, int64_t ldb_s, int b_block_rows,

@@ -287,3 +287,80 @@ def test_product_graph_replays_match_eager(exts, dev):
         exts["proj"].fp8_matmul(*exts["proj"].fp8_quantize(w), wq, ws)
         torch.cuda.synchronize()
         assert torch.equal(y, eager)
+
+
+# ---------------------------------------------------------------------------
+# Scales over their whole range
+# ---------------------------------------------------------------------------
+def _far_scales(M, N, K, bscale, rows, dev, seed=0):
+    """Scales of a from 2^-121 to 2^121 over K's blocks, and of b about their inverses, so that every
+    block adds to a result of ordinary size."""
+    g = torch.Generator().manual_seed(seed)
+    KB, NS = K // 128, N if rows == 1 else -(-N // 128)
+    mid = torch.linspace(6, 248, KB).round().int()
+    sa = mid + torch.randint(-5, 6, (M, KB), generator=g)
+    sb = 254 - mid + torch.randint(-5, 6, (NS, KB), generator=g)
+    sa, sb = sa.clamp(0, 254).to(torch.uint8).view(E8), sb.clamp(0, 254).to(torch.uint8).view(E8)
+    if bscale == "fp32":
+        sb = sb.float() * (1 + torch.rand(sb.shape, generator=g))
+    return sa.to(dev), sb.to(dev)
+
+
+FAR = [(1, 300, 2048), (2, 70, 2048), (16, 129, 2048), (40, 100, 2048), (70, 2048, 2048), (300, 1030, 2048), (700, 2100, 2048),
+       (300, 1030, 8448), (3, 130, 512), (100, 2500, 512), (300, 2040, 512), (520, 4090, 512), (1300, 4090, 512), (1594, 4090, 512),
+       (2092, 4090, 512), (2756, 4090, 512), (4100, 4090, 512)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("fa,fb", [(E4, E4), (E5, E4), (E5, E5)], ids=["e4e4", "e5e4", "e5e5"])
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
+@pytest.mark.parametrize("M,N,K", FAR)
+def test_product_of_far_scales(exts, dev, M, N, K, bscale, rows, fa, fb, out):
+    """Scales far from 1 that one operand's and the other's bring back together."""
+    a, _, b, _ = _operands(M, N, K, fa, fb, bscale, rows, dev)
+    sa, sb = _far_scales(M, N, K, bscale, rows, dev)
+    y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
+    assert torch.isfinite(y).all()
+    _check(y, a, sa, b, sb)
+
+
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
+@pytest.mark.parametrize("M,N,K", [(2, 70, 512), (40, 100, 512), (300, 1030, 512)])
+def test_far_scales_stay_in_their_rows(exts, dev, M, N, K, bscale, rows):
+    """A row of a and (by rows) one of b with far scales change no other result's bits."""
+    for out in (torch.float32, torch.bfloat16):
+        a, sa, b, sb = _operands(M, N, K, E4, E4, bscale, rows, dev)
+        want = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
+        s2, t2 = sa.clone(), sb.clone()
+        s2.view(torch.uint8)[1] = torch.tensor([3, 250, 20, 254], dtype=torch.uint8)
+        keep = torch.ones(M, N, dtype=torch.bool, device=dev)
+        keep[1] = False
+        if rows == 1:
+            t2[17] = torch.tensor([2.0 ** 100, 2.0 ** -100, 2.0 ** -126, 2.0 ** 126]).to(t2.dtype)
+            keep[:, 17] = False
+        got = exts["proj"].fp8_matmul(a, s2, b, t2, out_dtype=out)
+        assert torch.equal(got[keep], want[keep])
+
+
+def test_special_codes_and_scales_in_fp32_results(exts, dev):
+    """NaN codes and scales, infinite and zero scales reach exactly the outputs whose sums meet them."""
+    for M in (2, 40, 300):
+        for rows in (128, 1):
+            a, sa, b, sb = _operands(M, 300, 256, E4, E4, "e8m0", rows, dev)
+            clean = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=torch.float32)
+            sa.view(torch.uint8)[1, 0] = 255
+            sb.view(torch.uint8)[1, 1] = 255
+            y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=torch.float32)
+            want = torch.zeros(M, 300, dtype=torch.bool)
+            want[1], want[:, 128:256] = True, True
+            if rows == 1:
+                want[2:, 2:], want[0, 2:], want[:, :], want[:, 1] = False, False, False, True
+                want[1] = True
+            assert torch.equal(y.isnan().cpu(), want)
+            assert torch.equal(y[~want.to(dev)], clean[~want.to(dev)])
+    for out in (torch.float32, torch.bfloat16):
+        for M in (2, 40, 300):
+            a, sa, b, sb = _operands(M, 300, 256, E4, E4, "fp32", 1, dev)
+            sb[5], sb[6, 0], sb[7] = 0.0, float("inf"), 1e-42
+            y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
+            assert (y[:, 5] == 0).all() and not torch.isfinite(y[:, 6]).any() and torch.isfinite(y[:, [4, 5, 7]]).all()
