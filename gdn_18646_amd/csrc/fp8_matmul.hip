@@ -54,7 +54,7 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
             const int left = sx - cx, left0 = __builtin_amdgcn_readlane(left, 0), left1 = __builtin_amdgcn_readlane(left, 1);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                acc[i] += __builtin_amdgcn_ldexpf(fw * t[i], (i == 0 ? left0 : left1) + static_cast<int>(sw) - cw);
+                acc[i] = fmaf(fw, __builtin_amdgcn_ldexpf(t[i], (i == 0 ? left0 : left1) + static_cast<int>(sw) - cw), acc[i]);
         } else {
             t = mfma_fp8<FA, FB, 0, 0>(xc, wc, t, sx, static_cast<int>(sw));
 #pragma unroll

@@ -653,7 +653,7 @@ __global__ __launch_bounds__(TL::waves * 64)
                         rest = scale_rest(bits, byte);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[mt][nt][i] += __builtin_amdgcn_ldexpf(rest * sums[i], s[i] - nearby(s[i]) + left);
+                    for (int i = 0; i < 4; ++i) acc[mt][nt][i] = fmaf(rest, __builtin_amdgcn_ldexpf(sums[i], s[i] - nearby(s[i]) + left), acc[mt][nt][i]);
                     __builtin_amdgcn_sched_barrier(0);
                 });
             });
