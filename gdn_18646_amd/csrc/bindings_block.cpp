@@ -395,7 +395,9 @@ void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11
     proj.def("fp8_matmul", &fp8_matmul,
              "out [M, N] = (a a_scale) (b b_scale)^T for codes a [M, K], b [N, K] (float8_e4m3fn or float8_e5m2, K a multiple "
              "of 128) with a scale a block of 128: a_scale float8_e8m0fnu [M, K / 128]; b_scale float8_e8m0fnu or float32 "
-             "[N, K / 128] or, a 128 x 128 block each, [ceil(N / 128), K / 128].  fp32 sums.  Scales of a row and block each "
+             "[N, K / 128] or, a 128 x 128 block each, [ceil(N / 128), K / 128].  fp32 results sum every product in full; for "
+             "bf16 results the instruction drops up to 2^-10 of the product of the largest codes of a block, which matters where "
+             "large products of a block cancel.  Scales of a row and block each "
              "are read as fp8_quantize lays them out; others are copied into that layout first.",
              py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("out_dtype") = at::kBFloat16);
 }

@@ -289,6 +289,27 @@ def test_product_graph_replays_match_eager(exts, dev):
         assert torch.equal(y, eager)
 
 
+@pytest.mark.parametrize("bscale,rows", [("e8m0", 128), ("e8m0", 1), ("fp32", 128), ("fp32", 1)])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 512), (16, 129, 1152), (70, 2048, 512), (300, 1030, 512), (520, 4090, 384), (1300, 4090, 384), (2600, 2040, 384)])
+def test_product_of_large_terms_that_cancel(exts, dev, M, N, K, bscale, rows):
+    """In every block two products of 448^2 take each other away and the rest is small
+    beside them, 2^-17 of them or less for some: bf16 results are within the bound of
+    what the instruction drops, 2^-10 of 448^2 a block, fp32 results have all of it."""
+    g = torch.Generator().manual_seed(M)
+    small = torch.tensor([-1.0, -0.5, 0.5, 1.0])
+    a, b = (small[torch.randint(0, 4, (r, K), generator=g)] * 2.0 ** torch.randint(0, 2, (r, 1), generator=g) for r in (M, N))
+    for k in range(0, K, 128):
+        at = torch.randperm(128, generator=g)[:2] + k
+        a[:, at] = 448.0 * torch.where(torch.rand(M, 1, generator=g) < 0.5, -1.0, 1.0)
+        b[:, at] = torch.tensor([448.0, -448.0]) * torch.where(torch.rand(N, 1, generator=g) < 0.5, -1.0, 1.0)
+    _, sa, _, sb = _operands(M, N, K, E4, E4, bscale, rows, dev)
+    a, b = a.to(E4).to(dev), b.to(E4).to(dev)
+    for out in (torch.bfloat16, torch.float32):
+        y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
+        assert torch.isfinite(y).all()
+        _check(y, a, sa, b, sb)
+
+
 # ---------------------------------------------------------------------------
 # Scales over their whole range
 # ---------------------------------------------------------------------------
