@@ -81,13 +81,15 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp8_few_kernel(gdn_fp8::Matmul
 // kernels back to back on operands that the L2s do not hold: the tile that the fit
 // picks takes at most 1.12 times the best one's time (fp32 1.05) and 1.003 times on
 // average; 39 tiles were timed, those here are the ones whose absence costs.
-// Small products are bound by how fast a CU takes in its rows, some 45 GB/s, so
-// the small tiles spread them over the CUs, split K over groups of waves and keep
-// several stages under way: 16 x 2048 x 8192 takes 6.8 us on 16 x 16 with eight
-// groups and four stages (a workgroup a CU), 8.6 with two stages, 10.5 on 32 x 32;
-// 16 x 8224 x 2048 6.2 on 16 x 16 with three a CU, 6.8 on 64 x 32.  256 x 160 and 128
-// x 192 are up to 9% faster where they make one round of what others make two of
-// or a half (1500 x 6176 x 2048: 22.7 us on 256 x 160, 24.3 on 256 x 192).
+// Small products take some 3.3 us whatever their K (c + a), and then what a CU needs
+// to take in its rows: by b, 58 GB/s with one 256 x 256 tile, 76 to 78 with one of
+// 16 x 16 or 64 x 128, 110 with three of 16 x 16.  So the small tiles spread the rows
+// over the CUs, split K over groups of waves and keep several stages under way: 16 x
+// 2048 x 8192 takes 6.8 us on 16 x 16 with eight groups and four stages (a workgroup
+// a CU), 8.6 with two stages, 10.5 on 32 x 32; 16 x 8224 x 2048 6.2 on 16 x 16 with
+// three a CU, 6.8 on 64 x 32.  256 x 160 and 128 x 192 are up to 9% faster where they
+// make one round of what others make two of or a half (1500 x 6176 x 2048: 22.7 us on
+// 256 x 160, 24.3 on 256 x 192).
 struct TileCost {
     int tile, cols, toks, per_cu;
     float c, a1, b1, a2, b2;  // per_cu above 1: alone (1) and with per_cu on each CU (2)
