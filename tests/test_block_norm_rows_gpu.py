@@ -50,8 +50,8 @@ def _forward64(v, rs):
 def _close(x, ref, tol, what):
     half = torch.finfo(x.dtype).eps / 2
     far = (x.double() - ref).abs() - (half * ref.abs() + (1 + half) * tol + 1e-30)
-    assert x.shape == ref.shape and not (far > 0).any(), \
-        f"{what}: {(far > 0).sum().item()} values, the worst {far.max().item():.3g} past its bound"
+    assert x.shape == ref.shape and (far <= 0).all(), \
+        f"{what}: {(~(far <= 0)).sum().item()} values, the worst {far.max().item():.3g} past its bound"
 
 
 # sequences x tokens: two rows and more for every place of a workgroup, and a few rows left
