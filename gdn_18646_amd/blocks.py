@@ -73,7 +73,8 @@ def block_norm(y, residual=None, gate=None, post_gamma=None, gamma=None, scale=N
     """(h, n) of a block's output y [..., D]; n is None without ``gamma``.
 
     residual: y's shape.  gate: y's shape, [B, D] (a gate a sequence of
-    y [B, ..., D]) or [D]; act: none, sigmoid, silu or tanh.  post_gamma, gamma,
+    y [B, ..., D]; the backward pass takes at most 65535 of them) or [D]; act: none,
+    sigmoid, silu or tanh.  post_gamma, gamma,
     scale: [D].  What is None is left out.  Differentiable in every tensor, in
     reverse mode; an operand with a forward-mode tangent raises.
     """

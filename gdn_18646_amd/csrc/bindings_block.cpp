@@ -382,7 +382,8 @@ void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11
                 py::arg("inplace") = false);
     rmsnorm.def("block_norm_backward", &block_norm_backward,
                 "Gradients of block_norm: [dresidual, dy, dgate, dpost_gamma, dgamma, dscale], None for absent inputs.  dh, dn "
-                "(either may be None): those of h and n; rstd_y, rstd_h: block_norm's with stats.",
+                "(either may be None): those of h and n; rstd_y, rstd_h: block_norm's with stats.  At most 65535 gate rows that "
+                "several rows share.",
                 py::arg("dh"), py::arg("dn"), py::arg("y"), py::arg("residual") = none, py::arg("gate") = none,
                 py::arg("post_gamma") = none, py::arg("gamma") = none, py::arg("scale") = none,
                 py::arg("residual_scale") = 1.0, py::arg("act") = "none", py::arg("rstd_y") = none, py::arg("rstd_h") = none);
