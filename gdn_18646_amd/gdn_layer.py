@@ -173,12 +173,13 @@ class GDNLayerCustom:
             raise ValueError("prefill takes a scalar dt_bias (as the reference kernel)")
         if cu_seqlens is not None:
             return self._forward_packed(x, cu_seqlens, mask, return_state, state, xn)
-        x = xn if xn is not None else x
+        given = xn is not None
+        x = xn if given else x
         B, T, _ = x.shape
         Dd, Hh, dk, dv = self.D, self.H, self.DK, self.DV
         if mask is None:  # empty = every token kept (no fill kernel)
             mask = torch.empty(0, dtype=torch.float32, device=x.device)
-        xn = xn.contiguous() if xn is not None else self._rmsnorm(x.reshape(B * T, Dd)).reshape(B, T, Dd)
+        xn = xn.contiguous() if given else self._rmsnorm(x.reshape(B * T, Dd)).reshape(B, T, Dd)
         st = state or {}
         outs = self._layer.in_proj(xn, self.W_qkvab, self.conv_qkv, Hh, dk, dv,
                                    st.get('conv_q'), st.get('conv_k'), st.get('conv_v'), bool(return_state))
@@ -197,6 +198,8 @@ class GDNLayerCustom:
         nc = self.CK - 1
         if T >= nc:
             xn_hist = xn[:, T - nc:]
+            if given:  # the state's own rows: a decode step may write them in place
+                xn_hist = xn_hist.clone()
         else:
             prev = st.get('xn')
             if prev is None:

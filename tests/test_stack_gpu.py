@@ -39,6 +39,22 @@ def test_layer_takes_a_normed_input(layers, dev):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("B,T", [(1, 3), (1, 20), (2, 3), (2, 20), (1, 2)])
+def test_a_state_does_not_share_the_normed_input(layers, dev, B, T):
+    """Decoding in place from the state of a forward call leaves the call's xn as it was."""
+    x = _x((B, T, D), dev, 8)
+    xn = layers[0]._rmsnorm(x.reshape(-1, D)).reshape(B, T, D)
+    keep = xn.clone()
+    _, state = layers[0].forward(None, xn=xn, return_state=True)
+    _, want = layers[0].forward(x, return_state=True)
+    for t in range(3):
+        y, _ = layers[0].decode(_x((B, 1, D), dev, 30 + t), state, inplace=True)
+        y2, _ = layers[0].decode(_x((B, 1, D), dev, 30 + t), want, inplace=True)
+        assert torch.equal(y, y2)
+    assert torch.equal(xn, keep)
+    assert all(torch.equal(state[k], want[k]) for k in want)
+
+
 @pytest.mark.parametrize("post,scaled,final", [(False, False, True), (True, True, True), (True, False, False)])
 def test_stack_is_its_layers(layers, dev, post, scaled, final):
     """Against the same chain written out in fp32 torch around the layers; each of
