@@ -207,6 +207,8 @@ extern "C" int gdn_block_norm_hip(const void* y, int64_t ldy, const void* residu
     if (!gamma && (n || rstd_h)) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: n and rstd_h need gamma");
     if (!post_gamma && rstd_y) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rstd_y needs post_gamma");
     if (gate && rows_per_gate <= 0) return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rows_per_gate=%lld", (long long)rows_per_gate);
+    if (R > 1 && ((h && ldh < D) || (n && ldn < D)))
+        return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: rows of h or n overlap (ldh=%lld, ldn=%lld, D=%lld)", (long long)ldh, (long long)ldn, (long long)D);
     if (codes && (!scales || !aligned(codes, 16) || ldc % 16 != 0 || ldc < (D + kBlk - 1) / kBlk * kBlk || lds < R))
         return fail(GDN_ERR_INVALID_ARGUMENT, "block_norm: codes need scales [D / 128, >= R], 16-byte alignment and rows padded to 128");
     const size_t by = type_bytes(type_y), br = type_bytes(type_r), bp = type_bytes(type_p);

@@ -378,7 +378,8 @@ enum { GDN_ACT_NONE = 0, GDN_ACT_SIGMOID = 1, GDN_ACT_SILU = 2, GDN_ACT_TANH = 3
  *   fp32 fp32 fp32.  ld*: elements from a row to the next.  h may be written
  *   over the rows of residual, y or a gate a token (same address, type and
  *   stride); a call whose h is not apart from an input otherwise, by its range
- *   of memory or by columns within a common stride, is refused.
+ *   of memory or by columns within a common stride, is refused, and so are rows
+ *   of h or n that overlap.  The other outputs have to lie apart from the inputs.
  *   codes [R, ldc >= D padded to 128] and scales [ceil(D / 128), lds >= R]: n
  *   (h without gamma), unrounded, as e4m3 codes in blocks of 128 columns (see
  *   gdn_fp8_quantize_hip); codes 16-byte aligned, ldc % 16 == 0.

@@ -53,6 +53,13 @@ def test_block_norm_refuses_h_over_what_others_read(over, name):
         _norm(**{**far, **over})
 
 
+@pytest.mark.parametrize("bad", [dict(ldh=255), dict(ldh=0), dict(ldh=-256), dict(ldn=255), dict(ldn=0)])
+def test_block_norm_refuses_results_whose_rows_overlap(bad):
+    apart = dict(residual=1 << 20, gate=1 << 21, y=1 << 22, post=1 << 23, gamma=1 << 23, scale=1 << 23)
+    with pytest.raises(GdnError, match="INVALID_ARGUMENT.*overlap"):
+        _norm(**apart, **bad)
+
+
 def test_no_rows_is_no_call():
     _norm(R=0, residual=None)
     _norm(R=0, y=None)
