@@ -385,3 +385,22 @@ def test_special_codes_and_scales_in_fp32_results(exts, dev):
             sb[5], sb[6, 0], sb[7] = 0.0, float("inf"), 1e-42
             y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
             assert (y[:, 5] == 0).all() and not torch.isfinite(y[:, 6]).any() and torch.isfinite(y[:, [4, 5, 7]]).all()
+
+
+@pytest.mark.parametrize("rows", [128, 1])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 512), (2, 70, 512), (40, 100, 512), (300, 1030, 512), (1300, 4090, 256)])
+def test_negative_fp32_scales(exts, dev, M, N, K, rows):
+    a, sa, b, sb = _operands(M, N, K, E4, E4, "fp32", rows, dev)
+    sb[::2, 0] *= -1
+    sb[:, 1] *= -1
+    for out in (torch.float32, torch.bfloat16):
+        y = exts["proj"].fp8_matmul(a, sa, b, sb, out_dtype=out)
+        assert torch.isfinite(y).all()
+        ref, _ = _product64(a, sa, b, sb)
+        _, mag = _product64(a, sa, b, sb.abs())
+        tol = (K + 2) * 2.0 ** -24 * mag
+        if out == torch.bfloat16:
+            top = lambda t, s: t.double().abs().view(t.shape[0], -1, 128).amax(2) * s  # noqa: E731
+            wide = sb.double().abs().repeat_interleave(rows, 0)[:N]
+            tol += 2.0 ** -10 * top(a, sa.double()) @ top(b, wide).t() + 2.0 ** -8 * (ref.abs() + tol)
+        assert ((y.double() - ref).abs() <= tol).all()
