@@ -279,6 +279,37 @@ def test_capture_beside_an_eager_graph_behind_other_operations(dev):
         assert torch.equal(got[0], want[0])
 
 
+def test_capture_on_two_streams(dev):
+    """Nodes on a second stream that belongs to the capture are no eager ones."""
+    x, gm = _rand((16, 256), torch.bfloat16, dev, 1), _rand((256,), torch.bfloat16, dev, 2)
+    w = _rand((128, 256), torch.bfloat16, dev, 3, 0.05)
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def step():
+        second.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(second):
+            n = block_norm(x, gamma=gm)[1]
+        y = fp8_linear(x, w)
+        torch.cuda.current_stream().wait_stream(second)
+        grads = torch.autograd.grad([y, n], (x, gm, w), [torch.ones_like(y), torch.ones_like(n)])
+        torch.cuda.current_stream().wait_stream(second)
+        return [t.detach() for t in (y, n, *grads)]
+
+    first.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(first):
+        want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=first):
+        got = step()
+    for _ in range(3):
+        for t in got:
+            t.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_two_streams_at_once(exts, dev):
     """Calls on two streams share nothing."""
     x = [_rand((500, 2048), torch.bfloat16, dev, s, grad=False) for s in (1, 2)]
