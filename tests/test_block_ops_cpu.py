@@ -44,7 +44,7 @@ def test_block_norm_refusals(bad, match):
     (dict(gate=FAKE + 2048), "gate"),
     (dict(gate=FAKE, rpg=2), "gate"),                    # rows 0 and 1 are read by others
     (dict(gate=FAKE, rpg=4), "gate"),
-    (dict(post=FAKE), "post_gamma"), (dict(gamma=FAKE + 3072), "gamma"), (dict(scale=FAKE + 1500), "scale")])
+    (dict(post=FAKE), "post_gamma"), (dict(gamma=FAKE + 2048), "gamma"), (dict(scale=FAKE + 1500), "scale")])
 def test_block_norm_refuses_h_over_what_others_read(over, name):
     """h in every second 512 bytes of a buffer, at FAKE; the other operands elsewhere."""
     far = dict(y=1 << 20, residual=FAKE, ldr=512, ldy=512, ldg=512, gate=2 << 20, post=3 << 20, gamma=3 << 20, scale=3 << 20, h=FAKE, ldh=512,
