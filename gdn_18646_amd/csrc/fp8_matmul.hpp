@@ -52,8 +52,8 @@ __device__ __forceinline__ i32x8 join(const u32x4 lo, const u32x4 hi) {
 //
 // The instruction lines a block's products up with the largest and drops what
 // lies below about 2^-17 of that (measured: 2^-1 next to 1.75 * 2^16 is lost),
-// 1.4e-5 of a sum over normal values: nothing beside a bf16 result's 2^-9, too
-// much for an fp32 one.
+// 1.4e-5 of a sum over normal values: nothing beside a bf16 result's 2^-8 unless
+// large products cancel, too much for an fp32 one.
 template <int FX, int FW, int SX, int SW>
 __device__ __forceinline__ f32x4 mfma_fp8(const i32x8 x, const i32x8 w, const f32x4 c, int sx, int sw) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, c, FX, FW, SX, sx, SW, sw);
@@ -69,9 +69,10 @@ __device__ __forceinline__ float scale_rest(uint32_t bits, uint32_t byte) {
 }
 
 // codes_to_bf16 is exact while code times scale lies in bf16's normal range: for
-// e8m0 bytes 64 to 191 (`near`, in bit 7 of each byte of a word) in any case, and
-// sums of 128 products stay in fp32's.  Others are converted with a byte nearby,
-// and the powers of two that this leaves, `s - nearby(s)`, are applied to the sums.
+// e8m0 bytes 64 to 191 in any case (`near`, in bit 7 of each byte of a word).  Others
+// are converted with a byte nearby, 96 to 159, with which a block's sum is in fp32's
+// range whatever the codes, and the powers of two that this leaves, `s - nearby(s)`,
+// are applied to the sum.
 __device__ __forceinline__ uint32_t near_bits(uint32_t bytes) { return bytes ^ bytes << 1; }
 __device__ __forceinline__ int nearby(int s) { return s == 255 ? 255 : min(max(s, 96), 159); }
 
