@@ -252,8 +252,13 @@ int with_types(int ty, int tr, int tp, F&& f) {
     return f(bf16(), bf16(), bf16());
 }
 
-// (mean + eps)^-1/2 of a sum of squares, 1 ulp.
-__device__ __forceinline__ float rstd_of(float sum, float inv_D, float eps) { return __builtin_amdgcn_rsqf(fmaf(sum, inv_D, eps)); }
+// (mean + eps)^-1/2 of a sum of squares, 1 ulp.  The hardware's takes subnormal
+// numbers, rows of under 1e-19 without eps, for zero.
+__device__ __forceinline__ float rstd_of(float sum, float inv_D, float eps) {
+    const float v = fmaf(sum, inv_D, eps);
+    const bool tiny = v < 0x1p-126f;
+    return __builtin_amdgcn_rsqf(tiny ? v * 0x1p32f : v) * (tiny ? 0x1p16f : 1.f);
+}
 
 inline size_t type_bytes(int t) { return t == GDN_F32 ? 4 : 2; }
 

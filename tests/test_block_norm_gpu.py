@@ -246,6 +246,23 @@ def test_empty_and_zero_rows(exts, dev):
     assert (h == 0).all() and (codes.float() == 0).all() and (scales.float() == 1).all()
 
 
+@pytest.mark.parametrize("size", [1e-15, 1e-18, 1e-19, 3e-20, 1e-20])
+@pytest.mark.parametrize("D", [64, 300, 2048])
+def test_tiny_rows_without_eps(exts, dev, D, size):
+    """Rows whose mean of squares is subnormal: each square is off by half of 2^-149,
+    which the norm's other roundings join."""
+    y = torch.randn(5, D, generator=torch.Generator().manual_seed(D)).to(dev) * size
+    gm = torch.ones(D, device=dev)
+    h, n, _, _, ry, rh = exts["rmsnorm"].block_norm(y, post_gamma=gm, gamma=gm, eps=0.0, stats=True)
+    _, n2, _, _ = exts["rmsnorm"].block_norm(y, gamma=gm, eps=0.0)
+    ms = y.double().pow(2).mean(-1, keepdim=True)
+    ref = y.double() / ms.sqrt()
+    tol = (F32 + 2.0 ** -150 / ms) * ref.abs()
+    for t in (h, n, n2):
+        assert ((t.double() - ref).abs() <= tol).all()
+    assert ((ry.double() * ms.sqrt()[:, 0] - 1).abs() <= F32 + 2.0 ** -150 / ms[:, 0]).all() and torch.isfinite(rh).all()
+
+
 def test_not_finite_rows_stay_in_their_row(exts, dev):
     v = _inputs((4, 2048), gate="token")
     clean = exts["rmsnorm"].block_norm(**v, act="silu", quantize=True)
