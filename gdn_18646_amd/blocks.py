@@ -132,16 +132,16 @@ class _Fp8Linear(torch.autograd.Function):
         xt, xts, wt, wts = ctx.saved_tensors
         N, K = ctx.sizes
         need_x, need_w = ctx.needs_input_grad[:2]
+        if dy.numel() == 0:  # no tokens, or no columns
+            return (torch.zeros(ctx.shape, dtype=ctx.dtypes[0], device=dy.device) if need_x else None,
+                    torch.zeros(N, K, dtype=ctx.dtypes[1], device=dy.device) if need_w else None, None)
         d = proj.fp8_quantize(_adjacent(dy.reshape(-1, N)), dtype=torch.float8_e5m2, rows=need_x, columns=need_w)
         dx = dw = None
         if need_x:
             dx = proj.fp8_matmul(d[0], d[1], wt, wts, out_dtype=ctx.dtypes[0]).reshape(ctx.shape)
         if need_w:
             dt, dts = d[-2:]
-            if dt.shape[1] == 0:  # no tokens
-                dw = torch.zeros(N, K, dtype=ctx.dtypes[1], device=dy.device)
-            else:
-                dw = proj.fp8_matmul(dt, dts, xt, xts, out_dtype=ctx.dtypes[1])
+            dw = proj.fp8_matmul(dt, dts, xt, xts, out_dtype=ctx.dtypes[1])
         return dx, dw, None
 
 

@@ -71,6 +71,15 @@ def test_fp8_linear_partial_gradients(dev):
     assert y.shape == (0, 128) and dx.shape == (0, 256) and (dw == 0).all()
 
 
+def test_fp8_linear_of_nothing(dev):
+    """No tokens and no columns, forward and backward."""
+    for shape, N in (((0, 256), 128), ((3, 0, 256), 128), ((5, 256), 0), ((0, 256), 0)):
+        x, w = _rand(shape, torch.bfloat16, dev, 1), _rand((N, 256), torch.bfloat16, dev, 2)
+        y = fp8_linear(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+        assert y.shape == (*shape[:-1], N) and dx.shape == shape and dw.shape == (N, 256) and (dx == 0).all() and (dw == 0).all()
+
+
 def test_fp8_linear_of_expanded_and_transposed(dev):
     """Layouts that autograd and views make: a sum's expanded gradient, expanded and
     transposed inputs give what their copies give."""
