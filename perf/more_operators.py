@@ -138,21 +138,18 @@ def _packed(codes):
     return (c[:, 0::2] | c[:, 1::2] << 4).contiguous().view(E2M1X2)
 
 
-def _e8m0(e):
-    return (e + 127).to(torch.uint8).view(E8M0)
-
-
 def _operand(x, rows, fmt):
-    """(codes, scales) of x as the framework keeps them: 4-bit ones with a row's scales adjacent, 8-bit ones with a
-    block's, columns 16 apart at least."""
-    codes, e = _blocks(x, rows, fmt)
-    M, n = x.shape[0], FORMATS[fmt][0]
-    s = _e8m0(e[:, ::n])
+    """(codes, scales) of x as the framework keeps them: 4-bit ones in rows of whole 256 values with scales [M, K / 128,
+    4], 8-bit ones with scales [M, K / 128], both by blocks of 128 first and then by rows, 16 rows at a time."""
+    n, M = FORMATS[fmt][0], x.shape[0]
     if fmt == "e2m1":
-        return _packed(codes), s.contiguous()
-    buf = torch.zeros(s.shape[1], -(-M // 16) * 16, dtype=torch.uint8, device=x.device)
-    buf[:, :M] = s.view(torch.uint8).t()
-    return codes.to(E4M3 if fmt == "e4m3" else E5M2), buf.view(E8M0)[:, :M].t()
+        x = torch.nn.functional.pad(x, (0, -x.shape[1] % 256))
+    codes, e = _blocks(x, rows, fmt)
+    s = (e[:, ::n] + 127).to(torch.uint8).view(M, -1, 128 // n)
+    buf = torch.zeros(s.shape[1], -(-M // 16) * 16, 128 // n, dtype=torch.uint8, device=x.device)
+    buf[:, :M] = s.transpose(0, 1)
+    s = buf[:, :M].transpose(0, 1).view(E8M0)
+    return (_packed(codes), s) if fmt == "e2m1" else (codes.to(E4M3 if fmt == "e4m3" else E5M2), s[:, :, 0])
 
 
 def _shapes(c):
@@ -208,12 +205,13 @@ def _values(codes, scales):
         v = table[torch.stack((bytes_ & 15, bytes_ >> 4), -1).view(codes.shape[0], -1).int()]
     else:
         v = codes.float()
-    n = v.shape[1] // scales.shape[1]
-    return (v.view(v.shape[0], -1, n) * scales.float()[:, :, None]).view(v.shape)
+    s = scales.float().reshape(v.shape[0], -1)
+    return (v.view(v.shape[0], s.shape[1], -1) * s[:, :, None]).view(v.shape)
 
 
 def _plain_product(st):
-    y = _values(st["a"], st["a_scale"]) @ _values(st["b"], st["b_scale"]).t()
+    a, b = _values(st["a"], st["a_scale"]), _values(st["b"], st["b_scale"])
+    y = a @ b[:, :a.shape[1]].t()
     return y.to(TYPES[st["case"]["out"]])
 
 
@@ -327,7 +325,7 @@ def _decoded64(codes, scales):
         n = 32
     else:
         v, n = codes.double(), 128
-    return v * scales.double().index_select(1, torch.arange(v.shape[1], device=v.device) // n)
+    return v * scales.double().flatten(1).index_select(1, torch.arange(v.shape[1], device=v.device) // n)
 
 
 def exact(case, seed):
@@ -337,7 +335,7 @@ def exact(case, seed):
         x = st["x"].double()
         return [_as4(t, c["block"]) for there, t in ((c["rows"], x), (c["columns"], x.t())) if there]
     if c["kind"] == "product":
-        return torch.mm(_decoded64(st["a"], st["a_scale"]), _decoded64(st["b"], st["b_scale"]).t())
+        return torch.mm(_decoded64(st["a"], st["a_scale"])[:, :c["K"]], _decoded64(st["b"], st["b_scale"])[:, :c["K"]].t())
     if c["kind"] == "train":
         x, w, dy = st["x"].detach().double(), st["w"].detach().double(), st["dy"].double()
         w4 = _as4(w, 32)
