@@ -24,8 +24,9 @@ EXT = os.path.join(PKG, "_gdn_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 HIP_SOURCES = ["abi.cpp", "decode.hip", "prefill.hip", "rmsnorm.hip", "proj.hip", "proj_packed.hip", "proj_plain.hip", "layer.hip",
                "block_norm.hip", "block_norm_bwd.hip", "fp8_quantize.hip", "fp8_matmul.hip", "fp8_mm_e4m3_e4m3.hip",
-               "fp8_mm_e4m3_e5m2.hip", "fp8_mm_e5m2_e4m3.hip", "fp8_mm_e5m2_e5m2.hip"]
-BINDING_SOURCES = ["bindings.cpp", "bindings_block.cpp"]
+               "fp8_mm_e4m3_e5m2.hip", "fp8_mm_e5m2_e4m3.hip", "fp8_mm_e5m2_e5m2.hip", "fp4_quantize.hip", "fp4_matmul.hip",
+               "fp4_mm_e2m1.hip", "fp4_mm_e4m3.hip", "fp4_mm_e5m2.hip", "grad_norm.hip"]
+BINDING_SOURCES = ["bindings.cpp", "bindings_block.cpp", "bindings_fp4.cpp", "bindings_grads.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # Packed-FP32 VALU forms are disabled on purpose (some give wrong results on
 # the target boxes); the host pass warns that it does not know the feature.

@@ -16,6 +16,13 @@ _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_D = ctypes.c_double
+
+
+class GradTensor(ctypes.Structure):
+    """gdn_grad_t: one tensor of gdn_grad_norm_hip and gdn_clip_grad_norm_hip."""
+    _fields_ = [("grad", _P), ("out", _P), ("n", _I64), ("type", _I), ("type_out", _I)]
+
 
 # name -> (restype, argtypes), in declaration order of include/gdn_amd.h
 SIGNATURES = {
@@ -58,6 +65,12 @@ SIGNATURES = {
                                + [_P, _SZ, _P]),
     "gdn_fp8_quantize_hip": (_I, [_P, _I64, _I, _I64, _I64, _I, _I] + [_P, _I64] * 4 + [_P]),
     "gdn_fp8_matmul_hip": (_I, [_P, _I64, _I, _P, _I64] * 2 + [_I, _I, _P, _I64, _I] + [_I64] * 3 + [_P]),
+    "gdn_fp4_quantize_hip": (_I, [_P, _I64, _I, _I64, _I64, _I] + [_P, _I64] * 4 + [_P]),
+    "gdn_fp4_dequantize_hip": (_I, [_P, _I64] * 3 + [_I, _I64, _I64, _P]),
+    "gdn_fp4_matmul_hip": (_I, [_P, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I] + [_I64] * 3 + [_P]),
+    "gdn_grad_norm_workspace_bytes": (_SZ, [_I64]),
+    "gdn_grad_norm_hip": (_I, [_P, _I64, _P, _P, _SZ, _P]),
+    "gdn_clip_grad_norm_hip": (_I, [_P, _I64, _D, _P, _P, _SZ, _P]),
 }
 
 STATUS = {0: "GDN_OK", 1: "GDN_ERR_INVALID_ARGUMENT", 2: "GDN_ERR_UNSUPPORTED",

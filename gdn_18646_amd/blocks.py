@@ -1,6 +1,7 @@
-"""What stands between and beside layers: differentiable block norms and 8-bit
-linear layers on the kernels ``rmsnorm.block_norm`` and ``proj.fp8_quantize`` /
-``proj.fp8_matmul``.
+"""What stands between and beside layers: differentiable block norms, linear layers
+on 8-bit and 4-bit codes and the clipping of gradients, on the kernels
+``rmsnorm.block_norm``, ``proj.fp8_quantize`` / ``proj.fp8_matmul``,
+``proj.fp4_quantize`` / ``proj.fp4_matmul`` and ``grads``.
 
 * ``block_norm``: the norms before and after a block fused with its gate and
   residual scale,
@@ -12,7 +13,11 @@ linear layers on the kernels ``rmsnorm.block_norm`` and ``proj.fp8_quantize`` /
 * ``fp8_linear``: ``x W^T`` on 8-bit codes with a power-of-two scale for each
   block of 128 (1 x 128 of activations and gradients, 128 x 128 of weights),
   forward in e4m3, gradients in e5m2;
-* ``Fp8Weight``: a weight quantised once, for serving.
+* ``fp4_linear``: the same with the weight in 4-bit codes and a scale for each 32
+  x 32 of them, activations in 8-bit or 4-bit codes, gradients in e5m2;
+* ``Fp8Weight``, ``Fp4Weight``: a weight quantised once, for serving;
+* ``grad_norm``, ``clip_grad_norm``: the 2-norm of many gradients together, and
+  their clipping to it, in place or into other tensors.
 
 The kernels' own entry points (``compile_kernels()['rmsnorm'].block_norm`` and so
 on) take the same operands without recording gradients.
@@ -24,9 +29,10 @@ from torch.autograd.function import once_differentiable
 
 from . import compile_kernels, native_extension
 
-__all__ = ["block_norm", "fp8_linear", "Fp8Weight"]
+__all__ = ["block_norm", "fp8_linear", "Fp8Weight", "fp4_linear", "Fp4Weight", "grad_norm", "clip_grad_norm"]
 
 BLOCK = 128
+E2M1X2, E4M3, E5M2 = torch.float4_e2m1fn_x2, torch.float8_e4m3fn, torch.float8_e5m2
 
 
 def _check_capture():
@@ -156,3 +162,104 @@ def fp8_linear(x, weight):
     if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"fp8_linear: x [..., {x.shape[-1]}] and weight {tuple(weight.shape)}")
     return _Fp8Linear.apply(x, weight, torch.is_grad_enabled())
+
+
+class Fp4Weight:
+    """A weight [N, K] (bf16 or fp32) as e2m1 codes with a scale for each block_rows (32
+    or 1) x 32 block: ``codes`` / ``scales`` for x W^T and, with ``transposed``,
+    ``codes_t`` / ``scales_t`` for the gradient of x.  With block_rows=32 both stand for
+    the same weight, as ``fp4_linear`` quantises a tensor; blocks of 1 x 32 are finer,
+    along each product's own sum."""
+
+    def __init__(self, weight, transposed=False, block_rows=32):
+        if weight.dim() != 2:
+            raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+        self.shape = tuple(weight.shape)
+        out = compile_kernels()["proj"].fp4_quantize(_adjacent(weight.detach()), block_rows=block_rows, rows=True, columns=transposed)
+        self.codes, self.scales = out[:2]
+        self.codes_t, self.scales_t = out[2:] if transposed else (None, None)
+
+    def dequantize(self, dtype=torch.bfloat16):
+        """The weight that the codes stand for, [N, K]."""
+        return compile_kernels()["proj"].fp4_dequantize(self.codes, self.scales, columns=self.shape[1], dtype=dtype)
+
+
+class _Fp4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, activations, record):
+        proj = compile_kernels()["proj"]
+        need_x, need_w = (record and need for need in ctx.needs_input_grad[:2])
+        x2 = _adjacent(x.reshape(-1, x.shape[-1]))
+        q8 = activations == E4M3  # from one read with the codes that dW takes
+        q = proj.fp8_quantize(x2, rows=q8, columns=need_w) if q8 or need_w else []
+        a = q[:2] if q8 else proj.fp4_quantize(x2)
+        w = weight if isinstance(weight, Fp4Weight) else Fp4Weight(weight, transposed=need_x)
+        if need_x and w.codes_t is None:
+            raise ValueError("fp4_linear: the gradient of x needs an Fp4Weight with transposed=True")
+        ctx.save_for_backward(*(q[-2:] if need_w else (None, None)), *((w.codes_t, w.scales_t) if need_x else (None, None)))
+        ctx.shape, ctx.dtypes = x.shape, (x.dtype, getattr(weight, "dtype", None))
+        ctx.sizes = w.shape
+        return proj.fp4_matmul(a[0], a[1], w.codes, w.scales, out_dtype=x.dtype).reshape(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _check_capture()
+        proj = compile_kernels()["proj"]
+        xt, xts, wt, wts = ctx.saved_tensors
+        N, K = ctx.sizes
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if dy.numel() == 0:  # no tokens, or no columns
+            return (torch.zeros(ctx.shape, dtype=ctx.dtypes[0], device=dy.device) if need_x else None,
+                    torch.zeros(N, K, dtype=ctx.dtypes[1], device=dy.device) if need_w else None, None, None)
+        d = proj.fp8_quantize(_adjacent(dy.reshape(-1, N)), dtype=E5M2, rows=need_x, columns=need_w)
+        dx = dw = None
+        if need_x:
+            dx = proj.fp4_matmul(d[0], d[1], wt, wts, out_dtype=ctx.dtypes[0]).reshape(ctx.shape)
+        if need_w:
+            dt, dts = d[-2:]
+            dw = proj.fp8_matmul(dt, dts, xt, xts, out_dtype=ctx.dtypes[1])
+        return dx, dw, None, None
+
+
+def fp4_linear(x, weight, activations=E4M3):
+    """x [..., K] times weight^T, the weight in 4-bit codes: [..., N] of x's type.
+
+    weight: a tensor [N, K], quantised in the call in blocks of 32 x 32 and
+    differentiable (the quantisation passes gradients through), or an ``Fp4Weight``.
+    activations: torch.float8_e4m3fn (blocks of 1 x 128) or torch.float4_e2m1fn_x2
+    (blocks of 1 x 32, twice the speed for many tokens).  x and a weight tensor are bf16
+    or fp32; fp32 ones get fp32 results.  In the backward pass the incoming gradient is
+    quantised to e5m2 in blocks of 1 x 128 along each product's own sum, and multiplied
+    with the 4-bit weight for the gradient of x and with x in e4m3 along its tokens for
+    the weight's.
+    """
+    if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"fp4_linear: x [..., {x.shape[-1] if x.dim() else ''}] and weight {tuple(weight.shape)}")
+    if activations not in (E4M3, E2M1X2):
+        raise ValueError(f"fp4_linear: activations in torch.float8_e4m3fn or torch.float4_e2m1fn_x2, got {activations}")
+    return _Fp4Linear.apply(x, weight, activations, torch.is_grad_enabled())
+
+
+def grad_norm(grads):
+    """The 2-norm of all the gradients' elements together, a float32 tensor of no axes.
+
+    grads: a list of bf16 and fp32 tensors on one GPU, such as ``[p.grad for p in
+    parameters if p.grad is not None]``; None among them is left out, and without any
+    the norm is 0.
+    """
+    grads = [g for g in grads if g is not None]
+    return native_extension().grads.norm(grads) if grads else torch.zeros(())
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)), where norm is
+    ``grad_norm(grads)``, in place or into ``out`` (tensors of the same shapes, bf16 or
+    fp32, for an optimiser that keeps its own); returns the norm before.
+
+    Nothing is read back to the host, so the call can be captured into a graph.  A norm
+    that is NaN makes every result NaN.
+    """
+    if out is None:
+        grads = [g for g in grads if g is not None]
+    return native_extension().grads.clip(grads, float(max_norm), out) if grads else torch.zeros(())

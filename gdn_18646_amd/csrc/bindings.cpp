@@ -20,6 +20,8 @@
 #include "../../include/gdn_amd.h"
 
 void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11::module_& proj);  // bindings_block.cpp
+void bind_fp4_ops(pybind11::module_& proj);                                                        // bindings_fp4.cpp
+void bind_grad_ops(pybind11::module_& grads);                                                      // bindings_grads.cpp
 
 namespace {
 
@@ -627,4 +629,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     mj.def("forward", &proj_forward, "Fused linear projection + causal depthwise conv1d + SiLU (bf16)",
            py::arg("input"), py::arg("weight"), py::arg("conv_w"));
     bind_block_ops(m, mr, mj);
+    bind_fp4_ops(mj);
+    auto mg = m.def_submodule("grads", "Norm and clipping of gradients");
+    bind_grad_ops(mg);
 }

@@ -2,28 +2,11 @@
 //   rmsnorm.block_norm, rmsnorm.block_norm_backward, proj.fp8_quantize, proj.fp8_matmul
 // Errors surface as RuntimeError; launches go to torch's current HIP stream of
 // the tensors' device.
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/graph_task.h>
-#include <torch/extension.h>
 
-#include "../../include/gdn_amd.h"
+#include "bindings_common.hpp"
 
 namespace {
-
-using at::Tensor;
-using Opt = std::optional<Tensor>;
-
-void* stream_of(const Tensor& t) {
-    return reinterpret_cast<void*>(c10::hip::getCurrentHIPStream(t.get_device()).stream());
-}
-
-void check_status(int st, const char* who) {
-    TORCH_CHECK(st == GDN_OK, who, ": ", gdn_status_string(st), ": ", gdn_last_error());
-}
-
-bool given(const Opt& t) { return t.has_value() && t->defined(); }
 
 // An operand as rows of its last axis: how many, and the elements from one to the next.
 struct Rows {
@@ -49,11 +32,6 @@ Rows rows_of(const Tensor& t, const char* name) {
     }
     TORCH_CHECK(r.ld >= D, name, " must not have rows that overlap");
     return r;
-}
-
-int type_of(const Tensor& t, const char* name) {
-    TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name, " must be bfloat16 or float32");
-    return t.scalar_type() == at::kFloat ? GDN_F32 : GDN_BF16;
 }
 
 void check_like(const Tensor& t, const Tensor& y, const char* name) {
@@ -117,22 +95,6 @@ Operands operands(const Tensor& y, const Opt& residual, const Opt& gate, const O
     o.scale = param(scale, "scale");
     if (o.tp < 0) o.tp = o.tr;
     return o;
-}
-
-int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
-// An output on t's device, without the dispatcher's way round (a third of a
-// small call's host time).
-Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& t) {
-    return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
-}
-
-// Scales of M rows in KB blocks as the product reads them: a block's adjacent.
-Tensor down_columns(int64_t M, int64_t KB, at::ScalarType type, const Tensor& t) {
-    const int64_t Mp = up(M, 16);
-    Tensor s = at::detail::empty_strided_cuda({Mp, KB}, {1, Mp}, type, t.device());
-    if (Mp != M) s.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({M, KB}), at::IntArrayRef({1, Mp}));
-    return s;
 }
 
 std::vector<Opt> block_norm(const Tensor& y, const Opt& residual, const Opt& gate, const Opt& post_gamma, const Opt& gamma,
@@ -235,11 +197,6 @@ std::vector<Opt> block_norm_backward(const Opt& dh, const Opt& dn, const Tensor&
     return out;
 }
 
-int format_of(const Tensor& t, const char* name) {
-    TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kFloat8_e5m2, name, " must be float8_e4m3fn or float8_e5m2");
-    return t.scalar_type() == at::kFloat8_e4m3fn ? GDN_E4M3 : GDN_E5M2;
-}
-
 std::vector<Tensor> fp8_quantize(const Tensor& x, int64_t block_rows, at::ScalarType dtype, bool rows, bool columns) {
     TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a GPU tensor [M, K]");
     TORCH_CHECK(x.size(1) <= 1 || x.stride(1) == 1, "x must have adjacent elements along its last axis");
@@ -275,22 +232,6 @@ std::vector<Tensor> fp8_quantize(const Tensor& x, int64_t block_rows, at::Scalar
                                       ptr[3], lds[1], stream_of(x)),
                  "fp8_quantize");
     return out;
-}
-
-// Scales [M, KB] of a row and block each, with a block's adjacent and 16 apart
-// from the next: as given where they are, else laid out so.
-Tensor scale_rows(const Tensor& s, int64_t* ld) {
-    const int64_t M = s.size(0), KB = s.size(1), e = s.element_size();
-    const int64_t step = KB > 1 ? s.stride(1) : up(M, 16);
-    if ((M <= 1 || s.stride(0) == 1) && step % 16 == 0 && step >= M && reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0 &&
-        static_cast<int64_t>(s.storage().nbytes()) >= (s.storage_offset() + (KB - 1) * step + up(M, 16)) * e) {
-        *ld = step;
-        return s;
-    }
-    auto t = down_columns(M, KB, s.scalar_type(), s);
-    *ld = up(M, 16);
-    t.view(e == 1 ? at::kByte : at::kFloat).copy_(s.view(e == 1 ? at::kByte : at::kFloat));
-    return t;
 }
 
 Tensor fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, at::ScalarType out_dtype) {

@@ -1,0 +1,227 @@
+// Entry point of the product with 4-bit weights, the rule that picks its kernel, and
+// the kernel for one token or two.
+//
+// gdn_fp4_few_kernel (a decode step's token): what counts is the weights' bytes. A
+// workgroup owns 16 columns; each of its waves takes every WAVES-th 256 values of K
+// straight from memory into MFMA fragments (no LDS: nothing is used twice), and
+// the waves' sums meet in LDS.  The workgroups of an XCD begin at different
+// places: 16 rows at a stride of a power of two lie in one or two of its L2's
+// channels, and in step they would all wait for the same ones.
+#include "fp4_matmul.hpp"
+
+namespace {
+
+template <int FA, bool OUT32, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void gdn_fp4_few_kernel(gdn_fp4::MatmulParams p, int rot_mask) {
+    constexpr bool kFp4X = FA == GDN_E2M1, kBf16 = OUT32 && !kFp4X;
+    __shared__ f32x4 sums[WAVES][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g4 = lane >> 4;
+    const int n0 = blockIdx.x * 16, nblocks = p.K / 128, nslices = (nblocks + 1) / 2;
+    const int row = min(n0 + r16, p.N - 1), tok = min(r16, p.M - 1);
+    const uint8_t* const w = p.b + static_cast<size_t>(row) * p.ldb;
+    const uint8_t* const x = p.a + static_cast<size_t>(tok) * p.lda;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int rot = static_cast<int>(blockIdx.x >> 3) & rot_mask;
+    for (int i = wave; i < nslices; i += WAVES) {
+        const int slice = i + rot < nslices ? i + rot : i + rot - nslices;
+        const u32x4* const wp = reinterpret_cast<const u32x4*>(w + static_cast<size_t>(slice) * 128) + g4;
+        const u32x4 wc[2] = {wp[0], wp[4]};
+        u32x4 xc[2][2];
+        uint32_t sw[2], sx[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sw[h] = p.b_scale[(2 * slice + h) * p.ldb_s + row];
+            if constexpr (kFp4X) {
+                xc[h][0] = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(slice) * 128)[4 * h + g4];
+                sx[h] = reinterpret_cast<const uint32_t*>(p.a_scale)[(2 * slice + h) * p.lda_s + tok] >> (8 * g4);
+            } else {
+                const int kb = min(2 * slice + h, nblocks - 1);
+                const u32x4* const xp = reinterpret_cast<const u32x4*>(x + static_cast<size_t>(kb) * 128);
+                xc[h][0] = xp[kBf16 ? 2 * g4 : g4];
+                xc[h][1] = xp[kBf16 ? 2 * g4 + 1 : 4 + g4];
+                sx[h] = p.a_scale[kb * p.lda_s + tok];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!kFp4X && 2 * slice + h >= nblocks) break;
+            if constexpr (!kBf16) {
+                i32x8 xv;
+                if constexpr (kFp4X)
+                    xv = codes4(xc[h][0]);
+                else
+                    xv = join(xc[h][0], xc[h][1]);
+                acc = mfma_fp4<FA, 0, 0>(xv, codes4(wc[h]), acc, sx[h], sw[h] >> (8 * g4));
+            } else {
+                const uint32_t most = largest_byte(sw[h]), own = byte_over(sw[h] >> (8 * g4) & 0xffu, most);
+                f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    t = mfma16x16x32(codes_to_bf16<FA>(xc[h][q / 2][2 * (q % 2)], xc[h][q / 2][2 * (q % 2) + 1], 127u), fp4_to_bf16(wc[h][q], own), t);
+                // the tokens of accumulators 0 and 1; there are no others
+#pragma unroll
+                for (int t2 = 0; t2 < 2; ++t2)
+                    acc[t2] += scaled_sum(t[t2], static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sx[h]), t2)), most);
+            }
+        }
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) acc += sums[i][lane];
+    if (n0 + r16 >= p.N) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v[1] = {acc[i]};
+        if (4 * g4 + i < p.M) store_cols<OUT32>(p, 4 * g4 + i, n0 + r16, v);
+    }
+}
+
+// What a call on a tile takes, us: c + rounds (a + b slices of 256 of K), a round being
+// 256 workgroups, or, where a CU holds per_cu of them, up to per_cu times 256,
+// with a and b between a1, b1 (one a CU) and a2, b2 (per_cu).
+struct TileCost {
+    int tile, cols, toks, per_cu;
+    float c, a1, b1, a2, b2;  // per_cu above 1: alone (1) and with per_cu on each CU (2)
+};
+constexpr TileCost kCost4[] = {
+    {gdn_fp4::k256x256, 256, 256, 1, 0.f, 6.75f, 1.135f, 0.f, 0.f},
+    {gdn_fp4::k256x192, 256, 192, 1, 0.f, 6.22f, 1.012f, 0.f, 0.f},
+    {gdn_fp4::k256x160, 256, 160, 1, 0.f, 5.75f, 0.904f, 0.f, 0.f},
+    {gdn_fp4::k256x128, 256, 128, 1, 0.f, 5.56f, 0.725f, 0.f, 0.f},
+    {gdn_fp4::k128x192, 128, 192, 1, 0.f, 4.78f, 0.688f, 0.f, 0.f},
+    {gdn_fp4::k128x128, 128, 128, 1, 0.f, 4.28f, 0.511f, 0.f, 0.f},
+    {gdn_fp4::k64x128, 64, 128, 1, 0.40f, 4.22f, 0.315f, 0.f, 0.f},
+    {gdn_fp4::k64x64, 64, 64, 1, 0.92f, 3.20f, 0.222f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 1.26f, 2.73f, 0.144f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.48f, 2.16f, 0.106f, 0.f, 0.f},
+    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.64f, 1.78f, 0.054f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.60f, 0.70f, 0.064f, 1.37f, 0.112f},
+};
+constexpr TileCost kCost8[] = {
+    {gdn_fp4::k256x160, 256, 160, 1, 0.f, 5.75f, 1.604f, 0.f, 0.f},
+    {gdn_fp4::k256x128, 256, 128, 1, 0.f, 5.56f, 1.325f, 0.f, 0.f},
+    {gdn_fp4::k128x192, 128, 192, 1, 0.f, 4.78f, 1.188f, 0.f, 0.f},
+    {gdn_fp4::k128x128, 128, 128, 1, 0.f, 4.28f, 0.911f, 0.f, 0.f},
+    {gdn_fp4::k64x128, 64, 128, 1, 0.40f, 4.22f, 0.615f, 0.f, 0.f},
+    {gdn_fp4::k64x64, 64, 64, 1, 0.92f, 3.20f, 0.402f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 1.26f, 2.73f, 0.244f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.48f, 2.16f, 0.166f, 0.f, 0.f},
+    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.64f, 1.78f, 0.084f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.60f, 0.70f, 0.104f, 1.37f, 0.172f},
+};
+constexpr TileCost kCost32[] = {
+    {gdn_fp4::k128x128, 128, 128, 1, 1.01f, 3.08f, 1.915f, 0.f, 0.f},
+    {gdn_fp4::k64x128, 64, 128, 1, 0.11f, 4.40f, 1.025f, 0.f, 0.f},
+    {gdn_fp4::k64x64, 64, 64, 1, 0.76f, 3.32f, 0.646f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 1.09f, 3.09f, 0.380f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.34f, 2.25f, 0.280f, 0.f, 0.f},
+    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.63f, 1.84f, 0.114f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.61f, 0.70f, 0.151f, 1.53f, 0.223f},
+};
+
+struct Choice {
+    int tile;
+    float us;
+};
+template <size_t N>
+Choice choose_tile(const TileCost (&table)[N], long long M, long long cols, int K) {
+    constexpr long long kCUs = 256;
+    const float nk = static_cast<float>((K + 255) / 256);
+    Choice best = {0, 0.f};
+    for (size_t i = 0; i < N; ++i) {
+        const TileCost& t = table[i];
+        const long long tiles = (M + t.toks - 1) / t.toks * ((cols + t.cols - 1) / t.cols);
+        const float alone = t.a1 + t.b1 * nk, full = t.a2 + t.b2 * nk;
+        float us = t.c;
+        if (t.per_cu == 1) {
+            us += static_cast<float>((tiles + kCUs - 1) / kCUs) * alone;
+        } else {
+            const long long round = kCUs * t.per_cu, each = (tiles % round + kCUs - 1) / kCUs;  // workgroups a CU in the last one
+            us += static_cast<float>(tiles / round) * full;
+            if (each > 0) us += alone + static_cast<float>(each - 1) / static_cast<float>(t.per_cu - 1) * (full - alone);
+        }
+        if (i == 0 || us < best.us) best = {t.tile, us};
+    }
+    return best;
+}
+
+template <int FA>
+int launch(const gdn_fp4::MatmulParams& p, bool f32, hipStream_t stream) {
+    if (p.M <= 2) {
+        int mask = 1;
+        while (2 * mask <= (p.K + 255) / 256) mask *= 2;
+        const auto few = [&](auto out32, auto waves) {
+            constexpr int W = decltype(waves)::value;
+            hipLaunchKernelGGL((gdn_fp4_few_kernel<FA, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, mask - 1);
+            return gdn_host::check_launch("gdn_fp4_few_kernel");
+        };
+        const auto of_n = [&](auto out32) {
+            return p.N <= 4096 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
+        };
+        return f32 ? of_n(std::true_type{}) : of_n(std::false_type{});
+    }
+    const auto choose = [&](long long cols) {
+        if constexpr (FA == GDN_E2M1) return choose_tile(kCost4, p.M, cols, p.K);
+        return f32 ? choose_tile(kCost32, p.M, cols, p.K) : choose_tile(kCost8, p.M, cols, p.K);
+    };
+    // The last columns past a multiple of 256 in a launch of their own, on a tile
+    // of their size, where the fit says that this is faster than a column of
+    // large tiles for them.
+    const Choice whole = choose(p.N);
+    const int rest = p.N % 256, main = p.N - rest;
+    if (rest > 0 && main > 0) {
+        const Choice left = choose(main), right = choose(rest);
+        if (left.us + right.us < whole.us) {
+            gdn_fp4::MatmulParams q = p;
+            q.N = main;
+            const int st = gdn_fp4::launch_tile<FA>(left.tile, f32, q, stream);
+            if (st != GDN_OK) return st;
+            q.N = rest;
+            q.b = p.b + static_cast<size_t>(main) * p.ldb;
+            q.b_scale = p.b_scale + main;
+            q.out = static_cast<uint8_t*>(p.out) + static_cast<size_t>(main) * (f32 ? 4 : 2);
+            return gdn_fp4::launch_tile<FA>(right.tile, f32, q, stream);
+        }
+    }
+    return gdn_fp4::launch_tile<FA>(whole.tile, f32, p, stream);
+}
+
+}  // namespace
+
+extern "C" int gdn_fp4_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_t* a_scale, int64_t lda_s, const uint8_t* b,
+                                  int64_t ldb, const uint8_t* b_scale, int64_t ldb_s, void* out, int64_t ldo, int type_out, int64_t M,
+                                  int64_t N, int64_t K, void* stream) {
+    using gdn_host::aligned;
+    using gdn_host::fail;
+    if (M < 0 || N < 0 || K <= 0) return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_matmul: M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+    if (format_a != GDN_E4M3 && format_a != GDN_E5M2 && format_a != GDN_E2M1) return fail(GDN_ERR_UNSUPPORTED, "fp4_matmul: format %d of a", format_a);
+    const bool fp4 = format_a == GDN_E2M1;
+    if (K % (fp4 ? 256 : 128) != 0)
+        return fail(GDN_ERR_UNSUPPORTED, "fp4_matmul: K=%lld must be a multiple of %d (pad with zero codes)", (long long)K, fp4 ? 256 : 128);
+    if (type_out != GDN_BF16 && type_out != GDN_F32) return fail(GDN_ERR_UNSUPPORTED, "fp4_matmul: type %d of out", type_out);
+    // 32-bit copy offsets within a tile and a row of scales
+    constexpr int64_t kMost = int64_t{1} << 22, kRows = int64_t{1} << 28, kScales = int64_t{1} << 29;
+    if (K > kMost || lda > kMost || ldb > kMost || M > kRows || N > kRows || lda_s > kScales || ldb_s > kScales || (M + 15) / 16 * ((N + 15) / 16) > 0x7fffffffLL)
+        return fail(GDN_ERR_UNSUPPORTED, "fp4_matmul: problem too large (rows of at most 2^22 bytes, 2^28 of them)");
+    if (M == 0 || N == 0) return GDN_OK;
+    if (!a || !a_scale || !b || !b_scale || !out) return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_matmul: null pointer argument");
+    const int64_t row_a = fp4 ? K / 2 : K, row_b = (K + 255) / 256 * 128;
+    if (!aligned(a, 16) || !aligned(b, 16) || lda % 16 != 0 || ldb % 16 != 0 || lda < row_a || ldb < row_b)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_matmul: codes need 16-byte aligned rows of at least %lld (a) and %lld (b) bytes", (long long)row_a, (long long)row_b);
+    const int64_t whole = fp4 ? 4 : 16;
+    if (!aligned(a_scale, 16) || lda_s % whole != 0 || lda_s < M)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_matmul: a's scales [K / 128, lda_s%s] need 16-byte aligned rows of at least M", fp4 ? ", 4" : "");
+    if (!aligned(b_scale, 16) || ldb_s % 4 != 0 || ldb_s < N)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_matmul: b's scales [K / 128, ldb_s, 4] need 16-byte aligned rows of at least N");
+    if (!aligned(out, type_out == GDN_F32 ? 4 : 2) || ldo < N) return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_matmul: out unaligned or ldo < N");
+    gdn_fp4::MatmulParams p = {};
+    p.a = a, p.b = b, p.a_scale = a_scale, p.b_scale = reinterpret_cast<const uint32_t*>(b_scale), p.out = out;
+    p.lda = lda, p.ldb = ldb, p.lda_s = lda_s, p.ldb_s = ldb_s, p.ldo = ldo;
+    p.M = static_cast<int>(M), p.N = static_cast<int>(N), p.K = static_cast<int>(K);
+    const auto s = static_cast<hipStream_t>(stream);
+    const bool f32 = type_out == GDN_F32;
+    return fp4 ? launch<GDN_E2M1>(p, f32, s) : format_a == GDN_E4M3 ? launch<GDN_E4M3>(p, f32, s) : launch<GDN_E5M2>(p, f32, s);
+}

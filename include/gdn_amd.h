@@ -34,6 +34,11 @@
  *                                gate or norm after the block, and no backward pass)
  *   gdn_fp8_quantize_hip,     <- no reference counterpart (8-bit projections)
  *   gdn_fp8_matmul_hip
+ *   gdn_fp4_quantize_hip,     <- no reference counterpart (4-bit weights)
+ *   gdn_fp4_dequantize_hip,
+ *   gdn_fp4_matmul_hip
+ *   gdn_grad_norm_hip,        <- no reference counterpart (the reference does not train)
+ *   gdn_clip_grad_norm_hip
  */
 #ifndef GDN_AMD_H
 #define GDN_AMD_H
@@ -359,9 +364,9 @@ int gdn_layer_decode_step_hip(const gdn_bf16_t* x, const gdn_bf16_t* gamma, floa
                               gdn_bf16_t* k, gdn_bf16_t* v, gdn_bf16_t* a, gdn_bf16_t* b, float* o, gdn_bf16_t* y,
                               int B, int D, int H, int dk, int dv, int conv_k, void* stream);
 
-/* Element types, 8-bit formats (e4m3: largest 448; e5m2: largest 57344) and gate activations. */
+/* Element types, 8-bit (e4m3: largest 448; e5m2: largest 57344) and 4-bit (e2m1: largest 6) formats, and gate activations. */
 enum { GDN_BF16 = 0, GDN_F32 = 1, GDN_E8M0 = 2 };
-enum { GDN_E4M3 = 0, GDN_E5M2 = 1 };
+enum { GDN_E4M3 = 0, GDN_E5M2 = 1, GDN_E2M1 = 2 };
 enum { GDN_ACT_NONE = 0, GDN_ACT_SIGMOID = 1, GDN_ACT_SILU = 2, GDN_ACT_TANH = 3 };
 
 /*
@@ -456,6 +461,81 @@ int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_
                        const uint8_t* b, int64_t ldb, int format_b, const void* b_scale, int64_t ldb_s, int b_block_rows,
                        int type_b_scale, void* out, int64_t ldo, int type_out, int64_t M, int64_t N, int64_t K,
                        void* stream);
+
+/*
+ * x [M, K] (bf16 or fp32, rows ldx elements apart) to 4-bit floating point (e2m1),
+ * one power-of-two scale a block of block_rows (1 or 32) x 32 values: 2^e with the
+ * least e >= -127 for which the block's largest magnitude over 2^e is no larger than
+ * 6 (e = 0 for zeros), kept as the byte e + 127 (e8m0); a code is value / 2^e to the
+ * nearest, ties to even.  A block with an infinity or NaN gets scale NaN (0xff), codes
+ * 0.  Along the rows: codes [M, ldc bytes], two a byte, the earlier one low, columns K
+ * up to the next multiple of 256 zero; scales [K / 128, lds >= M, 4], blocks of 128
+ * columns first (as many as the codes have), a row's four bytes adjacent.  Along the
+ * columns, the same of x^T: codes_t [K, ldt bytes], columns M up to the next multiple
+ * of 256 zero; scales_t [M / 128, ldst >= K, 4].  Either pair may be NULL.  Code rows
+ * 16-byte aligned.  What lies behind these in wider buffers is left as it is.
+ */
+int gdn_fp4_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, int block_rows, uint8_t* codes,
+                         int64_t ldc, uint8_t* scales, int64_t lds, uint8_t* codes_t, int64_t ldt, uint8_t* scales_t,
+                         int64_t ldst, void* stream);
+
+/*
+ * What e2m1 codes [M, ldc bytes] with scales [K / 128, lds >= M, 4] stand for: out [M,
+ * ldo] bf16 or fp32 (type_out), exactly; what lies beyond bf16's range is infinite,
+ * a scale of 0xff NaN.  Any K, codes at 4 bytes.
+ */
+int gdn_fp4_dequantize_hip(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, void* out, int64_t ldo,
+                           int type_out, int64_t M, int64_t K, void* stream);
+
+/*
+ * Product with 4-bit weights:
+ *   out[m, n] = sum_k a[m, k] a_scale[m, block of k] b[n, k] b_scale[n, block of k]
+ * out [M, ldo] bf16 or fp32 (type_out), rounded once from fp32 sums.
+ *   b [N, ldb bytes] e2m1 codes in rows of whole 256 values (zero codes behind K),
+ *   b_scale e8m0 [K / 128 (an even number), ldb_s >= N, 4]: a scale a row and 32;
+ *   a (format_a): GDN_E2M1, the same with a_scale [K / 128, lda_s >= M, 4], K % 256 ==
+ *   0; or GDN_E4M3, GDN_E5M2 codes [M, lda] with a scale a row and 128, a_scale e8m0
+ *   [K / 128, lda_s >= M], K % 128 == 0 (as gdn_block_norm_hip and
+ *   gdn_fp8_quantize_hip write them).
+ * Code rows are 16-byte aligned and at most 2^22 bytes apart.  Scales: 16-byte aligned
+ * rows of K's blocks, ld % 4 == 0 (of 8-bit codes % 16), readable in whole.  M, N up to
+ * 2^28.  With 8-bit codes, bf16 results leave 128 products to one instruction, which
+ * drops what lies below 2^-17 of the largest; fp32 results sum every product in full.
+ * Scales may be anything that the type holds; only the product of the two (of a row and
+ * a column, in each block) has to be in fp32's range.  A row's sums do not depend on
+ * other rows' values; their order follows M, N, K and the column.
+ */
+int gdn_fp4_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_t* a_scale, int64_t lda_s,
+                       const uint8_t* b, int64_t ldb, const uint8_t* b_scale, int64_t ldb_s, void* out, int64_t ldo,
+                       int type_out, int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * The 2-norm of `count` tensors together (a HOST array of device pointers; each n
+ * adjacent elements, bf16 or fp32), norm [1] = sqrt(sum of squares), with sums in 64
+ * bits in a fixed order.  Elements count as often as they are given.  type_out and out
+ * are not read.  No tensors: 0.  workspace: gdn_grad_norm_workspace_bytes(count), 8-byte
+ * aligned.
+ */
+typedef struct {
+    const void* grad;
+    void* out;
+    int64_t n;
+    int type, type_out;
+} gdn_grad_t;
+
+size_t gdn_grad_norm_workspace_bytes(int64_t count);
+
+int gdn_grad_norm_hip(const gdn_grad_t* grads, int64_t count, float* norm, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
+ * The same, and out = grad min(1, max_norm / (norm + 1e-6)) for each tensor, rounded
+ * once to type_out; out may be grad itself (then of its type; not written where the
+ * factor is 1) and lies apart from the other tensors, or the call is refused.  A norm
+ * that is NaN makes every result NaN, an infinite one zeros and NaN.  max_norm >= 0.
+ */
+int gdn_clip_grad_norm_hip(const gdn_grad_t* grads, int64_t count, double max_norm, float* norm, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,218 @@
+"""Refusals of the 4-bit quantisation, product and the gradients' norm: every bad call
+is turned down on the host, before any HIP call (none runs here).  And what the 4-bit
+kernels' counted waits rest on, in their assembly."""
+
+import ctypes
+import re
+
+import pytest
+import torch
+
+from gdn_18646_amd import abi, blocks, compile_kernels, native_extension
+from gdn_18646_amd.abi import GdnError, GradTensor
+from tests.fp4 import nearest, pack, quantize64, unpack, values
+from tests.test_isa_cpu import _assembly, _events, _function
+
+FAKE = 4096  # non-null, aligned; never dereferenced
+BF, F32, E8 = 0, 1, 2
+E4M3, E2M1 = 0, 2
+
+
+def _quant(**k):
+    a = dict(x=FAKE, ldx=300, type=BF, M=200, K=300, block=1, codes=FAKE, ldc=256, scales=FAKE, lds=200, codes_t=FAKE, ldt=128, scales_t=FAKE, ldst=300,
+             stream=None)
+    assert set(k) <= set(a)
+    a.update(k)
+    abi.call("gdn_fp4_quantize_hip", *a.values())
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(M=-1), "INVALID_ARGUMENT"), (dict(block=128), "UNSUPPORTED.*128 x 32"), (dict(type=2), "type 2"), (dict(M=1 << 31), "too large"),
+    (dict(K=1 << 31), "too large"), (dict(codes=None, codes_t=None), "no output"), (dict(x=None), "null"), (dict(ldx=299), "ldx"), (dict(x=FAKE + 1), "unaligned"),
+    (dict(ldc=240), "codes"), (dict(ldc=264), "codes"), (dict(lds=199), "codes"), (dict(scales=None), "codes"), (dict(codes=FAKE + 8), "codes"),
+    (dict(scales=FAKE + 2), "codes"), (dict(ldt=112), "codes_t"), (dict(ldst=299), "codes_t"), (dict(scales_t=None), "codes_t")])
+def test_quantize_refusals(bad, match):
+    with pytest.raises(GdnError, match=match):
+        _quant(**bad)
+
+
+def _dequant(**k):
+    a = dict(codes=FAKE, ldc=152, scales=FAKE, lds=200, out=FAKE, ldo=300, to=BF, M=200, K=300, stream=None)
+    assert set(k) <= set(a)
+    a.update(k)
+    abi.call("gdn_fp4_dequantize_hip", *a.values())
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(M=-1), "INVALID_ARGUMENT"), (dict(to=E8), "type 2"), (dict(M=1 << 31), "too large"), (dict(codes=None), "codes"), (dict(codes=FAKE + 2), "codes"),
+    (dict(ldc=148), "codes"), (dict(ldc=154), "codes"), (dict(scales=None), "scales"), (dict(lds=199), "scales"), (dict(out=None), "out"),
+    (dict(out=FAKE + 1), "out"), (dict(ldo=299), "out")])
+def test_dequantize_refusals(bad, match):
+    with pytest.raises(GdnError, match=match):
+        _dequant(**bad)
+
+
+def _mm(**k):
+    a = dict(a=FAKE, lda=256, fa=E2M1, sa=FAKE, ldas=48, b=FAKE, ldb=256, sb=FAKE, ldbs=112, out=FAKE, ldo=100, to=BF, M=40, N=100, K=512, stream=None)
+    assert set(k) <= set(a)
+    a.update(k)
+    abi.call("gdn_fp4_matmul_hip", *a.values())
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(M=-1), "INVALID_ARGUMENT"), (dict(K=0), "INVALID_ARGUMENT"), (dict(K=384), "multiple of 256"), (dict(fa=E4M3, K=200), "multiple of 128"),
+    (dict(fa=3), "format 3"), (dict(to=E8), "type 2 of out"), (dict(lda=1 << 23), "too large"), (dict(M=1 << 29), "too large"), (dict(N=1 << 29), "too large"),
+    (dict(ldbs=1 << 30), "too large"), (dict(a=None), "null"), (dict(sb=None), "null"), (dict(out=None), "null"), (dict(a=FAKE + 8), "16-byte"),
+    (dict(ldb=240), "16-byte"), (dict(ldb=264), "16-byte"), (dict(fa=E4M3), "16-byte"), (dict(ldas=36), "a's scales"), (dict(ldas=42), "a's scales"),
+    (dict(sa=FAKE + 4), "a's scales"), (dict(fa=E4M3, lda=512, ldas=40), "a's scales"), (dict(ldbs=96), "b's scales"), (dict(ldbs=102), "b's scales"),
+    (dict(sb=FAKE + 8), "b's scales"), (dict(ldo=99), "ldo"), (dict(out=FAKE + 1), "unaligned"), (dict(fa=E4M3, K=384, lda=384, ldb=128), "16-byte")])
+def test_product_refusals(bad, match):
+    with pytest.raises(GdnError, match=match):
+        _mm(**bad)
+
+
+def test_nothing_to_do_is_no_call():
+    _quant(M=0)
+    _quant(K=0)
+    _dequant(M=0)
+    _dequant(K=0)
+    _mm(M=0)
+    _mm(N=0)
+
+
+def _grads(entry, tensors, most=1.0, norm=FAKE, ws=FAKE, size=1 << 24, count=None):
+    a = (GradTensor * max(len(tensors), 1))(*[GradTensor(*t) for t in tensors])
+    clip = [most] if "clip" in entry else []
+    abi.call(entry, ctypes.addressof(a), len(tensors) if count is None else count, *clip, norm, ws, size, None)
+
+
+A, B = 1 << 20, 1 << 24
+
+
+@pytest.mark.parametrize("tensors,kw,match", [
+    ([(A, A, 10, F32, F32)], dict(count=-1), "INVALID_ARGUMENT.*-1 tensors"), ([(A, A, 10, F32, F32)], dict(norm=None), "null"),
+    ([(A, A, 10, F32, F32)], dict(ws=None), "WORKSPACE"), ([(A, A, 10, F32, F32)], dict(size=16), "WORKSPACE"), ([(A, A, 10, F32, F32)], dict(ws=FAKE + 4), "WORKSPACE"),
+    ([(A, A, 10, 2, F32)], {}, "UNSUPPORTED.*type"), ([(A, A, -1, F32, F32)], {}, "elements"), ([(A, A, 1 << 60, F32, F32)], {}, "elements"),
+    ([(None, A, 10, F32, F32)], {}, "null or unaligned"), ([(A + 2, A, 10, F32, F32)], {}, "null or unaligned"), ([(A + 1, A, 10, BF, F32)], {}, "null or unaligned")])
+@pytest.mark.parametrize("entry", ["gdn_grad_norm_hip", "gdn_clip_grad_norm_hip"])
+def test_grad_refusals(entry, tensors, kw, match):
+    with pytest.raises(GdnError, match=match):
+        _grads(entry, tensors, **kw)
+
+
+@pytest.mark.parametrize("tensors,kw,match", [
+    ([(A, A, 10, F32, F32)], dict(most=-1.0), "max_norm"), ([(A, A, 10, F32, F32)], dict(most=float("nan")), "max_norm"),
+    ([(A, A, 10, F32, 2)], {}, "UNSUPPORTED.*type"), ([(A, None, 10, F32, F32)], {}, "null or unaligned"),
+    ([(A, A, 10, F32, BF)], {}, "lies over"),                                            # in place, of another type
+    ([(A, A + 4, 10, F32, F32)], {}, "lies over"), ([(A + 4, A, 10, F32, F32)], {}, "lies over"),  # an element on
+    ([(A, A, 10, F32, F32), (A, A, 10, F32, F32)], {}, "share memory"), ([(A, A, 10, F32, F32), (A + 36, A + 36, 10, F32, F32)], {}, "share memory"),
+    ([(A, A, 1000, F32, F32), (A + 400, B, 10, F32, F32)], {}, "lies over"), ([(A, B, 10, F32, F32), (B + 39 - 3, A - 4000, 10, F32, F32)], {}, "lies over"),
+    ([(A, B + 10000, 10, F32, F32), (A, B, 10, BF, F32), (B + 4, B - 10000, 10, BF, BF)], {}, "lies over")])
+def test_clip_refuses_results_over_what_others_read(tensors, kw, match):
+    with pytest.raises(GdnError, match=match):
+        _grads("gdn_clip_grad_norm_hip", tensors, **kw)
+
+
+def test_workspace_of_the_norm():
+    f = abi.load().gdn_grad_norm_workspace_bytes
+    assert f(0) == 8 and f(1) == f(128) == 2049 * 8 and f(129) == 4097 * 8 and f(-1) == 0
+
+
+def test_binding_refusals_on_the_host():
+    p, t = compile_kernels()["proj"], torch.zeros(4, 256, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        p.fp4_quantize(t)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        p.fp4_dequantize(t, t)
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        p.fp4_matmul(t, t, t, t)
+    grads = native_extension().grads
+    for call in (lambda: grads.norm([t]), lambda: grads.clip([t], 1.0)):
+        with pytest.raises(RuntimeError, match="GPU tensor"):
+            call()
+    with pytest.raises(RuntimeError, match="no tensors"):
+        grads.norm([])
+
+
+def test_layers_check_their_arguments():
+    x, w = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(8, 256, dtype=torch.bfloat16)
+    for args, match in (((x, w[:, :128]), "weight"), ((x, w[0]), "weight"), ((x[0, 0], w), "weight"), ((x, w, torch.bfloat16), "activations")):
+        with pytest.raises(ValueError, match=match):
+            blocks.fp4_linear(*args)
+    with pytest.raises(ValueError, match="weight"):
+        blocks.Fp4Weight(w[0])
+    assert blocks.grad_norm([]).item() == 0 and blocks.clip_grad_norm([None], 1.0).item() == 0
+
+
+def test_the_definition_that_the_kernels_are_held_to():
+    """Every value between two codes goes to the nearer one, ties to the even code."""
+    v = torch.arange(-96, 97, dtype=torch.float64) / 16
+    c = nearest(v)
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+    got = torch.where(c > 7, -1.0, 1.0) * table[(c & 7).long()]
+    step = torch.where(v.abs() >= 4, 2.0, torch.where(v.abs() >= 2, 1.0, 0.5))
+    assert torch.equal(got, torch.round(v / step) * step)
+    x = torch.randn(3, 70, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    codes, scales = quantize64(x, 1)
+    assert torch.equal(unpack(pack(codes)), codes)
+    big = x[:, :64].view(3, 2, 32).abs().amax(2)
+    s = torch.ldexp(torch.ones(3, 8, dtype=torch.float64), scales.int() - 127)
+    assert (big <= 6 * s[:, :2]).all() and (big > 3 * s[:, :2]).all() and (scales[:, 3:] == 127).all()
+    assert ((values(codes, scales)[:, :70] - x).abs() <= s.repeat_interleave(32, 1)[:, :70]).all()
+
+
+# ---------------------------------------------------------------------------
+# Assembly
+# ---------------------------------------------------------------------------
+# columns: staged rows of a token, waves along columns, tokens, MFMA tiles of a wave along each, stages
+PHASED = {"e2m1 256x256": (1, 4, 2, 4, 8, 2), "e2m1 256x192": (1, 4, 2, 4, 6, 2), "e2m1 256x160": (1, 4, 2, 4, 5, 2), "e2m1 256x128": (1, 4, 2, 4, 4, 3),
+          "e2m1 128x192": (1, 2, 4, 4, 3, 3), "e4m3 256x160": (2, 4, 2, 4, 5, 2), "e4m3 256x128": (2, 4, 2, 4, 4, 2), "e4m3 128x192": (2, 2, 4, 4, 3, 2)}
+
+
+@pytest.fixture(scope="module")
+def asm(tmp_path_factory):
+    return {f: _assembly(f"fp4_mm_{f}.hip", tmp_path_factory) for f in ("e2m1", "e4m3")}
+
+
+def _kernels(text, tile=""):
+    return re.findall(rf"^(_Z\w*gdn_fp4_matmul_kernel\w*Fp4TileI{tile}\w*):", text, re.M)
+
+
+def test_no_tile_spills(asm):
+    assert len(_kernels(asm["e2m1"])) == 2 * 12 and len(_kernels(asm["e4m3"])) == 10 + 7
+    for text in asm.values():
+        for name in _kernels(text):
+            assert not any("scratch_" in ln for ln in _function(text, name)), name
+
+
+@pytest.mark.parametrize("tile", PHASED)
+def test_phased_tiles_keep_their_counted_waits(asm, tile):
+    """A stage's LDS buffer is refilled region by region; the waits before the barriers that
+    open a phase count the copies issued after the region that the next phase reads, which
+    holds only for these copies in this order: none moved over a wait, merged or dropped."""
+    xh, cw, tw, wmt, wnt, ns = PHASED[tile]
+    m0, x0 = wmt // 2, (wnt + 1) // 2
+    groups = [2 * xh * tw * x0, 2 * cw * m0, 2 * cw * (wmt - m0), 2 * xh * tw * (wnt - x0)]  # X0, W0, W1, X1: 8-row copies, split over 8 waves
+    n = [g // 8 + g % 8 // 4 for g in groups]
+    n[0] += 2  # the scales of both operands
+    every = sum(n)
+    text = asm[tile.split()[0]]
+    names = _kernels(text, "".join(f"Li{v}E" for v in (xh, cw, tw, wmt, wnt, ns)))
+    assert len(names) == (2 if xh == 1 else 1), names  # bf16 and fp32 results
+    for name in names:
+        events = _events(_function(text, name))
+
+        def found(want):
+            return any(events[i:i + len(want)] == want for i in range(len(events)))
+
+        # a stage of the loop, from any of its phases on
+        stage = (["c"] * n[3] + [n[3] + (ns - 1) * every, "b", "b"] + ["c"] * n[0] + [n[0] + (ns - 1) * every, "b", "b"]
+                 + ["c"] * n[1] + ["b", "b"] + ["c"] * n[2] + [n[2] + (ns - 1) * every, "b", "b"])
+        assert any(found(stage[i:] + stage[:i]) for i in range(len(stage)))
+        # the stages after the last issued one, t of them left
+        for t in range(ns):
+            tail = [n[3] + t * every, "b", "b", t * every, "b", "b", "b", "b"]
+            tail += [n[2] + n[3] + (t - 1) * every, "b"] if t else []
+            assert found((["c"] * n[3] if t == ns - 1 else []) + tail), t
+        # the ring is filled (all but X1 of its last stage) before a tile's first stage waits for X0, the scales and W0
+        assert n[2] + (ns - 1) * every in events[events.index("c"):]

@@ -1,0 +1,411 @@
+"""4-bit quantisation, its inverse and the product with 4-bit weights on the GPU
+against their definitions.
+
+Quantisation has one answer and so has its inverse: both are compared bit for bit.
+
+The product.  4-bit codes on both sides: an instruction adds 128 products and the
+accumulator with an error of at most 2^-21 of the largest of them, none of which is
+larger than the sum of the terms' magnitudes; K / 128 instructions and at most eight
+partial sums make (K / 128 + 8) 2^-21 of it.  8-bit codes, fp32 results: every
+product is exact in fp32 (4 by 2 bits) and so are the powers of two, so the result is
+off by the half steps of its K + K / 128 + 8 additions, 2^-24 each.  8-bit codes, bf16
+results: the instruction drops 2^-17 of the largest product for each of 128, 2^-10 of
+it a block.  A bf16 result adds half its own step, 2^-8.
+"""
+
+import pytest
+import torch
+
+from gdn_18646_amd import abi
+from tests.fp4 import E2, E4, E5, E8, pack, quantize64, unpack, up, values, words
+
+pytestmark = pytest.mark.gpu
+
+SPECIAL = torch.tensor([0.0, -0.0, 6.0, 6.1, 0.25, -0.75, 2.5, 5.0, 1e-38, 1e-40, 3e38, -3e38, 1.0, 2.0 ** -126, 2.0 ** -133])
+
+
+def _bits(t):
+    return t.view(torch.uint8).cpu()
+
+
+def _compare(codes, scales, x, rows):
+    rc, rs = quantize64(x, rows)
+    assert codes.dtype == E2 and scales.dtype == E8 and scales.shape == (x.shape[0], up(x.shape[1], 256) // 128, 4)
+    assert torch.equal(_bits(scales).reshape(x.shape[0], -1), rs)
+    got = unpack(codes)
+    assert got.shape == rc.shape
+    same = (got == rc) | ((got & 7 == 0) & (rc & 7 == 0))  # the sign of an underflowed zero is free
+    assert same.all(), (got[~same][:5], rc[~same][:5])
+
+
+@pytest.mark.parametrize("block", [1, 32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 16), (1, 2048), (3, 130), (77, 1000), (128, 128), (129, 384), (300, 513), (260, 8), (33, 31)])
+def test_quantize(exts, dev, M, K, dtype, block):
+    g = torch.Generator().manual_seed(M * K)
+    x = (torch.randn(M, K, generator=g) * torch.exp(3 * torch.randn(M, 1, generator=g))).to(dtype)
+    n = min(len(SPECIAL), M * K)
+    x.view(-1)[torch.randint(0, M * K, (n,), generator=g)] = SPECIAL[:n].to(dtype)
+    if M > 2:
+        x[1] = 0
+    q = exts["proj"].fp4_quantize(x.to(dev), block_rows=block, rows=True, columns=True)
+    _compare(*q[:2], x, block)
+    _compare(*q[2:], x.t(), block)
+    for kw, pair in ((dict(rows=True), q[:2]), (dict(rows=False, columns=True), q[2:])):  # each alone gives the same
+        alone = exts["proj"].fp4_quantize(x.to(dev), block_rows=block, **kw)
+        assert len(alone) == 2 and all(torch.equal(_bits(a), _bits(b)) for a, b in zip(alone, pair))
+    if block == 32:  # the same values both ways
+        rows, columns = (exts["proj"].fp4_dequantize(*p, columns=c, dtype=torch.float32) for p, c in ((q[:2], K), (q[2:], M)))
+        assert torch.equal(rows, columns.t())
+
+
+@pytest.mark.parametrize("K", [*range(2, 10), *range(25, 40), *range(249, 265)])
+def test_quantize_every_remainder_of_columns(exts, dev, K):
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(5, K, generator=torch.Generator().manual_seed(K)).to(dtype)
+        q = exts["proj"].fp4_quantize(x.to(dev), rows=True, columns=True)
+        _compare(*q[:2], x, 1)
+        _compare(*q[2:], x.t(), 1)
+
+
+def test_every_tie_rounds_to_the_even_code(exts, dev):
+    x = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, 0.0]).repeat(1, 2)
+    codes, _ = exts["proj"].fp4_quantize(x.to(dev))
+    assert unpack(codes)[0, :16].tolist() == [7, 0, 2, 2, 4, 4, 6, 6, 8, 10, 10, 12, 12, 14, 14, 0]
+
+
+@pytest.mark.parametrize("block", [1, 32])
+def test_quantize_not_finite(exts, dev, block):
+    x = torch.randn(200, 300, generator=torch.Generator().manual_seed(1))
+    x[5, 7], x[150, 290], x[40, 40] = float("nan"), float("-inf"), float("inf")
+    q = exts["proj"].fp4_quantize(x.to(dev), block_rows=block, rows=True, columns=True)
+    for pair, t in ((q[:2], x), (q[2:], x.t())):
+        _compare(*pair, t, block)
+        v = exts["proj"].fp4_dequantize(*pair, columns=t.shape[1], dtype=torch.float32).cpu()
+        rc, rs = quantize64(t, block)
+        assert torch.equal(v.isnan(), (rs == 255).repeat_interleave(32, 1)[:, :t.shape[1]])
+
+
+def test_quantize_strided_rows(exts, dev):
+    wide = torch.randn(90, 700, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(dev)
+    for lo, hi in ((64, 320), (3, 290), (64, 321)):
+        a = exts["proj"].fp4_quantize(wide[:, lo:hi], rows=True, columns=True)
+        b = exts["proj"].fp4_quantize(wide[:, lo:hi].contiguous(), rows=True, columns=True)
+        assert all(torch.equal(_bits(x), _bits(y)) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("block", [1, 32])
+@pytest.mark.parametrize("M,K", [(1, 200), (97, 130), (126, 300), (130, 257)])
+def test_quantize_leaves_what_lies_behind(dev, M, K, block):
+    """Through the C ABI, into buffers that are wider and longer than the results."""
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(torch.bfloat16).to(dev)
+    Mp, Kp = up(M, 256), up(K, 256)
+    ldc, ldt, lds, ldst = Kp // 2 + 32, Mp // 2 + 48, M + 7, K + 5
+    codes, scales, codes_t, scales_t = (torch.full(s, 0x55, dtype=torch.uint8, device=dev)
+                                        for s in ((M + 2, ldc), (Kp // 128 + 1, lds, 4), (K + 2, ldt), (Mp // 128 + 1, ldst, 4)))
+    abi.call("gdn_fp4_quantize_hip", x.data_ptr(), K, 0, M, K, block, codes.data_ptr(), ldc, scales.data_ptr(), lds,
+             codes_t.data_ptr(), ldt, scales_t.data_ptr(), ldst, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for got_c, got_s, t in ((codes, scales, x.cpu()), (codes_t, scales_t, x.t().cpu())):
+        rc, rs = quantize64(t, block)
+        m, k = rc.shape
+        keep_c, keep_s = got_c.cpu(), got_s.cpu()
+        assert (keep_c[m:] == 0x55).all() and (keep_c[:, k // 2:] == 0x55).all()
+        assert (keep_s[k // 128:] == 0x55).all() and (keep_s[:, m:] == 0x55).all()
+        c = unpack(keep_c[:m, :k // 2].contiguous())
+        assert ((c == rc) | ((c & 7 == 0) & (rc & 7 == 0))).all()
+        assert torch.equal(keep_s[:k // 128, :m].transpose(0, 1).reshape(m, -1), rs)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,K", [(1, 256), (3, 256), (16, 512), (70, 2048)])
+def test_dequantize(exts, dev, M, K, dtype):
+    """Every code with every scale; bf16's and fp32's largest numbers are the same, give or take a rounding."""
+    g = torch.Generator().manual_seed(M)
+    codes = torch.randint(0, 16, (M, K), generator=g)
+    scales = torch.randint(0, 256, (M, K // 32), generator=g).to(torch.uint8)
+    want = values(codes, scales).float()
+    c, s = pack(codes).to(dev), scales.view(E8).to(dev)
+    for n in (K, K - 1, 37, 8, 1, 0):
+        for layout in (s, words(s), s.view(M, -1, 4)):
+            got = exts["proj"].fp4_dequantize(c, layout, columns=n, dtype=dtype)
+            assert got.dtype == dtype and got.shape == (M, n)
+            torch.testing.assert_close(got.float().cpu(), want[:, :n], rtol=0, atol=0, equal_nan=True)
+    wide = torch.zeros(M, K, dtype=torch.uint8, device=dev)
+    wide[:, 20:20 + K // 2] = c.view(torch.uint8)
+    assert torch.equal(_bits(exts["proj"].fp4_dequantize(wide.view(E2)[:, 20:20 + K // 2], s, dtype=dtype)), _bits(exts["proj"].fp4_dequantize(c, s, dtype=dtype)))
+
+
+# ---------------------------------------------------------------------------
+# The product
+# ---------------------------------------------------------------------------
+TOP = {E4: 448.0, E5: 57344.0}
+
+
+class Side:
+    """Codes and scales of an operand, on the CPU and on the GPU, and its values in 64 bits."""
+
+    def __init__(self, rows, K, fmt, g, dev, lo=115, hi=140):
+        self.fmt, self.K = fmt, K
+        if fmt == E2:
+            kp = up(K, 256)
+            codes = torch.randint(0, 16, (rows, kp), generator=g)
+            codes[:, K:] = 0
+            scales = torch.randint(lo, hi, (rows, kp // 32), generator=g).to(torch.uint8)
+            self.codes, self.scales = pack(codes).to(dev), words(scales.view(E8).to(dev))
+            self.values = values(codes, scales)[:, :K].to(dev)
+        else:
+            self.codes = (torch.randn(rows, K, generator=g) * (100 if fmt == E4 else 3000)).clamp(-TOP[fmt], TOP[fmt]).to(fmt).to(dev)
+            scales = torch.randint(lo, hi, (rows, K // 128), generator=g).to(torch.uint8)
+            self.scales = scales.view(E8).to(dev)
+            self.values = self.codes.double() * self.scales.double().repeat_interleave(128, 1)
+
+    def top(self):
+        return self.values.abs().view(self.values.shape[0], -1, 128).amax(2)
+
+
+def _operands(M, N, K, fa, dev, seed=0, **kw):
+    g = torch.Generator().manual_seed(seed + M + 31 * N + 7 * K)
+    return Side(M, K, fa, g, dev, **kw), Side(N, K, E2, g, dev, **kw)
+
+
+def _check(y, a, b):
+    ref, mag, K = a.values @ b.values.t(), a.values.abs() @ b.values.abs().t(), a.K
+    if a.fmt == E2:
+        tol = (K / 128 + 8) * 2.0 ** -21 * mag
+    else:
+        tol = (K + K / 128 + 8) * 2.0 ** -24 * mag
+        if y.dtype == torch.bfloat16:
+            tol = tol + 2.0 ** -10 * a.top() @ b.top().t()
+    if y.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (ref.abs() + tol)
+    far = (y.double() - ref).abs() - tol
+    assert y.shape == ref.shape and not (far > 0).any() and torch.isfinite(y).all(), f"{(far > 0).sum().item()} values, the worst {far.max().item():.3g} past its bound"
+
+
+def _product(exts, a, b, out=torch.bfloat16):
+    y = exts["proj"].fp4_matmul(a.codes, a.scales, b.codes, b.scales, out_dtype=out)
+    assert y.dtype == out
+    return y
+
+
+SIZES = [(1, 1, 256), (1, 2048, 2048), (2, 100, 512), (16, 129, 1280), (17, 40, 256), (33, 65, 256), (77, 300, 1280), (64, 64, 8448),
+         (130, 1040, 512), (300, 1030, 512), (513, 2100, 256), (1030, 2050, 512), (2500, 5003, 256), (5, 33, 8448), (3, 5000, 768),
+         (16, 4100, 768), (1, 8224, 2048), (48, 2048, 4096), (700, 1500, 768), (1500, 3100, 512), (2100, 450, 768), (2341, 200, 256)]
+
+
+@pytest.mark.parametrize("fa", [E2, E4, E5], ids=["e2m1", "e4m3", "e5m2"])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_product(exts, dev, M, N, K, fa):
+    a, b = _operands(M, N, K, fa, dev)
+    for out in (torch.float32, torch.bfloat16):
+        print(f"{M} x {N} x {K} {fa} {out}", flush=True)
+        _check(_product(exts, a, b, out), a, b)
+
+
+@pytest.mark.parametrize("fa", [E4, E5], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 128), (2, 300, 384), (3, 33, 128), (16, 129, 640), (70, 300, 1152), (130, 1040, 384), (300, 1030, 896),
+                                   (1030, 2050, 384), (2500, 5003, 128), (1500, 3100, 640), (2756, 1500, 128), (2092, 450, 384)])
+def test_product_over_half_a_row_of_codes(exts, dev, M, N, K, fa):
+    """8-bit codes of an odd number of blocks: the weight's last 128 codes are padding."""
+    a, b = _operands(M, N, K, fa, dev)
+    b.codes.view(torch.uint8)[:, K // 2:] = 0x77  # whatever it holds: there is nothing to multiply it with
+    for out in (torch.float32, torch.bfloat16):
+        print(f"{M} x {N} x {K} {fa} {out}", flush=True)
+        _check(_product(exts, a, b, out), a, b)
+
+
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+@pytest.mark.parametrize("M,N", [(2100, 4400), (4200, 4400), (300, 1030), (1300, 1300), (40, 700)])
+def test_product_long(exts, dev, M, N, fa):
+    a, b = _operands(M, N, 8448, fa, dev)
+    for out in (torch.float32, torch.bfloat16):
+        _check(_product(exts, a, b, out), a, b)
+
+
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+@pytest.mark.parametrize("M,N,K,out", [(4096, 4118, 256, torch.bfloat16), (3000, 1297, 512, torch.float32)])
+def test_product_in_two_launches(exts, dev, M, N, K, out, fa):
+    """A few columns past a multiple of 256 run on tiles of their own."""
+    a, b = _operands(M, N, K, fa, dev)
+    _check(_product(exts, a, b, out), a, b)
+
+
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+@pytest.mark.parametrize("M,N,K", [(2499, 4090, 256), (2600, 2040, 768), (2590, 4090, 256), (1594, 4090, 256), (2756, 1500, 256), (2092, 450, 256),
+                                   (2341, 200, 256), (2756, 130, 256), (1677, 130, 256)])
+def test_product_of_one_round_of_tiles(exts, dev, M, N, K, fa):
+    a, b = _operands(M, N, K, fa, dev)
+    for out in (torch.float32, torch.bfloat16):
+        _check(_product(exts, a, b, out), a, b)
+
+
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+@pytest.mark.parametrize("M,N,K", [(3, 200, 512), (150, 300, 256)])
+def test_product_strides_and_scale_layouts(exts, dev, M, N, K, fa):
+    """Codes in wider rows, scales in any layout: the same bits."""
+    a, b = _operands(M, N, K, fa, dev)
+    f = exts["proj"].fp4_matmul
+    want = f(a.codes, a.scales, b.codes, b.scales)
+    wide = lambda t, at: torch.nn.functional.pad(t.view(torch.uint8), (at, 48)).view(t.dtype)[:, at:at + t.shape[1]]  # noqa: E731
+    assert torch.equal(f(wide(a.codes, 16), a.scales, wide(b.codes, 64), b.scales), want)
+    assert torch.equal(f(a.codes, a.scales.contiguous(), b.codes, b.scales.contiguous()), want)
+    assert torch.equal(f(a.codes, a.scales, b.codes, b.scales.flatten(1)), want)
+    assert torch.equal(f(a.codes, a.scales, b.codes, wide(b.scales.flatten(1), 3)), want)
+    if fa == E2:
+        assert torch.equal(f(a.codes, a.scales.flatten(1), b.codes, b.scales), want)
+    assert torch.equal(f(a.codes[:, :a.codes.shape[1]], a.scales, b.codes[5:], b.scales[5:]), f(a.codes, a.scales, b.codes[5:].clone(), words(b.scales.flatten(1)[5:])))
+
+
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+@pytest.mark.parametrize("M", [1, 2, 40, 300])
+def test_product_of_nan(exts, dev, M, fa):
+    """NaN scales (and codes of 8 bits) reach exactly the outputs whose sums meet them."""
+    for out in (torch.bfloat16, torch.float32):
+        a, b = _operands(M, 300, 512, fa, dev)
+        clean = _product(exts, a, b, out)
+        want = torch.zeros(M, 300, dtype=torch.bool)
+        _bits_on = lambda s: s.view(torch.uint8)  # noqa: E731
+        _bits_on(a.scales)[M - 1, 1] = 255
+        _bits_on(b.scales)[17, 3, 2] = 255
+        want[M - 1], want[:, 17] = True, True
+        if fa == E4 and M > 1:
+            _bits_on(a.codes)[0, 200] = 0x7f
+            want[0] = True
+        y = _product(exts, a, b, out)
+        assert torch.equal(y.isnan().cpu(), want)
+        assert torch.equal(y[~want.to(dev)], clean[~want.to(dev)])
+
+
+def test_product_of_nothing(exts, dev):
+    a, b = _operands(4, 32, 256, E2, dev)
+    f = exts["proj"].fp4_matmul
+    assert f(a.codes[:0], a.scales[:0], b.codes, b.scales).shape == (0, 32)
+    assert f(a.codes, a.scales, b.codes[:0], b.scales[:0]).shape == (4, 0)
+    q = exts["proj"].fp4_quantize(torch.zeros(0, 300, dtype=torch.bfloat16, device=dev), rows=True, columns=True)
+    assert [tuple(t.shape) for t in q] == [(0, 256), (0, 4, 4), (300, 0), (300, 0, 4)]
+    assert exts["proj"].fp4_dequantize(q[0], q[1], columns=300).shape == (0, 300)
+
+
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+def test_rows_do_not_depend_on_their_neighbours(exts, dev, fa):
+    a, b = _operands(200, 300, 512, fa, dev)
+    for out in (torch.bfloat16, torch.float32):
+        want = _product(exts, a, b, out)
+        s = a.scales.clone()
+        s.view(torch.uint8)[100:] = 255
+        assert torch.equal(exts["proj"].fp4_matmul(a.codes, s, b.codes, b.scales, out_dtype=out)[:100], want[:100])
+        assert torch.equal(_product(exts, a, b, out), want)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("fa", [E2, E4, E5], ids=["e2m1", "e4m3", "e5m2"])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 2048), (2, 70, 2048), (16, 129, 2048), (40, 100, 2048), (70, 2048, 2048), (300, 1030, 2048),
+                                   (700, 2100, 2048), (1594, 4090, 512), (4100, 4090, 512)])
+def test_product_of_far_scales(exts, dev, M, N, K, fa, out):
+    """Scales far from 1 that one operand's and the other's bring back together."""
+    a, b = _operands(M, N, K, fa, dev)
+    g = torch.Generator().manual_seed(K)
+    mid = torch.linspace(6, 248, K // 128).round().int()
+    near = lambda rows, n, at: (at[None, :, None] + torch.randint(-4, 5, (rows, K // 128, n), generator=g)).clamp(0, 250).to(torch.uint8)  # noqa: E731
+    sa, sb = near(M, 4 if fa == E2 else 1, mid), near(N, 4, 254 - mid)
+    of = lambda s: torch.ldexp(torch.ones(s.shape, dtype=torch.float64), s.int() - 127).flatten(1)  # noqa: E731
+    old_a = a.scales.double().flatten(1)
+    a.values = a.values / old_a.repeat_interleave(K // old_a.shape[1], 1) * of(sa).to(dev).repeat_interleave(K // (sa[0].numel()), 1)
+    b.values = b.values / b.scales.double().flatten(1).repeat_interleave(32, 1)[:, :K] * of(sb).to(dev).repeat_interleave(32, 1)
+    a.scales = words(sa.flatten(1).view(E8).to(dev)) if fa == E2 else sa[:, :, 0].contiguous().view(E8).to(dev)
+    b.scales = words(sb.flatten(1).view(E8).to(dev))
+    _check(_product(exts, a, b, out), a, b)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 300, 512), (16, 129, 1152), (70, 2048, 512), (300, 1030, 512), (520, 4090, 384), (2600, 2040, 384)])
+def test_product_of_large_terms_that_cancel(exts, dev, M, N, K):
+    """In every block two products of 448 and 6 take each other away and the rest is small
+    beside them: bf16 results are within the bound of what the instruction drops, fp32
+    results have all of it."""
+    g = torch.Generator().manual_seed(M)
+    small = torch.tensor([-0.0625, -0.03125, 0.03125, 0.0625])
+    a, b = _operands(M, N, K, E4, dev)
+    va = small[torch.randint(0, 4, (M, K), generator=g)]
+    cb = torch.randint(0, 2, (N, b.codes.shape[1] * 2), generator=g)
+    for k in range(0, K, 128):
+        at = torch.randperm(32, generator=g)[:2] + k
+        va[:, at] = 448.0
+        cb[:, at[0]], cb[:, at[1]] = 7, 15
+    cb[:, K:] = 0
+    a.codes, b.codes = va.to(E4).to(dev), pack(cb).to(dev)
+    sb = b.scales.flatten(1).contiguous()
+    a.values = a.codes.double() * a.scales.double().repeat_interleave(128, 1)
+    b.values = values(cb, _bits(sb))[:, :K].to(dev)
+    for out in (torch.bfloat16, torch.float32):
+        _check(_product(exts, a, b, out), a, b)
+
+
+def test_quantised_operands_go_straight_in(exts, dev):
+    """The codes of block_norm, fp8_quantize and fp4_quantize as they come, K no multiple of 256."""
+    g = torch.Generator().manual_seed(8)
+    x, w = (torch.randn(n, 1100, generator=g).to(torch.bfloat16).to(dev) for n in (70, 330))
+    wc, ws = exts["proj"].fp4_quantize(w)
+    wv = exts["proj"].fp4_dequantize(wc, ws, columns=1100, dtype=torch.float32).double()
+    q8, q4 = exts["proj"].fp8_quantize(x), exts["proj"].fp4_quantize(x)
+    _, _, nc, ns = exts["rmsnorm"].block_norm(x, gamma=torch.ones(1100, dtype=torch.bfloat16, device=dev), quantize=True)
+    for codes, scales in (q8, q4, (nc, ns)):
+        if codes.dtype == E2:
+            v = exts["proj"].fp4_dequantize(codes, scales, columns=1100, dtype=torch.float32).double()
+        else:
+            v = (codes.double() * scales.double().repeat_interleave(128, 1))[:, :1100]
+        y = exts["proj"].fp4_matmul(codes, scales, wc, ws, out_dtype=torch.float32)
+        tol = (1280 + 18) * 2.0 ** -23 * (v.abs() @ wv.abs().t())  # either bound above, at K = 1280
+        assert ((y.double() - v @ wv.t()).abs() <= tol).all()
+
+
+def test_offsets_past_32_bits(exts, dev):
+    """A weight of more than 2^32 bytes of codes and results of more than 2^32 bytes."""
+    N, K, M = 600_000, 16384, 40
+    codes = torch.zeros(N, K // 2, dtype=torch.uint8, device=dev)
+    scales = torch.full((K // 128, up(N, 16), 4), 127, dtype=torch.uint8, device=dev)
+    rows = torch.tensor([0, 5, 262143, 262144, 524288, 524289, N - 1], device=dev)
+    g = torch.Generator().manual_seed(5)
+    some = torch.randint(0, 256, (len(rows), K // 2), generator=g).to(torch.uint8).to(dev)
+    codes[rows] = some
+    s = scales.view(E8)[:, :N].transpose(0, 1)
+    for M in (2, 40):
+        x = torch.randn(M, K, generator=g).to(torch.bfloat16).to(dev)
+        xc, xs = exts["proj"].fp4_quantize(x)
+        y = exts["proj"].fp4_matmul(xc, xs, codes.view(E2), s)
+        part = exts["proj"].fp4_matmul(xc, xs, some.view(E2), words(torch.full((len(rows), K // 32), 127, dtype=torch.uint8, device=dev).view(E8)),
+                                       out_dtype=torch.float32)
+        assert ((y[:, rows].float() - part).abs() <= 2.0 ** -7 * part.abs() + 2.0 ** -10).all()
+        rest = torch.ones(N, dtype=torch.bool, device=dev)
+        rest[rows] = False
+        assert (y[:, rest] == 0).all()
+    v = exts["proj"].fp4_dequantize(codes.view(E2)[-70000:], s[-70000:])  # 2.3 GB of results
+    want = exts["proj"].fp4_dequantize(some[-1:].view(E2), s[:1])
+    assert torch.equal(v[-1:], want)
+
+
+def test_on_another_stream_and_replayed(exts, dev):
+    x = torch.randn(130, 512, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(dev)
+    w = torch.randn(300, 512, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(dev)
+    wq, ws = exts["proj"].fp4_quantize(w, block_rows=32)
+
+    def f():
+        return exts["proj"].fp4_matmul(*exts["proj"].fp8_quantize(x), wq, ws), exts["proj"].fp4_matmul(*exts["proj"].fp4_quantize(x), wq, ws)
+
+    eager = f()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = f()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(there, eager))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = f()
+    for _ in range(3):
+        for t in y:
+            t.fill_(7.0)
+        graph.replay()
+        exts["proj"].fp4_matmul(*exts["proj"].fp8_quantize(w), wq, ws)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(y, eager))

@@ -1,0 +1,193 @@
+"""The norm of many gradients and their clipping, on the GPU against 64 bits.
+
+The squares are summed in 64 bits, so the norm has one rounding to 32 bits (2^-24) and
+some 2^-40 of the sums' own; a clipped value has the factor's rounding and its own:
+2^-24 and half its type's step.
+"""
+
+import math
+
+import pytest
+import torch
+
+from gdn_18646_amd import abi, native_extension
+from gdn_18646_amd.blocks import clip_grad_norm, grad_norm
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+HALF = {BF: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+def _norm64(grads):
+    return math.sqrt(math.fsum((g.double() ** 2).sum().item() for g in grads))
+
+
+def _check_norm(norm, grads):
+    ref = _norm64(grads)
+    assert norm.dtype == F32 and norm.shape == () and abs(norm.item() - ref) <= (2.0 ** -24 + 2.0 ** -40) * ref
+    return ref
+
+
+def _make(sizes, types, seed, dev):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=g) * 10.0 ** (i % 5 - 3)).to(types[i % len(types)]).to(dev) for i, s in enumerate(sizes)]
+
+
+SETS = {
+    "one": [(1,)], "short": [(n,) for n in range(1, 40)], "empty": [(0,), (3, 0), (5,), (0,)], "matrices": [(256, 2048), (2048,), (2048, 4)],
+    "odd": [(1001, 333), (16385,), (16383,), (32769,), (7, 3)], "many": [(37 + i % 50,) for i in range(700)],
+    "a table": [(100 + i,) for i in range(128)], "a table and one": [(100 + i,) for i in range(129)], "large": [(4099, 8209), (11,)],
+}
+
+
+@pytest.mark.parametrize("types", [(BF,), (F32,), (BF, F32)], ids=["bf16", "fp32", "mixed"])
+@pytest.mark.parametrize("name", SETS)
+def test_norm_and_clip(dev, name, types):
+    grads = _make(SETS[name], types, len(name), dev)
+    ref = _check_norm(grad_norm(grads), grads)
+    assert torch.equal(grad_norm(grads), grad_norm(grads))
+    for most in (0.0, 0.37 * ref, 2 * ref + 1, float("inf")):
+        f = min(1.0, most / (ref + 1e-6))
+        wide = [torch.full(g.shape, 7.0, dtype=F32, device=dev) for g in grads]
+        small = [torch.full(g.shape, 7.0, dtype=BF, device=dev) for g in grads]
+        here = [g.clone() for g in grads]
+        for out in (wide, small, None):
+            norm = clip_grad_norm(grads if out is not None else here, most, out=out)
+            _check_norm(norm, grads)
+            for g, o in zip(grads, out if out is not None else here):
+                want = g.double() * f
+                assert ((o.double() - want).abs() <= (HALF[o.dtype] + 2.0 ** -23) * want.abs() + 2.0 ** -149).all()
+                if f == 1.0 and o.dtype == g.dtype:
+                    assert torch.equal(o, g)
+
+
+def test_squares_that_32_bits_do_not_hold(dev):
+    for scale in (1e30, 1e-30, 3e38):
+        grads = [torch.full((1000,), scale, device=dev), torch.full((77,), -scale, dtype=BF, device=dev)]
+        if scale < 1e38:
+            _check_norm(grad_norm(grads), grads)
+        f = 1e-3 * scale / (_norm64(grads) + 1e-6)
+        clip_grad_norm(grads, 1e-3 * scale)
+        assert ((grads[0].double() - min(f, 1.0) * scale).abs() <= 2.0 ** -22 * scale).all()
+    assert grad_norm([torch.full((100,), 3e38, device=dev)]).item() == float("inf")  # the norm itself is past 32 bits
+
+
+def test_billions_of_equal_terms(dev):
+    """2^28 terms of one size: a 32-bit sum would stop growing."""
+    g = torch.full((1 << 28,), 1.0, dtype=BF, device=dev)
+    assert grad_norm([g, g]).item() == pytest.approx(math.sqrt(2.0 ** 29), rel=2.0 ** -24)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_not_finite(dev, bad):
+    for n, at in ((10, 9), (100_003, 100_002)):
+        grads = [torch.ones(n, device=dev), torch.ones(33, dtype=BF, device=dev)]
+        grads[0][at] = bad
+        norm = clip_grad_norm(grads, 1.0)
+        if math.isnan(bad):
+            assert norm.isnan() and grads[0].isnan().all() and grads[1].isnan().all()
+        else:
+            assert norm.item() == float("inf") and grads[0][at].isnan() and (grads[1] == 0).all() and (grads[0][:at] == 0).all()
+
+
+def test_orders_offsets_and_views(dev):
+    g = torch.Generator().manual_seed(4)
+    flat = torch.randn(100_000, generator=g).to(BF).to(dev)
+    grads = [flat[1:4001], flat[4001:14000].view(9999), flat[14001:14001 + 300 * 200].view(300, 200).t(), flat[80000:80000 + 2400].view(2, 30, 40).permute(2, 0, 1)]
+    before = flat.clone()
+    ref = _check_norm(grad_norm(grads), grads)
+    outs = [torch.empty_like(t, dtype=F32) for t in grads]
+    clip_grad_norm(grads, 0.5 * ref, out=outs)
+    for t, o in zip(grads, outs):
+        assert ((o.double() - 0.5 * t.double()).abs() <= 2.0 ** -22 * t.double().abs() + 1e-6 * t.double().abs() / ref).all()
+    clip_grad_norm(grads, 0.5 * ref)
+    keep = torch.ones(100_000, dtype=torch.bool, device=dev)
+    for lo, hi in ((1, 14000), (14001, 74001), (80000, 82400)):
+        keep[lo:hi] = False
+    assert torch.equal(flat[keep], before[keep])
+    assert torch.equal(flat[1:4001], outs[0].to(BF))
+
+
+def test_an_element_counts_as_often_as_it_is_given(dev):
+    t = torch.randn(5000, generator=torch.Generator().manual_seed(1)).to(dev)
+    _check_norm(grad_norm([t, t, t[:100]]), [t, t, t[:100]])
+
+
+def test_refusals(dev):
+    f = native_extension().grads
+    a, b = torch.ones(100, device=dev), torch.ones(100, device=dev)
+    for grads, out, match in (([a, a], None, "share memory"), ([a, a[50:]], None, "share memory"), ([a, b], [b, a], "lies over"),
+                              ([a, b], [torch.empty_like(a), a], "lies over"), ([a, b], [b[:50], b], "shape"), ([a], [a, b], "1 grads and 2 out"),
+                              ([a], [a.view(BF)[:100]], "lies over"), ([a[::2]], None, "gaps"), ([torch.ones(1, device=dev).expand(9)], None, "overlaps"),
+                              ([a.double()], None, "bfloat16 or float32"), ([a.cpu()], None, "GPU"), ([a, b.cpu()], None, "device"),
+                              ([torch.ones(3, 4, device=dev)], [torch.ones(4, 3, device=dev).t()], "order of axes")):
+        with pytest.raises(RuntimeError, match=match):
+            f.clip(grads, 0.5, out)
+    assert (a == 1).all() and (b == 1).all()
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(RuntimeError, match="max_norm"):
+            f.clip([a], bad)
+    leaf = torch.ones(5, device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError, match="requires grad"):
+        f.clip([leaf], 0.5)
+    with torch.no_grad():
+        f.clip([leaf], 0.5)
+    assert (leaf < 0.3).all()
+
+
+def test_clipping_counts_as_an_in_place_operation(dev):
+    w, g = torch.ones(8, device=dev, requires_grad=True), torch.ones(8, device=dev)
+    loss = (w * g).sum()
+    clip_grad_norm([g], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_streams_and_replays(dev):
+    grads = _make([(300, 200), (1001,), (64, 64)], (BF, F32), 5, dev)
+    outs = [torch.empty_like(g) for g in grads]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        norm = clip_grad_norm(grads, 0.5, out=outs)
+    torch.cuda.current_stream().wait_stream(side)
+    want_n, want = norm.clone(), [o.clone() for o in outs]
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = clip_grad_norm(grads, 0.5, out=outs)
+    with torch.cuda.graph(second):
+        other = grad_norm(grads[:1])
+    for i in range(3):
+        new = _make([(300, 200), (1001,), (64, 64)], (BF, F32), 5 + i, dev)
+        for g, n in zip(grads, new):
+            g.copy_(n)
+        for o in outs:
+            o.fill_(9.0)
+        graph.replay()
+        second.replay()
+        torch.cuda.synchronize()
+        eager = [torch.empty_like(g) for g in grads]
+        assert torch.equal(clip_grad_norm(grads, 0.5, out=eager), got) and torch.equal(grad_norm(grads[:1]), other)
+        assert all(torch.equal(a, b) for a, b in zip(eager, outs))
+        if i == 0:
+            assert torch.equal(got, want_n) and all(torch.equal(a, b) for a, b in zip(want, outs))
+
+
+def test_parameters_as_they_are_used(dev):
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Linear(64, 128), torch.nn.Linear(128, 8)).to(dev)
+    net(torch.randn(16, 64, device=dev)).square().sum().backward()
+    grads = [p.grad for p in net.parameters()]
+    want = [g.clone() for g in grads]
+    ref = _norm64(want)
+    _check_norm(clip_grad_norm(grads + [None], 1.0), want)
+    for g, w in zip(grads, want):
+        assert ((g.double() - w.double() / (ref + 1e-6)).abs() <= 2.0 ** -22 * w.double().abs() / ref).all()
+    assert grad_norm([]).item() == 0.0 and clip_grad_norm([None], 1.0).item() == 0.0
+
+
+def test_c_abi_of_no_tensors(dev):
+    norm, ws = torch.full((1,), 5.0, device=dev), torch.empty(64, dtype=torch.uint8, device=dev)
+    abi.call("gdn_grad_norm_hip", None, 0, norm.data_ptr(), ws.data_ptr(), 64, torch.cuda.current_stream().cuda_stream)
+    assert norm.item() == 0.0
