@@ -86,40 +86,37 @@ struct TileCost {
     int tile, cols, toks, per_cu;
     float c, a1, b1, a2, b2;  // per_cu above 1: alone (1) and with per_cu on each CU (2)
 };
+// Fitted to 320 products each, 3 to 8192 tokens, N 64 to 8224, K 256 to 8192, kernels
+// back to back on operands that the L2s do not hold: the tile that the fit picks takes
+// 1.016 times the best one's time on average (1.35 at most; 8-bit codes 1.010 and 1.12,
+// fp32 results of those 1.007 and 1.09).  Up to ten tiles were timed; those here are the
+// ones whose absence costs.
 constexpr TileCost kCost4[] = {
-    {gdn_fp4::k256x256, 256, 256, 1, 0.f, 6.75f, 1.135f, 0.f, 0.f},
-    {gdn_fp4::k256x192, 256, 192, 1, 0.f, 6.22f, 1.012f, 0.f, 0.f},
-    {gdn_fp4::k256x160, 256, 160, 1, 0.f, 5.75f, 0.904f, 0.f, 0.f},
-    {gdn_fp4::k256x128, 256, 128, 1, 0.f, 5.56f, 0.725f, 0.f, 0.f},
-    {gdn_fp4::k128x192, 128, 192, 1, 0.f, 4.78f, 0.688f, 0.f, 0.f},
-    {gdn_fp4::k128x128, 128, 128, 1, 0.f, 4.28f, 0.511f, 0.f, 0.f},
-    {gdn_fp4::k64x128, 64, 128, 1, 0.40f, 4.22f, 0.315f, 0.f, 0.f},
-    {gdn_fp4::k64x64, 64, 64, 1, 0.92f, 3.20f, 0.222f, 0.f, 0.f},
-    {gdn_fp4::k64x32, 64, 32, 1, 1.26f, 2.73f, 0.144f, 0.f, 0.f},
-    {gdn_fp4::k32x32, 32, 32, 1, 1.48f, 2.16f, 0.106f, 0.f, 0.f},
-    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.64f, 1.78f, 0.054f, 0.f, 0.f},
-    {gdn_fp4::k16x16, 16, 16, 3, 2.60f, 0.70f, 0.064f, 1.37f, 0.112f},
+    {gdn_fp4::k256x256, 256, 256, 1, 0.00f, 6.66f, 1.887f, 0.f, 0.f},
+    {gdn_fp4::k128x128, 128, 128, 2, 3.36f, 1.26f, 0.937f, 3.47f, 1.181f},
+    {gdn_fp4::k128x64, 128, 64, 2, 1.51f, 1.83f, 0.573f, 2.78f, 0.801f},
+    {gdn_fp4::k64x128, 64, 128, 1, 0.82f, 2.98f, 0.450f, 0.f, 0.f},
+    {gdn_fp4::k64x64, 64, 64, 1, 1.07f, 2.39f, 0.322f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 1.40f, 2.21f, 0.177f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.88f, 1.72f, 0.119f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.71f, 1.20f, 0.027f, 0.86f, 0.145f},
 };
-constexpr TileCost kCost8[] = {
-    {gdn_fp4::k256x160, 256, 160, 1, 0.f, 5.75f, 1.604f, 0.f, 0.f},
-    {gdn_fp4::k256x128, 256, 128, 1, 0.f, 5.56f, 1.325f, 0.f, 0.f},
-    {gdn_fp4::k128x192, 128, 192, 1, 0.f, 4.78f, 1.188f, 0.f, 0.f},
-    {gdn_fp4::k128x128, 128, 128, 1, 0.f, 4.28f, 0.911f, 0.f, 0.f},
-    {gdn_fp4::k64x128, 64, 128, 1, 0.40f, 4.22f, 0.615f, 0.f, 0.f},
-    {gdn_fp4::k64x64, 64, 64, 1, 0.92f, 3.20f, 0.402f, 0.f, 0.f},
-    {gdn_fp4::k64x32, 64, 32, 1, 1.26f, 2.73f, 0.244f, 0.f, 0.f},
-    {gdn_fp4::k32x32, 32, 32, 1, 1.48f, 2.16f, 0.166f, 0.f, 0.f},
-    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.64f, 1.78f, 0.084f, 0.f, 0.f},
-    {gdn_fp4::k16x16, 16, 16, 3, 2.60f, 0.70f, 0.104f, 1.37f, 0.172f},
+constexpr TileCost kCost8[] = {  // 8-bit codes of a, bf16 results
+    {gdn_fp4::k256x128, 256, 128, 1, 0.69f, 4.34f, 1.641f, 0.f, 0.f},
+    {gdn_fp4::k128x64, 128, 64, 2, 3.06f, 0.80f, 0.874f, 1.78f, 1.113f},
+    {gdn_fp4::k64x64, 64, 64, 1, 0.86f, 2.61f, 0.402f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 1.20f, 2.31f, 0.230f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.73f, 1.75f, 0.179f, 0.f, 0.f},
+    {gdn_fp4::k16x16Alone, 16, 16, 1, 2.29f, 1.41f, 0.062f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.56f, 1.20f, 0.067f, 0.91f, 0.194f},
 };
-constexpr TileCost kCost32[] = {
-    {gdn_fp4::k128x128, 128, 128, 1, 1.01f, 3.08f, 1.915f, 0.f, 0.f},
-    {gdn_fp4::k64x128, 64, 128, 1, 0.11f, 4.40f, 1.025f, 0.f, 0.f},
-    {gdn_fp4::k64x64, 64, 64, 1, 0.76f, 3.32f, 0.646f, 0.f, 0.f},
-    {gdn_fp4::k64x32, 64, 32, 1, 1.09f, 3.09f, 0.380f, 0.f, 0.f},
-    {gdn_fp4::k32x32, 32, 32, 1, 1.34f, 2.25f, 0.280f, 0.f, 0.f},
-    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.63f, 1.84f, 0.114f, 0.f, 0.f},
-    {gdn_fp4::k16x16, 16, 16, 3, 2.61f, 0.70f, 0.151f, 1.53f, 0.223f},
+constexpr TileCost kCost32[] = {  // the same, fp32 results
+    {gdn_fp4::k128x64, 128, 64, 2, 2.76f, 0.44f, 1.889f, 3.29f, 2.653f},
+    {gdn_fp4::k64x64, 64, 64, 1, 0.56f, 2.79f, 1.011f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 0.95f, 2.64f, 0.542f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.33f, 2.08f, 0.333f, 0.f, 0.f},
+    {gdn_fp4::k16x16Alone, 16, 16, 1, 1.80f, 1.83f, 0.116f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.64f, 0.97f, 0.120f, 1.04f, 0.278f},
 };
 
 struct Choice {

@@ -152,6 +152,12 @@ __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, lds_u8* 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(voff), "s"(sbase)
                  : "memory", "m0");
 }
+// The same of 4 bytes per lane, to lds_base + 4 lane.
+__device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, lds_u8* lds_base) {
+    const uint32_t m0v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_base));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(voff), "s"(sbase)
+                 : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // Workgroup barrier for LDS producer/consumer hand-off: LDS writes of this
@@ -173,6 +179,9 @@ __device__ __forceinline__ u32x4 buffer_load16(__amdgpu_buffer_rsrc_t r, uint32_
 }
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// The same with the last N LDS accesses of this wave still under way (LDS answers in order).
+template <int N>
+__device__ __forceinline__ void lds_barrier_but() { asm volatile("s_waitcnt lgkmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
 // vmcnt(N) with the other counters open (gfx9 layout: vmcnt[3:0] | expcnt[6:4]
 // | lgkmcnt[11:8] | vmcnt[5:4] at [15:14]).  Vector memory ops retire in issue

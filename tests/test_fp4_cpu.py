@@ -11,7 +11,7 @@ import torch
 from gdn_18646_amd import abi, blocks, compile_kernels, native_extension
 from gdn_18646_amd.abi import GdnError, GradTensor
 from tests.fp4 import nearest, pack, quantize64, unpack, values
-from tests.test_isa_cpu import _assembly, _events, _function
+from tests.test_isa_cpu import _assembly, _function
 
 FAKE = 4096  # non-null, aligned; never dereferenced
 BF, F32, E8 = 0, 1, 2
@@ -164,9 +164,8 @@ def test_the_definition_that_the_kernels_are_held_to():
 # ---------------------------------------------------------------------------
 # Assembly
 # ---------------------------------------------------------------------------
-# columns: staged rows of a token, waves along columns, tokens, MFMA tiles of a wave along each, stages
-PHASED = {"e2m1 256x256": (1, 4, 2, 4, 8, 2), "e2m1 256x192": (1, 4, 2, 4, 6, 2), "e2m1 256x160": (1, 4, 2, 4, 5, 2), "e2m1 256x128": (1, 4, 2, 4, 4, 3),
-          "e2m1 128x192": (1, 2, 4, 4, 3, 3), "e4m3 256x160": (2, 4, 2, 4, 5, 2), "e4m3 256x128": (2, 4, 2, 4, 4, 2), "e4m3 128x192": (2, 2, 4, 4, 3, 2)}
+# staged rows of a token, waves along columns, tokens, MFMA tiles of a wave along each, stages, workgroups on a CU
+STREAM = {"e2m1 256x256": (0, 2, 4, 8, 4, 2, 1), "e2m1 128x128": (0, 2, 2, 4, 4, 2, 2), "e4m3 256x128": (1, 4, 2, 4, 4, 2, 1), "e4m3 128x64": (1, 2, 2, 4, 2, 2, 2)}
 
 
 @pytest.fixture(scope="module")
@@ -174,45 +173,38 @@ def asm(tmp_path_factory):
     return {f: _assembly(f"fp4_mm_{f}.hip", tmp_path_factory) for f in ("e2m1", "e4m3")}
 
 
-def _kernels(text, tile=""):
-    return re.findall(rf"^(_Z\w*gdn_fp4_matmul_kernel\w*Fp4TileI{tile}\w*):", text, re.M)
+def _kernels(text, kind, tile=""):
+    return re.findall(rf"^(_Z\w*gdn_fp4_{kind}_kernel\w*Fp4TileILb{tile}\w*):", text, re.M)
 
 
 def test_no_tile_spills(asm):
-    assert len(_kernels(asm["e2m1"])) == 2 * 12 and len(_kernels(asm["e4m3"])) == 10 + 7
-    for text in asm.values():
-        for name in _kernels(text):
-            assert not any("scratch_" in ln for ln in _function(text, name)), name
+    """And every copy into LDS has its base in scalar registers."""
+    for text, stream, ring in ((asm["e2m1"], 2 * 2, 2 * 6), (asm["e4m3"], 2, 5 + 6)):
+        kernels = _kernels(text, "stream"), _kernels(text, "ring")
+        assert [len(k) for k in kernels] == [stream, ring]
+        for name in sum(kernels, []):
+            lines = _function(text, name)
+            assert not any("scratch_" in ln for ln in lines), name
+            assert not any("global_load_lds" in ln and "s[" not in ln for ln in lines), name
 
 
-@pytest.mark.parametrize("tile", PHASED)
-def test_phased_tiles_keep_their_counted_waits(asm, tile):
-    """A stage's LDS buffer is refilled region by region; the waits before the barriers that
-    open a phase count the copies issued after the region that the next phase reads, which
-    holds only for these copies in this order: none moved over a wait, merged or dropped."""
-    xh, cw, tw, wmt, wnt, ns = PHASED[tile]
-    m0, x0 = wmt // 2, (wnt + 1) // 2
-    groups = [2 * xh * tw * x0, 2 * cw * m0, 2 * cw * (wmt - m0), 2 * xh * tw * (wnt - x0)]  # X0, W0, W1, X1: 8-row copies, split over 8 waves
-    n = [g // 8 + g % 8 // 4 for g in groups]
-    n[0] += 2  # the scales of both operands
-    every = sum(n)
+@pytest.mark.parametrize("tile", STREAM)
+def test_stream_tiles_keep_their_counted_waits(asm, tile):
+    """A stage's wait counts what has been issued since the copies that it waits for: the next
+    W with its scales, and the stores of the tile before.  It holds if there are no fewer of
+    them: all of a tile's products before its stores, at least as many stores as are counted,
+    and no vector memory access of the compiler's own."""
+    x8, cw, tw, wmt, wnt, ns, per = STREAM[tile]
+    w, x = 2 * wmt // tw, 2 * wnt * (1 + x8) // cw  # 1 KiB copies of a wave: 16 wmt cw rows over 8 cw tw, and so on
     text = asm[tile.split()[0]]
-    names = _kernels(text, "".join(f"Li{v}E" for v in (xh, cw, tw, wmt, wnt, ns)))
-    assert len(names) == (2 if xh == 1 else 1), names  # bf16 and fp32 results
+    names = _kernels(text, "stream", "".join(("%dE" % x8, *(f"Li{v}E" for v in (cw, tw, wmt, wnt, ns, per)))))
+    assert len(names) == (1 if x8 else 2), names  # bf16 and fp32 results
     for name in names:
-        events = _events(_function(text, name))
-
-        def found(want):
-            return any(events[i:i + len(want)] == want for i in range(len(events)))
-
-        # a stage of the loop, from any of its phases on
-        stage = (["c"] * n[3] + [n[3] + (ns - 1) * every, "b", "b"] + ["c"] * n[0] + [n[0] + (ns - 1) * every, "b", "b"]
-                 + ["c"] * n[1] + ["b", "b"] + ["c"] * n[2] + [n[2] + (ns - 1) * every, "b", "b"])
-        assert any(found(stage[i:] + stage[:i]) for i in range(len(stage)))
-        # the stages after the last issued one, t of them left
-        for t in range(ns):
-            tail = [n[3] + t * every, "b", "b", t * every, "b", "b", "b", "b"]
-            tail += [n[2] + n[3] + (t - 1) * every, "b"] if t else []
-            assert found((["c"] * n[3] if t == ns - 1 else []) + tail), t
-        # the ring is filled (all but X1 of its last stage) before a tile's first stage waits for X0, the scales and W0
-        assert n[2] + (ns - 1) * every in events[events.index("c"):]
+        lines = _function(text, name)
+        assert sum("v_mfma_scale" in ln for ln in lines) == 2 * wmt * wnt
+        waits = {int(n) for ln in lines for n in re.findall(r"vmcnt\((\d+)\)", ln)}
+        assert waits == {0, w + 2, 4 * wnt + w + 2, w + 2 + x}, waits
+        last = max(i for i, ln in enumerate(lines) if "v_mfma" in ln)
+        whole = [ln for ln in lines if re.search(r"global_store_dwordx[24]", ln)]
+        assert len(whole) >= 2 * 4 * wnt  # inside the result, and at its edges
+        assert not any(re.search(r"\bglobal_load_(?!lds)|\bflat_|\bbuffer_", ln) for ln in lines[:last])
