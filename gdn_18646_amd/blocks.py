@@ -32,7 +32,7 @@ from . import compile_kernels, native_extension
 __all__ = ["block_norm", "fp8_linear", "Fp8Weight", "fp4_linear", "Fp4Weight", "grad_norm", "clip_grad_norm"]
 
 BLOCK = 128
-E2M1X2, E4M3, E5M2 = torch.float4_e2m1fn_x2, torch.float8_e4m3fn, torch.float8_e5m2
+E2M1X2, E4M3 = torch.float4_e2m1fn_x2, torch.float8_e4m3fn
 
 
 def _check_capture():
@@ -184,44 +184,6 @@ class Fp4Weight:
         return compile_kernels()["proj"].fp4_dequantize(self.codes, self.scales, columns=self.shape[1], dtype=dtype)
 
 
-class _Fp4Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, activations, record):
-        proj = compile_kernels()["proj"]
-        need_x, need_w = (record and need for need in ctx.needs_input_grad[:2])
-        x2 = _adjacent(x.reshape(-1, x.shape[-1]))
-        q8 = activations == E4M3  # from one read with the codes that dW takes
-        q = proj.fp8_quantize(x2, rows=q8, columns=need_w) if q8 or need_w else []
-        a = q[:2] if q8 else proj.fp4_quantize(x2)
-        w = weight if isinstance(weight, Fp4Weight) else Fp4Weight(weight, transposed=need_x)
-        if need_x and w.codes_t is None:
-            raise ValueError("fp4_linear: the gradient of x needs an Fp4Weight with transposed=True")
-        ctx.save_for_backward(*(q[-2:] if need_w else (None, None)), *((w.codes_t, w.scales_t) if need_x else (None, None)))
-        ctx.shape, ctx.dtypes = x.shape, (x.dtype, getattr(weight, "dtype", None))
-        ctx.sizes = w.shape
-        return proj.fp4_matmul(a[0], a[1], w.codes, w.scales, out_dtype=x.dtype).reshape(*x.shape[:-1], w.shape[0])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        _check_capture()
-        proj = compile_kernels()["proj"]
-        xt, xts, wt, wts = ctx.saved_tensors
-        N, K = ctx.sizes
-        need_x, need_w = ctx.needs_input_grad[:2]
-        if dy.numel() == 0:  # no tokens, or no columns
-            return (torch.zeros(ctx.shape, dtype=ctx.dtypes[0], device=dy.device) if need_x else None,
-                    torch.zeros(N, K, dtype=ctx.dtypes[1], device=dy.device) if need_w else None, None, None)
-        d = proj.fp8_quantize(_adjacent(dy.reshape(-1, N)), dtype=E5M2, rows=need_x, columns=need_w)
-        dx = dw = None
-        if need_x:
-            dx = proj.fp4_matmul(d[0], d[1], wt, wts, out_dtype=ctx.dtypes[0]).reshape(ctx.shape)
-        if need_w:
-            dt, dts = d[-2:]
-            dw = proj.fp8_matmul(dt, dts, xt, xts, out_dtype=ctx.dtypes[1])
-        return dx, dw, None, None
-
-
 def fp4_linear(x, weight, activations=E4M3):
     """x [..., K] times weight^T, the weight in 4-bit codes: [..., N] of x's type.
 
@@ -238,7 +200,12 @@ def fp4_linear(x, weight, activations=E4M3):
         raise ValueError(f"fp4_linear: x [..., {x.shape[-1] if x.dim() else ''}] and weight {tuple(weight.shape)}")
     if activations not in (E4M3, E2M1X2):
         raise ValueError(f"fp4_linear: activations in torch.float8_e4m3fn or torch.float4_e2m1fn_x2, got {activations}")
-    return _Fp4Linear.apply(x, weight, activations, torch.is_grad_enabled())
+    f, fp4 = compile_kernels()["proj"].fp4_linear, activations == E2M1X2
+    if not isinstance(weight, Fp4Weight):
+        return f(x, weight, None, None, None, None, weight.shape[0], fp4)
+    if weight.codes_t is None and x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("fp4_linear: the gradient of x needs an Fp4Weight with transposed=True")
+    return f(x, None, weight.codes, weight.scales, weight.codes_t, weight.scales_t, weight.shape[0], fp4)
 
 
 def grad_norm(grads):

@@ -197,7 +197,9 @@ std::vector<Opt> block_norm_backward(const Opt& dh, const Opt& dn, const Tensor&
     return out;
 }
 
-std::vector<Tensor> fp8_quantize(const Tensor& x, int64_t block_rows, at::ScalarType dtype, bool rows, bool columns) {
+}  // namespace
+
+std::vector<Tensor> gdn_bindings::fp8_quantize(const Tensor& x, int64_t block_rows, at::ScalarType dtype, bool rows, bool columns) {
     TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a GPU tensor [M, K]");
     TORCH_CHECK(x.size(1) <= 1 || x.stride(1) == 1, "x must have adjacent elements along its last axis");
     TORCH_CHECK(dtype == at::kFloat8_e4m3fn || dtype == at::kFloat8_e5m2, "dtype must be float8_e4m3fn or float8_e5m2");
@@ -234,7 +236,7 @@ std::vector<Tensor> fp8_quantize(const Tensor& x, int64_t block_rows, at::Scalar
     return out;
 }
 
-Tensor fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, at::ScalarType out_dtype) {
+Tensor gdn_bindings::fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, at::ScalarType out_dtype) {
     TORCH_CHECK(a.is_cuda() && a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(1), "a, b must be GPU tensors [M, K], [N, K]");
     TORCH_CHECK(a_scale.device() == a.device() && b.device() == a.device() && b_scale.device() == a.device(),
                 "the operands must be on one device");
@@ -271,6 +273,8 @@ Tensor fp8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     return out;
 }
 
+namespace {
+
 // Whether a node's stream is one that a capture on the current stream must not
 // wait for or write to: another than the current one, and not part of a capture.
 bool outside_capture(const c10::Stream& s) {
@@ -285,9 +289,11 @@ bool outside_capture(const c10::Stream& s) {
     return status != hipStreamCaptureStatusActive;
 }
 
+}  // namespace
+
 // The nodes that the running backward pass has to run (empty outside of one), by
 // name, and whether each belongs to a stream outside of the current capture.
-std::vector<std::pair<std::string, bool>> backward_nodes() {
+std::vector<std::pair<std::string, bool>> gdn_bindings::backward_nodes() {
     std::vector<std::pair<std::string, bool>> out;
     const auto* const nodes = torch::autograd::get_current_graph_task_nodes_in_graph();
     if (!nodes) return out;
@@ -303,11 +309,9 @@ std::vector<std::pair<std::string, bool>> backward_nodes() {
     return out;
 }
 
-}  // namespace
-
 void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11::module_& proj) {
     namespace py = pybind11;
-    top.def("_backward_nodes", &backward_nodes);
+    top.def("_backward_nodes", &gdn_bindings::backward_nodes);
     const py::object none = py::none();
     rmsnorm.def("block_norm", &block_norm,
                 "u = RMSNorm(y) post_gamma; h = residual + residual_scale scale act(gate) u; n = RMSNorm(h) gamma.\n"
@@ -328,13 +332,13 @@ void bind_block_ops(pybind11::module_& top, pybind11::module_& rmsnorm, pybind11
                 py::arg("dh"), py::arg("dn"), py::arg("y"), py::arg("residual") = none, py::arg("gate") = none,
                 py::arg("post_gamma") = none, py::arg("gamma") = none, py::arg("scale") = none,
                 py::arg("residual_scale") = 1.0, py::arg("act") = "none", py::arg("rstd_y") = none, py::arg("rstd_h") = none);
-    proj.def("fp8_quantize", &fp8_quantize,
+    proj.def("fp8_quantize", &gdn_bindings::fp8_quantize,
              "x [M, K] (bf16 or fp32) to 8-bit codes with a power-of-two scale for each block of block_rows (1 or 128) x 128: "
              "[codes, scales] along the rows (codes [M, K padded to 128]), and / or along the columns (codes of x^T "
              "[K, M padded to 128]), in that order.  Scales: float8_e8m0fnu, a row of codes or 128 of them by blocks.",
              py::arg("x"), py::arg("block_rows") = 1, py::arg("dtype") = at::kFloat8_e4m3fn, py::arg("rows") = true,
              py::arg("columns") = false);
-    proj.def("fp8_matmul", &fp8_matmul,
+    proj.def("fp8_matmul", &gdn_bindings::fp8_matmul,
              "out [M, N] = (a a_scale) (b b_scale)^T for codes a [M, K], b [N, K] (float8_e4m3fn or float8_e5m2, K a multiple "
              "of 128) with a scale a block of 128: a_scale float8_e8m0fnu [M, K / 128]; b_scale float8_e8m0fnu or float32 "
              "[N, K / 128] or, a 128 x 128 block each, [ceil(N / 128), K / 128].  fp32 results sum every product in full; for "

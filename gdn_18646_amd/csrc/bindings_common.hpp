@@ -9,6 +9,13 @@
 
 #include "../../include/gdn_amd.h"
 
+// Defined in bindings_block.cpp.
+namespace gdn_bindings {
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, int64_t block_rows, at::ScalarType dtype, bool rows, bool columns);
+at::Tensor fp8_matmul(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, at::ScalarType out_dtype);
+std::vector<std::pair<std::string, bool>> backward_nodes();
+}  // namespace gdn_bindings
+
 namespace {
 
 using at::Tensor;

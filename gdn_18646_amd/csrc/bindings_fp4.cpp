@@ -1,7 +1,11 @@
 // Torch binding of the 4-bit quantisation and the product with 4-bit weights:
-//   proj.fp4_quantize, proj.fp4_dequantize, proj.fp4_matmul
+//   proj.fp4_quantize, proj.fp4_dequantize, proj.fp4_matmul, proj.fp4_linear
 // Errors surface as RuntimeError; launches go to torch's current HIP stream of
 // the tensors' device.
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "bindings_common.hpp"
 
 namespace {
@@ -117,6 +121,101 @@ Tensor fp4_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     return out;
 }
 
+// x [M, K] with a row's elements adjacent, as the quantisation reads them; expanded
+// and transposed ones are copied.
+Tensor adjacent(const Tensor& x) {
+    return x.stride(1) == 1 && x.stride(0) >= x.size(1) ? x : x.contiguous();
+}
+
+// Refuses a backward pass that is being captured into a graph and has yet to reach nodes
+// of eager work, such as the gradient accumulators of leaves that an eager graph keeps
+// alive: they belong to the eager work's stream, which autograd would draw into the
+// capture, and that ends the process.
+void check_capture() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    std::string outside;
+    for (const auto& node : gdn_bindings::backward_nodes())
+        if (node.second && outside.find(node.first) == std::string::npos) outside += (outside.empty() ? "" : ", ") + node.first;
+    TORCH_CHECK(outside.empty(), "a backward pass is captured while an eager autograd graph of the same leaves is alive: drop (or detach) "
+                                 "the eager results before the capture (", outside, ")");
+}
+
+// The linear layer with its gradients, in C++: forward and backward take 96 us of host time,
+// through Python's autograd 133; the kernels of 2683 x 2048 x 2048 take 95.
+class Fp4Linear : public torch::autograd::Function<Fp4Linear> {
+public:
+    // weight: a tensor to quantise here, or none, with w its codes and scales (and those of
+    // its transpose, or undefined ones).  record: whether gradients are recorded.
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Opt& weight, std::vector<Tensor> w, int64_t N, bool fp4,
+                          bool record) {
+        const bool need_x = record && x.requires_grad(), need_w = record && given(weight) && weight->requires_grad();
+        const int64_t K = x.size(-1);
+        const Tensor x2 = adjacent(x.reshape({-1, K}));
+        std::vector<Tensor> q8, q4;
+        if (!fp4 || need_w) q8 = gdn_bindings::fp8_quantize(x2, 1, at::kFloat8_e4m3fn, !fp4, need_w);  // from one read with the codes that dW takes
+        if (fp4) q4 = fp4_quantize(x2, 1, true, false);
+        if (given(weight)) {
+            w = fp4_quantize(adjacent(weight->detach()), 32, true, need_x);
+            w.resize(4);
+        }
+        ctx->save_for_backward({need_w ? q8[q8.size() - 2] : Tensor(), need_w ? q8.back() : Tensor(), need_x ? w[2] : Tensor(), need_x ? w[3] : Tensor()});
+        ctx->saved_data["need_x"] = need_x;
+        ctx->saved_data["need_w"] = need_w;
+        ctx->saved_data["sizes"] = x.sizes().vec();
+        ctx->saved_data["N"] = N;
+        ctx->saved_data["types"] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), static_cast<int64_t>(given(weight) ? weight->scalar_type() : x.scalar_type())};
+        const auto& a = fp4 ? q4 : q8;
+        auto sizes = x.sizes().vec();
+        sizes.back() = N;
+        return at::_unsafe_view(fp4_matmul(a[0], a[1], w[0], w[1], x.scalar_type()), sizes);  // no view: a caller may write to it
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(6);
+        {
+            const at::NoGradGuard no_grad;
+            compute(ctx, grads[0], out);
+        }
+        if (!at::GradMode::is_enabled()) return out;
+        // a graph of the gradients is recorded: using it for second derivatives raises
+        for (auto& t : out)
+            if (t.defined()) {
+                t.requires_grad_();
+                t = (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice fp4_linear, which has first derivatives alone", 1))({t})[0];
+            }
+        return out;
+    }
+
+private:
+    static void compute(torch::autograd::AutogradContext* ctx, const Tensor& dy, torch::autograd::variable_list& out) {
+        check_capture();
+        const auto saved = ctx->get_saved_variables();
+        const bool need_x = ctx->saved_data["need_x"].toBool() && ctx->needs_input_grad(0);
+        const bool need_w = ctx->saved_data["need_w"].toBool() && ctx->needs_input_grad(1);
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        const auto tx = static_cast<at::ScalarType>(types[0]), tw = static_cast<at::ScalarType>(types[1]);
+        const int64_t N = ctx->saved_data["N"].toInt(), K = sizes.back();
+        if (!dy.defined() || (!need_x && !need_w)) return;
+        if (dy.numel() == 0) {  // no tokens, or no columns
+            if (need_x) out[0] = at::zeros(sizes, dy.options().dtype(tx));
+            if (need_w) out[1] = at::zeros({N, K}, dy.options().dtype(tw));
+            return;
+        }
+        const auto d = gdn_bindings::fp8_quantize(adjacent(dy.reshape({-1, N})), 1, at::kFloat8_e5m2, need_x, need_w);
+        if (need_x) out[0] = at::_unsafe_view(fp4_matmul(d[0], d[1], saved[2], saved[3], tx), sizes);
+        if (need_w) out[1] = gdn_bindings::fp8_matmul(d[d.size() - 2], d.back(), saved[0], saved[1], tw);
+    }
+};
+
+Tensor fp4_linear(const Tensor& x, const Opt& weight, const Opt& codes, const Opt& scales, const Opt& codes_t, const Opt& scales_t, int64_t N, bool fp4) {
+    TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
+    TORCH_CHECK(given(weight) ? weight->dim() == 2 && x.dim() >= 1 && weight->size(0) == N && weight->size(1) == x.size(-1) : given(codes) && given(scales),
+                "fp4_linear: a weight [N, K] for x [..., K], or its codes and scales");
+    std::vector<Tensor> w;
+    for (const auto* const t : {&codes, &scales, &codes_t, &scales_t}) w.push_back(given(*t) ? **t : Tensor());
+    return Fp4Linear::apply(x, weight, w, N, fp4, at::GradMode::is_enabled());
+}
+
 }  // namespace
 
 void bind_fp4_ops(pybind11::module_& proj) {
@@ -138,4 +237,8 @@ void bind_fp4_ops(pybind11::module_& proj) {
              "below 2^-17 of the largest of 128 products.  Scales are read as fp4_quantize and fp8_quantize lay them out; others are "
              "copied into that layout first.",
              py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("out_dtype") = at::kBFloat16);
+    proj.def("fp4_linear", &fp4_linear,
+             "x [..., K] times a weight [N, K]^T on 4-bit codes of the weight and 8-bit (fp4: 4-bit) ones of x, with gradients: what "
+             "blocks.fp4_linear calls.  weight, or codes and scales (and codes_t, scales_t for the gradient of x).",
+             py::arg("x"), py::arg("weight"), py::arg("codes"), py::arg("scales"), py::arg("codes_t"), py::arg("scales_t"), py::arg("N"), py::arg("fp4"));
 }

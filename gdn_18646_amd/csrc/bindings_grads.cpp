@@ -1,6 +1,8 @@
 // Torch binding of the gradients' norm and clipping: grads.norm, grads.clip.
 // Errors surface as RuntimeError; launches go to torch's current HIP stream of
 // the tensors' device.
+#include <c10/hip/HIPCachingAllocator.h>
+
 #include "bindings_common.hpp"
 
 namespace {
@@ -13,7 +15,8 @@ void check_dense(const Tensor& t, const Tensor& first, const char* name, size_t 
 
 struct Call {
     std::vector<gdn_grad_t> grads;
-    Tensor norm, workspace;
+    Tensor norm;
+    c10::DataPtr workspace;  // the allocator's own: a tensor costs more host time
     size_t bytes = 0;
 };
 Call call_of(const std::vector<Tensor>& grads) {
@@ -30,14 +33,14 @@ Call call_of(const std::vector<Tensor>& grads) {
 void allocate(Call& c, const Tensor& t) {
     c.norm = fresh({}, at::kFloat, t);
     c.bytes = gdn_grad_norm_workspace_bytes(static_cast<int64_t>(c.grads.size()));
-    c.workspace = fresh({static_cast<int64_t>(c.bytes)}, at::kByte, t);
+    c.workspace = c10::hip::HIPCachingAllocator::get()->allocate(c.bytes);
 }
 
 Tensor norm(const std::vector<Tensor>& grads) {
     Call c = call_of(grads);
     const c10::DeviceGuard guard(grads[0].device());
     allocate(c, grads[0]);
-    check_status(gdn_grad_norm_hip(c.grads.data(), static_cast<int64_t>(c.grads.size()), c.norm.data_ptr<float>(), c.workspace.data_ptr(), c.bytes,
+    check_status(gdn_grad_norm_hip(c.grads.data(), static_cast<int64_t>(c.grads.size()), c.norm.data_ptr<float>(), c.workspace.get(), c.bytes,
                                    stream_of(grads[0])),
                  "grad_norm");
     return c.norm;
@@ -68,7 +71,7 @@ Tensor clip(const std::vector<Tensor>& grads, double max_norm, const std::option
     const c10::DeviceGuard guard(grads[0].device());
     allocate(c, grads[0]);
     check_status(gdn_clip_grad_norm_hip(c.grads.data(), static_cast<int64_t>(c.grads.size()), max_norm, c.norm.data_ptr<float>(),
-                                        c.workspace.data_ptr(), c.bytes, stream_of(grads[0])),
+                                        c.workspace.get(), c.bytes, stream_of(grads[0])),
                  "clip_grad_norm");
     for (const Tensor& t : to)
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // a graph that saved it raises

@@ -152,12 +152,6 @@ __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, lds_u8* 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(voff), "s"(sbase)
                  : "memory", "m0");
 }
-// The same of 4 bytes per lane, to lds_base + 4 lane.
-__device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, lds_u8* lds_base) {
-    const uint32_t m0v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds_base));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(voff), "s"(sbase)
-                 : "memory", "m0");
-}
 #pragma clang diagnostic pop
 
 // Workgroup barrier for LDS producer/consumer hand-off: LDS writes of this
