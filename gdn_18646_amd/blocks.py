@@ -222,11 +222,15 @@ def grad_norm(grads):
 def clip_grad_norm(grads, max_norm, out=None):
     """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)), where norm is
     ``grad_norm(grads)``, in place or into ``out`` (tensors of the same shapes, bf16 or
-    fp32, for an optimiser that keeps its own); returns the norm before.
+    fp32, for an optimiser that keeps its own, one for each of the gradients); returns
+    the norm before.  None among the gradients is left out.
 
     Nothing is read back to the host, so the call can be captured into a graph.  A norm
     that is NaN makes every result NaN.
     """
-    if out is None:
-        grads = [g for g in grads if g is not None]
+    if out is not None:
+        if len(out) != len(grads):
+            raise ValueError(f"clip_grad_norm: {len(grads)} gradients and {len(out)} results")
+        out = [o for g, o in zip(grads, out) if g is not None]
+    grads = [g for g in grads if g is not None]
     return native_extension().grads.clip(grads, float(max_norm), out) if grads else torch.zeros(())

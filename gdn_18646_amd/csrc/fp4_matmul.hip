@@ -152,6 +152,8 @@ int launch(const gdn_fp4::MatmulParams& p, bool f32, hipStream_t stream) {
         while (2 * mask <= (p.K + 255) / 256) mask *= 2;
         const auto few = [&](auto out32, auto waves) {
             constexpr int W = decltype(waves)::value;
+            if (!gdn_host::grid_fits((p.N + 15) / 16, 64 * W))
+                return gdn_host::fail(GDN_ERR_UNSUPPORTED, "fp4_matmul: M=%d N=%d are too large for a launch", p.M, p.N);
             hipLaunchKernelGGL((gdn_fp4_few_kernel<FA, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, mask - 1);
             return gdn_host::check_launch("gdn_fp4_few_kernel");
         };

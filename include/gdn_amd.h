@@ -502,7 +502,9 @@ int gdn_fp4_dequantize_hip(const uint8_t* codes, int64_t ldc, const uint8_t* sca
  * 2^28.  With 8-bit codes, bf16 results leave 128 products to one instruction, which
  * drops what lies below 2^-17 of the largest; fp32 results sum every product in full.
  * Scales may be anything that the type holds; only the product of the two (of a row and
- * a column, in each block) has to be in fp32's range.  A row's sums do not depend on
+ * a column, in each block) has to be in fp32's range (fp32 results of 8-bit codes: where
+ * the four scales of 128 values of b lie more than 2^110 apart, the smallest ones'
+ * products lose bits).  A row's sums do not depend on
  * other rows' values; their order follows M, N, K and the column.
  */
 int gdn_fp4_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_t* a_scale, int64_t lda_s,

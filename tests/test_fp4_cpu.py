@@ -62,7 +62,7 @@ def _mm(**k):
 @pytest.mark.parametrize("bad,match", [
     (dict(M=-1), "INVALID_ARGUMENT"), (dict(K=0), "INVALID_ARGUMENT"), (dict(K=384), "multiple of 256"), (dict(fa=E4M3, K=200), "multiple of 128"),
     (dict(fa=3), "format 3"), (dict(to=E8), "type 2 of out"), (dict(lda=1 << 23), "too large"), (dict(M=1 << 29), "too large"), (dict(N=1 << 29), "too large"),
-    (dict(ldbs=1 << 30), "too large"), (dict(a=None), "null"), (dict(sb=None), "null"), (dict(out=None), "null"), (dict(a=FAKE + 8), "16-byte"),
+    (dict(ldbs=1 << 30), "too large"), (dict(M=1, N=1 << 28, ldbs=1 << 28, ldo=1 << 28), "too large for a launch"), (dict(a=None), "null"), (dict(sb=None), "null"), (dict(out=None), "null"), (dict(a=FAKE + 8), "16-byte"),
     (dict(ldb=240), "16-byte"), (dict(ldb=264), "16-byte"), (dict(fa=E4M3), "16-byte"), (dict(ldas=36), "a's scales"), (dict(ldas=42), "a's scales"),
     (dict(sa=FAKE + 4), "a's scales"), (dict(fa=E4M3, lda=512, ldas=40), "a's scales"), (dict(ldbs=96), "b's scales"), (dict(ldbs=102), "b's scales"),
     (dict(sb=FAKE + 8), "b's scales"), (dict(ldo=99), "ldo"), (dict(out=FAKE + 1), "unaligned"), (dict(fa=E4M3, K=384, lda=384, ldb=128), "16-byte")])

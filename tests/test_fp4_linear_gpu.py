@@ -270,3 +270,19 @@ def test_what_autograd_may_ask(dev):
         assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw)
         x.grad = w.grad = None
         assert torch.equal(torch.utils.checkpoint.checkpoint(fp4_linear, x, w, a, use_reentrant=False), y.detach())
+
+
+def test_one_axis_and_another_stream(dev):
+    """A single token without a batch axis; forward and backward on a stream of their own."""
+    x, w = _rand((256,), torch.bfloat16, dev, 1), _rand((128, 256), torch.bfloat16, dev, 2, 0.05)
+    x2 = x.detach().view(1, 256).requires_grad_()
+    y, y2 = fp4_linear(x, w), fp4_linear(x2, w)
+    want = torch.autograd.grad(y2.sum(), (x2, w))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        z = fp4_linear(x, w)
+        dx, dw = torch.autograd.grad(z.sum(), (x, w))
+    side.synchronize()
+    assert y.shape == (128,) and dx.shape == (256,) and torch.equal(y, y2[0]) and torch.equal(z, y)
+    assert torch.equal(dx, want[0][0]) and torch.equal(dw, want[1])

@@ -191,3 +191,17 @@ def test_c_abi_of_no_tensors(dev):
     norm, ws = torch.full((1,), 5.0, device=dev), torch.empty(64, dtype=torch.uint8, device=dev)
     abi.call("gdn_grad_norm_hip", None, 0, norm.data_ptr(), ws.data_ptr(), 64, torch.cuda.current_stream().cuda_stream)
     assert norm.item() == 0.0
+
+
+def test_results_of_gradients_with_none_among_them(dev):
+    g = torch.Generator().manual_seed(4)
+    grads = [torch.randn(50, generator=g).to(dev), None, torch.randn(3, 7, generator=g).to(dev, BF)]
+    outs = [torch.full((50,), 9.0, device=dev), torch.full((4,), 9.0, device=dev), torch.full((3, 7), 9.0, device=dev)]
+    want = [torch.empty(50, device=dev), torch.empty(3, 7, device=dev)]
+    norm = clip_grad_norm(grads, 0.5, out=outs)
+    assert torch.equal(norm, clip_grad_norm([grads[0], grads[2]], 0.5, out=want))
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[2], want[1]) and (outs[1] == 9.0).all()
+    with pytest.raises(ValueError, match="3 gradients and 2 results"):
+        clip_grad_norm(grads, 0.5, out=outs[:2])
+    with pytest.raises(ValueError, match="0 gradients and 3 results"):
+        clip_grad_norm([], 0.5, out=outs)
