@@ -85,10 +85,11 @@ __global__ __launch_bounds__(64 * WAVES) void gdn_fp4_few_kernel(gdn_fp4::Matmul
 struct TileCost {
     int tile, cols, toks, per_cu;
     float c, a1, b1, a2, b2;  // per_cu above 1: alone (1) and with per_cu on each CU (2)
+    int least_k = 0;          // shorter rows go to other tiles: what is stored then takes longer than the products
 };
 // Fitted to 320 products each, 3 to 8192 tokens, N 64 to 8224, K 256 to 8192, kernels
 // back to back on operands that the L2s do not hold: the tile that the fit picks takes
-// 1.016 times the best one's time on average (1.35 at most; 8-bit codes 1.010 and 1.12,
+// 1.016 times the best one's time on average (1.35 at most; 8-bit codes 1.011 and 1.17,
 // fp32 results of those 1.007 and 1.09).  Up to ten tiles were timed; those here are the
 // ones whose absence costs.
 constexpr TileCost kCost4[] = {
@@ -102,13 +103,14 @@ constexpr TileCost kCost4[] = {
     {gdn_fp4::k16x16, 16, 16, 3, 2.71f, 1.20f, 0.027f, 0.86f, 0.145f},
 };
 constexpr TileCost kCost8[] = {  // 8-bit codes of a, bf16 results
-    {gdn_fp4::k256x128, 256, 128, 1, 0.69f, 4.34f, 1.641f, 0.f, 0.f},
-    {gdn_fp4::k128x64, 128, 64, 2, 3.06f, 0.80f, 0.874f, 1.78f, 1.113f},
-    {gdn_fp4::k64x64, 64, 64, 1, 0.86f, 2.61f, 0.402f, 0.f, 0.f},
-    {gdn_fp4::k64x32, 64, 32, 1, 1.20f, 2.31f, 0.230f, 0.f, 0.f},
-    {gdn_fp4::k32x32, 32, 32, 1, 1.73f, 1.75f, 0.179f, 0.f, 0.f},
-    {gdn_fp4::k16x16Alone, 16, 16, 1, 2.29f, 1.41f, 0.062f, 0.f, 0.f},
-    {gdn_fp4::k16x16, 16, 16, 3, 2.56f, 1.20f, 0.067f, 0.91f, 0.194f},
+    {gdn_fp4::k256x256, 256, 256, 1, 0.00f, 8.65f, 2.482f, 0.f, 0.f, 1280},
+    {gdn_fp4::k256x128, 256, 128, 1, 0.00f, 5.08f, 1.661f, 0.f, 0.f},
+    {gdn_fp4::k128x64, 128, 64, 2, 3.42f, 0.33f, 0.908f, 1.43f, 1.108f},
+    {gdn_fp4::k64x64, 64, 64, 1, 0.77f, 2.62f, 0.413f, 0.f, 0.f},
+    {gdn_fp4::k64x32, 64, 32, 1, 1.08f, 2.36f, 0.234f, 0.f, 0.f},
+    {gdn_fp4::k32x32, 32, 32, 1, 1.53f, 1.81f, 0.186f, 0.f, 0.f},
+    {gdn_fp4::k16x16Alone, 16, 16, 1, 2.09f, 1.47f, 0.066f, 0.f, 0.f},
+    {gdn_fp4::k16x16, 16, 16, 3, 2.51f, 1.04f, 0.076f, 0.94f, 0.197f},
 };
 constexpr TileCost kCost32[] = {  // the same, fp32 results
     {gdn_fp4::k128x64, 128, 64, 2, 2.76f, 0.44f, 1.889f, 3.29f, 2.653f},
@@ -130,6 +132,7 @@ Choice choose_tile(const TileCost (&table)[N], long long M, long long cols, int 
     Choice best = {0, 0.f};
     for (size_t i = 0; i < N; ++i) {
         const TileCost& t = table[i];
+        if (K < t.least_k) continue;
         const long long tiles = (M + t.toks - 1) / t.toks * ((cols + t.cols - 1) / t.cols);
         const float alone = t.a1 + t.b1 * nk, full = t.a2 + t.b2 * nk;
         float us = t.c;
@@ -140,7 +143,7 @@ Choice choose_tile(const TileCost (&table)[N], long long M, long long cols, int 
             us += static_cast<float>(tiles / round) * full;
             if (each > 0) us += alone + static_cast<float>(each - 1) / static_cast<float>(t.per_cu - 1) * (full - alone);
         }
-        if (i == 0 || us < best.us) best = {t.tile, us};
+        if (best.us == 0.f || us < best.us) best = {t.tile, us};
     }
     return best;
 }

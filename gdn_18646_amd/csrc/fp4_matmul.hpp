@@ -1,7 +1,8 @@
 // Parameter block, launches and operand helpers of the product with 4-bit weights
 // (fp4_matmul.hip holds its entry point, the rule that picks its kernel and the
-// kernel for one token or two; fp4_tiles.hpp the tiled kernels, instantiated for each
-// format of the activations in fp4_mm_*.hip).
+// kernel for one token or two; fp4_tiles.hpp and fp4_phased.hpp the tiled kernels and
+// fp4_launch.hpp their launches, instantiated for each format of the activations in
+// fp4_mm_*.hip).
 #pragma once
 
 #include "fp4_blocks.hpp"
@@ -18,8 +19,8 @@ struct MatmulParams {
     int M, N, K;           // K: a multiple of 128, of 256 where a's codes are 4-bit too
 };
 
-// Tiles of the tiled kernels (columns x tokens), largest first: 256 x 256, 128 x 128 and 64 x
-// 128 for 4-bit codes of a alone, 256 x 128 and 16 x 16 alone on a CU for 8-bit ones.
+// Tiles of the tiled kernels (columns x tokens), largest first: 128 x 128 and 64 x 128 for
+// 4-bit codes of a alone, 256 x 128 and 16 x 16 alone on a CU for 8-bit ones.
 enum Tile { k256x256 = 0, k256x128, k128x128, k128x64, k64x128, k64x64, k64x32, k32x32, k16x16Alone, k16x16 };
 
 // Defined in fp4_mm_*.hip for each format of a.  f32: out is fp32, else bf16.

@@ -208,3 +208,17 @@ def test_stream_tiles_keep_their_counted_waits(asm, tile):
         whole = [ln for ln in lines if re.search(r"global_store_dwordx[24]", ln)]
         assert len(whole) >= 2 * 4 * wnt  # inside the result, and at its edges
         assert not any(re.search(r"\bglobal_load_(?!lds)|\bflat_|\bbuffer_", ln) for ln in lines[:last])
+
+
+def test_the_phased_tile(asm):
+    """No spills, scalar bases, the counted waits of its phases, and none of the compiler's own before its stores."""
+    (name,) = re.findall(r"^(_Z\w*gdn_fp4_phased_kernel\w*):", asm["e4m3"], re.M)
+    lines = _function(asm["e4m3"], name)
+    assert not any("scratch_" in ln for ln in lines) and not any("global_load_lds" in ln and "s[" not in ln for ln in lines)
+    w, x, stages = 1, 2, 3  # copies of a region by a wave: 64 columns, 128 tokens a wave's part
+    all_ = 2 * (w + x) + 2
+    steady = {x + (stages - 1) * all_, x + 2 + (stages - 1) * all_, w + (stages - 1) * all_}
+    last = {x + t * all_ for t in range(stages)} | {t * all_ for t in range(stages)} | {w + x + (t - 1) * all_ for t in range(1, stages)}
+    assert {int(n) for ln in lines for n in re.findall(r"vmcnt\((\d+)\)", ln)} == steady | last | {0}
+    assert sum("v_mfma_scale" in ln for ln in lines) == 4 * 8 * (1 + stages)
+    assert not any(re.search(r"\bglobal_load_(?!lds)|\bflat_|\bbuffer_", ln) for ln in lines)

@@ -215,6 +215,14 @@ def test_product_over_half_a_row_of_codes(exts, dev, M, N, K, fa):
         _check(_product(exts, a, b, out), a, b)
 
 
+@pytest.mark.parametrize("fa", [E4, E5], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("M,N,K", [(1490, 8210, 1408), (4000, 8100, 1280), (2048, 8192, 2048), (3800, 4111, 1536), (8000, 2000, 4224)])
+def test_product_of_large_tiles(exts, dev, M, N, K, fa):
+    """8-bit codes by 256 x 256 tiles: rows and columns past the end, odd numbers of blocks, one round and two."""
+    a, b = _operands(M, N, K, fa, dev)
+    _check(_product(exts, a, b), a, b)
+
+
 @pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
 @pytest.mark.parametrize("M,N", [(2100, 4400), (4200, 4400), (300, 1030), (1300, 1300), (40, 700)])
 def test_product_long(exts, dev, M, N, fa):
