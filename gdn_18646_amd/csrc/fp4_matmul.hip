@@ -6,7 +6,10 @@
 // straight from memory into MFMA fragments (no LDS: nothing is used twice), and
 // the waves' sums meet in LDS.  The workgroups of an XCD begin at different
 // places: 16 rows at a stride of a power of two lie in one or two of its L2's
-// channels, and in step they would all wait for the same ones.
+// channels, and in step they would all wait for the same ones.  A token by 8224 x 2048
+// takes 3.9 us with 4-bit codes and 4.4 with 8-bit ones, by 65536 x 2048 (71 MB) 14.3, 5.0
+// TB/s, and 18.0; the 16 x 16 tile of fp4_tiles.hpp, which takes three tokens and more, 4.4,
+// 4.3, 20.8 and 23.1, and fp32 results of 8-bit codes 5-30% longer than here.
 #include "fp4_matmul.hpp"
 
 namespace {
@@ -160,8 +163,12 @@ int launch(const gdn_fp4::MatmulParams& p, bool f32, hipStream_t stream) {
             hipLaunchKernelGGL((gdn_fp4_few_kernel<FA, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, mask - 1);
             return gdn_host::check_launch("gdn_fp4_few_kernel");
         };
+        // The CUs hold 512 workgroups of eight waves or 1024 of four: between those
+        // numbers the smaller ones need one round, the others two (9216 x 4096, 8-bit codes,
+        // 8.7 us with four and 9.5 with eight); else eight read more at a time (8192 x 4096
+        // 8.2 and 7.2, 2048 x 8192 9.5 and 6.1, 65536 x 2048 18.9 and 18.0).
         const auto of_n = [&](auto out32) {
-            return p.N <= 4096 ? few(out32, std::integral_constant<int, 8>{}) : few(out32, std::integral_constant<int, 4>{});
+            return p.N > 8192 && p.N < 16384 ? few(out32, std::integral_constant<int, 4>{}) : few(out32, std::integral_constant<int, 8>{});
         };
         return f32 ? of_n(std::true_type{}) : of_n(std::false_type{});
     }

@@ -215,6 +215,14 @@ def test_product_over_half_a_row_of_codes(exts, dev, M, N, K, fa):
         _check(_product(exts, a, b, out), a, b)
 
 
+@pytest.mark.parametrize("fa", [E2, E4], ids=["e2m1", "e4m3"])
+@pytest.mark.parametrize("M,N,K", [(1, 8192, 256), (2, 9001, 512), (1, 16383, 2560), (2, 16384, 256), (1, 20010, 4352)])
+def test_product_of_a_token_by_many_columns(exts, dev, M, N, K, fa):
+    a, b = _operands(M, N, K, fa, dev)
+    for out in (torch.float32, torch.bfloat16):
+        _check(_product(exts, a, b, out), a, b)
+
+
 @pytest.mark.parametrize("fa", [E4, E5], ids=["e4m3", "e5m2"])
 @pytest.mark.parametrize("M,N,K", [(1490, 8210, 1408), (4000, 8100, 1280), (2048, 8192, 2048), (3800, 4111, 1536), (8000, 2000, 4224)])
 def test_product_of_large_tiles(exts, dev, M, N, K, fa):
