@@ -66,6 +66,7 @@ SIGNATURES = {
     "gdn_fp8_quantize_hip": (_I, [_P, _I64, _I, _I64, _I64, _I, _I] + [_P, _I64] * 4 + [_P]),
     "gdn_fp8_matmul_hip": (_I, [_P, _I64, _I, _P, _I64] * 2 + [_I, _I, _P, _I64, _I] + [_I64] * 3 + [_P]),
     "gdn_fp4_quantize_hip": (_I, [_P, _I64, _I, _I64, _I64, _I] + [_P, _I64] * 4 + [_P]),
+    "gdn_fp4_fp8_quantize_hip": (_I, [_P, _I64, _I, _I64, _I64] + [_P, _I64] * 4 + [_P]),
     "gdn_fp4_dequantize_hip": (_I, [_P, _I64] * 3 + [_I, _I64, _I64, _P]),
     "gdn_fp4_matmul_hip": (_I, [_P, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I] + [_I64] * 3 + [_P]),
     "gdn_grad_norm_workspace_bytes": (_SZ, [_I64]),

@@ -1,5 +1,5 @@
 // Torch binding of the 4-bit quantisation and the product with 4-bit weights:
-//   proj.fp4_quantize, proj.fp4_dequantize, proj.fp4_matmul, proj.fp4_linear
+//   proj.fp4_quantize, proj.fp4_fp8_quantize, proj.fp4_dequantize, proj.fp4_matmul, proj.fp4_linear
 // Errors surface as RuntimeError; launches go to torch's current HIP stream of
 // the tensors' device.
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -65,6 +65,22 @@ std::vector<Tensor> fp4_quantize(const Tensor& x, int64_t block_rows, bool rows,
     check_status(gdn_fp4_quantize_hip(x.data_ptr(), ld, type, M, K, static_cast<int>(block_rows), ptr[0], up(K, 256) / 2, ptr[1], up(M, 16),
                                       ptr[2], up(M, 256) / 2, ptr[3], up(K, 16), stream_of(x)),
                  "fp4_quantize");
+    return out;
+}
+
+std::vector<Tensor> fp4_fp8_quantize(const Tensor& x) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a GPU tensor [M, K]");
+    TORCH_CHECK(x.size(1) <= 1 || x.stride(1) == 1, "x must have adjacent elements along its last axis");
+    const int type = type_of(x, "x");
+    const int64_t M = x.size(0), K = x.size(1), ld = M > 1 ? x.stride(0) : std::max<int64_t>(K, 1), Kp = up(K, 256), Mp = up(M, 128);
+    TORCH_CHECK(M == 0 || ld >= K, "x must not have rows that overlap");
+    const c10::DeviceGuard guard(x.device());
+    std::vector<Tensor> out = {fresh({M, Kp / 2}, kFp4, x), words(M, Kp / 128, x), fresh({K, Mp}, at::kFloat8_e4m3fn, x),
+                               down_columns(K, Mp / 128, at::kFloat8_e8m0fnu, x)};
+    if (M == 0 || K == 0) return out;  // no values: codes and scales are empty too
+    const auto ptr = [&](int i) { return static_cast<uint8_t*>(out[i].data_ptr()); };
+    check_status(gdn_fp4_fp8_quantize_hip(x.data_ptr(), ld, type, M, K, ptr(0), Kp / 2, ptr(1), up(M, 16), ptr(2), Mp, ptr(3), up(K, 16), stream_of(x)),
+                 "fp4_fp8_quantize");
     return out;
 }
 
@@ -151,23 +167,23 @@ public:
         const bool need_x = record && x.requires_grad(), need_w = record && given(weight) && weight->requires_grad();
         const int64_t K = x.size(-1);
         const Tensor x2 = adjacent(x.reshape({-1, K}));
-        std::vector<Tensor> q8, q4;
-        if (!fp4 || need_w) q8 = gdn_bindings::fp8_quantize(x2, 1, at::kFloat8_e4m3fn, !fp4, need_w);  // from one read with the codes that dW takes
-        if (fp4) q4 = fp4_quantize(x2, 1, true, false);
+        // x's codes for y and, from the same read, those that dW takes
+        const std::vector<Tensor> q = !fp4    ? gdn_bindings::fp8_quantize(x2, 1, at::kFloat8_e4m3fn, true, need_w)
+                                      : need_w ? fp4_fp8_quantize(x2)
+                                               : fp4_quantize(x2, 1, true, false);
         if (given(weight)) {
             w = fp4_quantize(adjacent(weight->detach()), 32, true, need_x);
             w.resize(4);
         }
-        ctx->save_for_backward({need_w ? q8[q8.size() - 2] : Tensor(), need_w ? q8.back() : Tensor(), need_x ? w[2] : Tensor(), need_x ? w[3] : Tensor()});
+        ctx->save_for_backward({need_w ? q[2] : Tensor(), need_w ? q[3] : Tensor(), need_x ? w[2] : Tensor(), need_x ? w[3] : Tensor()});
         ctx->saved_data["need_x"] = need_x;
         ctx->saved_data["need_w"] = need_w;
         ctx->saved_data["sizes"] = x.sizes().vec();
         ctx->saved_data["N"] = N;
         ctx->saved_data["types"] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), static_cast<int64_t>(given(weight) ? weight->scalar_type() : x.scalar_type())};
-        const auto& a = fp4 ? q4 : q8;
         auto sizes = x.sizes().vec();
         sizes.back() = N;
-        return at::_unsafe_view(fp4_matmul(a[0], a[1], w[0], w[1], x.scalar_type()), sizes);  // no view: a caller may write to it
+        return at::_unsafe_view(fp4_matmul(q[0], q[1], w[0], w[1], x.scalar_type()), sizes);  // no view: a caller may write to it
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         torch::autograd::variable_list out(6);
@@ -225,6 +241,10 @@ void bind_fp4_ops(pybind11::module_& proj) {
              "block_rows (1 or 32) x 32: [codes, scales] along the rows (float4_e2m1fn_x2 [M, K padded to 256, / 2]; float8_e8m0fnu [M, "
              "padded K / 128, 4]), and / or along the columns (of x^T), in that order.  With block_rows=32 both stand for the same values.",
              py::arg("x"), py::arg("block_rows") = 1, py::arg("rows") = true, py::arg("columns") = false);
+    proj.def("fp4_fp8_quantize", &fp4_fp8_quantize,
+             "From one read of x [M, K]: [codes, scales] of fp4_quantize(x) and those along the columns of fp8_quantize(x, rows=False, "
+             "columns=True), what a training step with 4-bit activations takes of x.",
+             py::arg("x"));
     proj.def("fp4_dequantize", &fp4_dequantize,
              "What 4-bit codes [M, K / 2] with scales [M, K / 128, 4] (or [M, K / 32]) stand for: [M, columns] (all of them without "
              "columns), bfloat16 or float32, exactly.",

@@ -1,19 +1,22 @@
 // Quantisation to 4-bit floating point in blocks of 32 (fp4_blocks.hpp), along the
 // rows of x [M, K], along its columns (the codes of x^T, for a product that sums
 // over x's rows), or both from one read; a block is 1 x 32 values along the codes'
-// own rows, or 32 x 32 of x, whose codes are the same ones both ways.  And back.
+// own rows, or 32 x 32 of x, whose codes are the same ones both ways.  Or along its rows
+// in 4 bits and along its columns in 8 (e4m3, blocks of 1 x 128, fp8_blocks.hpp): what a
+// training step with 4-bit activations takes of them, from one read.  And back.
 //
 // Quantisation: one workgroup a 128 x 128 tile, as for 8 bits: a thread holds 4 x 8
 // of it in registers, a row's maximum meets over 4 lanes by DPP, a column's over
 // LDS, and the transposed codes pass through LDS.  Bound by memory where there are tiles
 // enough: 8224 x 2048 bf16 both ways (52 MB) 12.9 us, 4.0 TB/s; 8192 x 4096 along the rows
-// (85 MB) 15.9, 5.4; one row of 2048 3.3 us, a launch, a load and a store.
+// (85 MB) 15.9, 5.4, and with 8-bit columns (118 MB) 24.1, 4.9 (two kernels 33.3); one row of 2048 3.3 us, a launch, a load and a store.
 //
 // Back: 8224 x 2048 to bf16 (43 MB) 9.2 us, 4.6 TB/s.
 #include <algorithm>
 
 #include "block_norm.hpp"
 #include "fp4_blocks.hpp"
+#include "fp8_blocks.hpp"
 
 namespace {
 
@@ -23,7 +26,7 @@ struct Quant4Params {
     const void* x;
     long long ldx;
     uint8_t *codes, *codes_t;      // [M, ldc bytes], [K, ldt bytes]; null: not wanted
-    uint32_t *scales, *scales_t;   // words of four bytes: [K / 128][lds], [M / 128][ldst]
+    uint32_t *scales, *scales_t;   // words of four bytes: [K / 128][lds], [M / 128][ldst] (8-bit columns: bytes)
     long long ldc, lds, ldt, ldst;
     int M, K, kb;                  // kb: tiles along K (256-value rows: an even number)
     int vec;                       // 16-byte loads fit
@@ -40,9 +43,11 @@ __device__ __forceinline__ uint32_t max4(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-template <class TX, bool BLOCK>
+// T8: the columns' codes are 8-bit ones.
+template <class TX, bool BLOCK, bool T8>
 __global__ __launch_bounds__(512) void gdn_fp4_quantize_kernel(Quant4Params p) {
-    constexpr int RT = 4, PITCH = 68;  // rows of a thread; bytes of a transposed row in LDS (17 words: 16 lanes' columns on 8 banks)
+    constexpr int RT = 4, PITCH = T8 ? 128 : 68;  // rows of a thread; bytes of a transposed row in LDS (17 words: 16 lanes' columns on 8 banks)
+    static_assert(!(BLOCK && T8), "8-bit columns are blocks of 1 x 128");
     __shared__ __attribute__((aligned(16))) unsigned char tile[128 * PITCH];
     __shared__ __attribute__((aligned(16))) uint32_t most[32][BLOCK ? 4 : 132];
     __shared__ __attribute__((aligned(16))) uint32_t bytes[4][132];
@@ -128,7 +133,16 @@ __global__ __launch_bounds__(512) void gdn_fp4_quantize_kernel(Quant4Params p) {
         *reinterpret_cast<u32x4*>(&most[rg][8 * cg]) = w[0];
         *reinterpret_cast<u32x4*>(&most[rg][8 * cg + 4]) = w[1];
         __syncthreads();
-        {
+        if constexpr (T8) {
+            if (tid < 128) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) m = max(m, most[i][tid]);
+                m = Fp8<GDN_E4M3>::scale_byte(m);
+                bytes[0][tid] = m;
+                if (k0 + tid < p.K) reinterpret_cast<uint8_t*>(p.scales_t)[mt * p.ldst + k0 + tid] = static_cast<uint8_t>(m);
+            }
+        } else {
             const int col = tid & 127, q = tid >> 7;
             uint32_t m = 0;
 #pragma unroll
@@ -136,10 +150,28 @@ __global__ __launch_bounds__(512) void gdn_fp4_quantize_kernel(Quant4Params p) {
             bytes[q][col] = fp4_scale_byte(m);
         }
         __syncthreads();
-        if (tid < 128 && k0 + tid < p.K)
+        if (!T8 && tid < 128 && k0 + tid < p.K)
             p.scales_t[mt * p.ldst + k0 + tid] = bytes[0][tid] | bytes[1][tid] << 8 | bytes[2][tid] << 16 | bytes[3][tid] << 24;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) colb[j] = bytes[rg >> 3][8 * cg + j];
+        for (int j = 0; j < 8; ++j) colb[j] = bytes[T8 ? 0 : rg >> 3][8 * cg + j];
+    }
+    if constexpr (T8) {
+        // Row k of the transposed tile holds its 4-byte piece q (rows m0 + 4 q ..) at slot
+        // q ^ 4 (k / 8 % 8): the 16 lanes of a row group write to different banks, and 16
+        // bytes stay together.
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint32_t*>(tile + (8 * cg + j) * PITCH + 4 * (rg ^ (4 * (cg & 7)))) =
+                Fp8<GDN_E4M3>::codes4(f[0][j], f[1][j], f[2][j], f[3][j], Fp8<GDN_E4M3>::inverse(colb[j]), colb[j] == 0xffu);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int k = 64 * i + tid / 8;
+            if (k0 + k < p.K)
+                *reinterpret_cast<u32x4*>(p.codes_t + (k0 + k) * p.ldt + m0 + 16 * (tid & 7)) =
+                    *reinterpret_cast<const u32x4*>(tile + k * PITCH + 16 * ((tid & 7) ^ (k / 8 & 7)));
+        }
+        return;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -223,12 +255,42 @@ extern "C" int gdn_fp4_quantize_hip(const void* x, int64_t ldx, int type_x, int6
     p.codes_t = codes_t, p.scales_t = reinterpret_cast<uint32_t*>(scales_t), p.ldt = ldt, p.ldst = ldst;
     p.vec = K % 8 == 0 && vec_rows(x, ldx, type_x);
     const auto launch = [&](auto tx, auto blk) {
-        hipLaunchKernelGGL((gdn_fp4_quantize_kernel<decltype(tx), decltype(blk)::value>), dim3(static_cast<unsigned>(tiles_m * KB)),
+        hipLaunchKernelGGL((gdn_fp4_quantize_kernel<decltype(tx), decltype(blk)::value, false>), dim3(static_cast<unsigned>(tiles_m * KB)),
                            dim3(512), 0, static_cast<hipStream_t>(stream), p);
         return gdn_host::check_launch("gdn_fp4_quantize_kernel");
     };
     const auto of_type = [&](auto blk) { return type_x == GDN_F32 ? launch(0.f, blk) : launch(bf16(), blk); };
     return block_rows == 32 ? of_type(std::true_type{}) : of_type(std::false_type{});
+}
+
+extern "C" int gdn_fp4_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, uint8_t* codes, int64_t ldc, uint8_t* scales,
+                                        int64_t lds, uint8_t* codes_t, int64_t ldt, uint8_t* scales_t, int64_t ldst, void* stream) {
+    using gdn_host::aligned;
+    using gdn_host::fail;
+    if (M < 0 || K < 0) return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_fp8_quantize: M=%lld K=%lld", (long long)M, (long long)K);
+    if (type_x != GDN_BF16 && type_x != GDN_F32) return fail(GDN_ERR_UNSUPPORTED, "fp4_fp8_quantize: type %d of x", type_x);
+    const int64_t MB = (M + kTile - 1) / kTile, KB = (K + kFp4Row - 1) / kFp4Row * 2;
+    if (M > 0x7fffffffLL - kFp4Row || K > 0x7fffffffLL - kFp4Row || MB * KB > 0x7fffffffLL || !gdn_host::grid_fits(MB * KB, 512))
+        return fail(GDN_ERR_UNSUPPORTED, "fp4_fp8_quantize: problem too large");
+    if (M == 0 || K == 0) return GDN_OK;
+    if (!x || !aligned(x, type_bytes(type_x)) || ldx < K) return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_fp8_quantize: x null, unaligned or ldx < K");
+    if (!codes || !scales || !aligned(codes, 16) || ldc % 16 != 0 || ldc < KB * kTile / 2 || !aligned(scales, 4) || lds < M)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_fp8_quantize: codes [M, ldc >= %lld bytes] with 16-byte rows, scales [%lld, lds >= %lld, 4] at 4 bytes",
+                    (long long)(KB * kTile / 2), (long long)KB, (long long)M);
+    if (!codes_t || !scales_t || !aligned(codes_t, 16) || ldt % 16 != 0 || ldt < MB * kTile || ldst < K)
+        return fail(GDN_ERR_INVALID_ARGUMENT, "fp4_fp8_quantize: codes_t [K, ldt >= %lld] with 16-byte rows, scales_t [%lld, ldst >= %lld]",
+                    (long long)(MB * kTile), (long long)MB, (long long)K);
+    Quant4Params p = {};
+    p.x = x, p.ldx = ldx, p.M = static_cast<int>(M), p.K = static_cast<int>(K), p.kb = static_cast<int>(KB);
+    p.codes = codes, p.scales = reinterpret_cast<uint32_t*>(scales), p.ldc = ldc, p.lds = lds;
+    p.codes_t = codes_t, p.scales_t = reinterpret_cast<uint32_t*>(scales_t), p.ldt = ldt, p.ldst = ldst;
+    p.vec = K % 8 == 0 && vec_rows(x, ldx, type_x);
+    const dim3 grid(static_cast<unsigned>(MB * KB));
+    if (type_x == GDN_F32)
+        hipLaunchKernelGGL((gdn_fp4_quantize_kernel<float, false, true>), grid, dim3(512), 0, static_cast<hipStream_t>(stream), p);
+    else
+        hipLaunchKernelGGL((gdn_fp4_quantize_kernel<bf16, false, true>), grid, dim3(512), 0, static_cast<hipStream_t>(stream), p);
+    return gdn_host::check_launch("gdn_fp4_quantize_kernel");
 }
 
 extern "C" int gdn_fp4_dequantize_hip(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, void* out, int64_t ldo,

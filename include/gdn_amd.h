@@ -35,6 +35,7 @@
  *   gdn_fp8_quantize_hip,     <- no reference counterpart (8-bit projections)
  *   gdn_fp8_matmul_hip
  *   gdn_fp4_quantize_hip,     <- no reference counterpart (4-bit weights)
+ *   gdn_fp4_fp8_quantize_hip,
  *   gdn_fp4_dequantize_hip,
  *   gdn_fp4_matmul_hip
  *   gdn_grad_norm_hip,        <- no reference counterpart (the reference does not train)
@@ -478,6 +479,16 @@ int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_
 int gdn_fp4_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, int block_rows, uint8_t* codes,
                          int64_t ldc, uint8_t* scales, int64_t lds, uint8_t* codes_t, int64_t ldt, uint8_t* scales_t,
                          int64_t ldst, void* stream);
+
+/*
+ * Both from one read of x: e2m1 codes along its rows, in blocks of 1 x 32 (codes and
+ * scales as gdn_fp4_quantize_hip writes them), and e4m3 codes along its columns, in
+ * blocks of 128 (codes_t [K, ldt >= M up to the next multiple of 128] and scales_t [M /
+ * 128, ldst >= K] as gdn_fp8_quantize_hip writes them).
+ */
+int gdn_fp4_fp8_quantize_hip(const void* x, int64_t ldx, int type_x, int64_t M, int64_t K, uint8_t* codes, int64_t ldc,
+                             uint8_t* scales, int64_t lds, uint8_t* codes_t, int64_t ldt, uint8_t* scales_t, int64_t ldst,
+                             void* stream);
 
 /*
  * What e2m1 codes [M, ldc bytes] with scales [K / 128, lds >= M, 4] stand for: out [M,

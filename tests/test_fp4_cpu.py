@@ -36,6 +36,25 @@ def test_quantize_refusals(bad, match):
         _quant(**bad)
 
 
+def _quant48(**k):
+    a = dict(x=FAKE, ldx=300, type=BF, M=200, K=300, codes=FAKE, ldc=256, scales=FAKE, lds=200, codes_t=FAKE, ldt=256, scales_t=FAKE, ldst=300, stream=None)
+    assert set(k) <= set(a)
+    a.update(k)
+    abi.call("gdn_fp4_fp8_quantize_hip", *a.values())
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(M=-1), "INVALID_ARGUMENT"), (dict(type=2), "type 2"), (dict(M=1 << 31), "too large"), (dict(K=1 << 31), "too large"), (dict(x=None), "null"),
+    (dict(ldx=299), "ldx"), (dict(x=FAKE + 1), "unaligned"), (dict(codes=None), "codes "), (dict(ldc=240), "codes "), (dict(lds=199), "codes "),
+    (dict(scales=FAKE + 2), "codes "), (dict(codes_t=None), "codes_t"), (dict(codes_t=FAKE + 8), "codes_t"), (dict(ldt=240), "codes_t"),
+    (dict(ldt=264), "codes_t"), (dict(ldst=299), "codes_t"), (dict(scales_t=None), "codes_t")])
+def test_quantize_to_both_formats_refusals(bad, match):
+    with pytest.raises(GdnError, match=match):
+        _quant48(**bad)
+    _quant48(M=0)
+    _quant48(K=0)
+
+
 def _dequant(**k):
     a = dict(codes=FAKE, ldc=152, scales=FAKE, lds=200, out=FAKE, ldo=300, to=BF, M=200, K=300, stream=None)
     assert set(k) <= set(a)

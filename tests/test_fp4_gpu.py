@@ -118,6 +118,35 @@ def test_quantize_leaves_what_lies_behind(dev, M, K, block):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 2048), (3, 130), (77, 1000), (128, 128), (129, 384), (300, 513), (260, 8), (1030, 1300), (0, 256), (5, 0)])
+def test_quantize_to_both_formats(exts, dev, M, K, dtype):
+    """4-bit codes along the rows and 8-bit ones along the columns, from one read: what two give."""
+    g = torch.Generator().manual_seed(M + 7 * K)
+    x = (torch.randn(M, K, generator=g) * torch.exp2(torch.randint(-30, 30, (M, 1), generator=g).float())).to(dev, dtype)
+    if M > 100:
+        x[3, 5], x[40, 7], x[M - 1, K - 1] = float("nan"), float("inf"), 0.0
+        x[:, 6] = 0
+    for t in (x, torch.cat([x, x], 1)[:, :K], x[::2]):
+        got = exts["proj"].fp4_fp8_quantize(t)
+        want = exts["proj"].fp4_quantize(t) + exts["proj"].fp8_quantize(t, rows=False, columns=True)
+        for a, b in zip(got, want):
+            assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            assert a.stride() == b.stride() or a.numel() == 0
+
+
+def test_quantize_to_both_formats_leaves_what_lies_behind(dev):
+    M, K, ldc, lds, ldt, ldst = 130, 300, 272, 136, 272, 310
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(3)).to(dev)
+    full = lambda *n: torch.full(n, 0x5a, dtype=torch.uint8, device=dev)  # noqa: E731
+    codes, scales, codes_t, scales_t = full(M + 1, ldc), full(4, lds, 4), full(K + 1, ldt), full(2, ldst)
+    abi.call("gdn_fp4_fp8_quantize_hip", x.data_ptr(), K, 1, M, K, codes.data_ptr(), ldc, scales.data_ptr(), lds, codes_t.data_ptr(), ldt,
+             scales_t.data_ptr(), ldst, torch.cuda.current_stream().cuda_stream)
+    assert (codes[M:] == 0x5a).all() and (codes[:, 256:] == 0x5a).all() and (scales[:, M:] == 0x5a).all()
+    assert (codes_t[K:] == 0x5a).all() and (codes_t[:, 256:] == 0x5a).all() and (scales_t[:, K:] == 0x5a).all()
+    assert (codes[:M, 150:256] == 0).all() and (codes_t[:K, M:256] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("M,K", [(1, 256), (3, 256), (16, 512), (70, 2048)])
 def test_dequantize(exts, dev, M, K, dtype):
     """Every code with every scale; bf16's and fp32's largest numbers are the same, give or take a rounding."""
