@@ -213,7 +213,7 @@ def grad_norm(grads):
 
     grads: a list of bf16 and fp32 tensors on one GPU, such as ``[p.grad for p in
     parameters if p.grad is not None]``; None among them is left out, and without any
-    the norm is 0.
+    the norm is 0.  No gradients of the norm are recorded.
     """
     grads = [g for g in grads if g is not None]
     return native_extension().grads.norm(grads) if grads else torch.zeros(())
@@ -226,7 +226,7 @@ def clip_grad_norm(grads, max_norm, out=None):
     the norm before.  None among the gradients is left out.
 
     Nothing is read back to the host, so the call can be captured into a graph.  A norm
-    that is NaN makes every result NaN.
+    that is NaN makes every result NaN.  No gradients are recorded.
     """
     if out is not None:
         if len(out) != len(grads):

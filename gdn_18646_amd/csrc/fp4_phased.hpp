@@ -12,8 +12,8 @@
 // Against the 256 x 128 tile of fp4_tiles.hpp, where both fill the CUs: 8192 x 8192 x 8192
 // 420 us (2.6 PFLOP/s) instead of 470, 16384 x 6144 x 2048 166 and 183, 1500 x 8224 x 2048
 // (198 tiles, one round) 30 and 35.  A block of K takes 1.2-1.3 us, of which the matrix
-// cores need 0.9; tiles of 160 and 192 tokens and of 128 columns were no faster than the
-// 256 x 128 one.
+// cores need 0.9; tiles of 160 and 192 tokens and of 128 columns were slower than the
+// 256 x 128 one or within 3% of it.
 #pragma once
 
 #include "fp4_tiles.hpp"

@@ -4,6 +4,7 @@ block norm, projection, backward, clipping; and the serving run on the same kern
 import pytest
 import torch
 import torch.utils.checkpoint
+from torch.autograd import forward_ad
 
 from gdn_18646_amd.blocks import Fp4Weight, block_norm, clip_grad_norm, fp4_linear
 from tests.fp4 import E2, E4, E5, quantize64, values
@@ -287,3 +288,21 @@ def test_one_axis_and_another_stream(dev):
     side.synchronize()
     assert y.shape == (128,) and dx.shape == (256,) and torch.equal(y, y2[0]) and torch.equal(z, y)
     assert torch.equal(dx, want[0][0]) and torch.equal(dw, want[1])
+
+
+@pytest.mark.parametrize("activations", [E4, E2], ids=["e4m3", "e2m1"])
+def test_checkpoints_saved_tensors_and_transforms(dev, activations):
+    x, w = _rand((70, 512), torch.bfloat16, dev, 1), _rand((384, 512), torch.float32, dev, 2, 0.05)
+    dy = _rand((70, 384), torch.bfloat16, dev, 3, grad=False)
+    want = torch.autograd.grad(fp4_linear(x, w, activations), (x, w), dy)
+    again = torch.utils.checkpoint.checkpoint(fp4_linear, x, w, activations, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, (x, w), dy), want))
+    with torch.autograd.graph.save_on_cpu():
+        y = fp4_linear(x, w, activations)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), want))
+    with torch.inference_mode():
+        assert torch.equal(fp4_linear(x, w, activations), y.detach())
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda t: fp4_linear(t, w, activations).float().sum())(x.detach())
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+        fp4_linear(forward_ad.make_dual(x.detach(), torch.ones_like(x)), w, activations)
