@@ -307,7 +307,7 @@ __device__ __forceinline__ void store(const gdn_fp4::MatmulParams& p, const f32x
     });
 }
 // The same of a tile inside the result: at least TL::WNT * 4 stores, whatever the lane.
-// They go past the caches, which the operands need: a training step of 16384 tokens
+// They go past the caches, which the operands need: a training step of 8192 x 2048 x 4096
 // (three products among quantisations) takes 219 us, with ordinary stores 230.
 template <class TL, bool OUT32>
 __device__ __forceinline__ void store_inside(const gdn_fp4::MatmulParams& p, const f32x4 (&acc)[TL::WMT][TL::WNT], int R0, int C0) {
