@@ -542,8 +542,9 @@ int gdn_grad_norm_hip(const gdn_grad_t* grads, int64_t count, float* norm, void*
                       void* stream);
 
 /*
- * The same, and out = grad min(1, max_norm / (norm + 1e-6)) for each tensor, rounded
- * once to type_out; out may be grad itself (then of its type; not written where the
+ * The same, and out = grad min(1, max_norm / (norm + 1e-6)) for each tensor: the factor
+ * from the 64-bit sums and the product each rounded to 24 bits of mantissa (a factor below
+ * fp32's normal numbers keeps them), then to type_out; out may be grad itself (then of its type; not written where the
  * factor is 1) and lies apart from the other tensors, or the call is refused.  A norm
  * that is NaN makes every result NaN, an infinite one zeros and NaN.  max_norm >= 0.
  */

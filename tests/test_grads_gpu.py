@@ -205,3 +205,23 @@ def test_results_of_gradients_with_none_among_them(dev):
         clip_grad_norm(grads, 0.5, out=outs[:2])
     with pytest.raises(ValueError, match="0 gradients and 3 results"):
         clip_grad_norm([], 0.5, out=outs)
+
+
+@pytest.mark.parametrize("types", [(BF,), (F32,), (BF, F32)], ids=["bf16", "fp32", "mixed"])
+@pytest.mark.parametrize("most", [1e30, 1.0, 1e-4, 1e-6, 1e-20, 1e-38, 0.0])
+def test_factors_below_32_bit_numbers(dev, most, types):
+    """Clipped values where the factor is no normal number of 32 bits, held to what they should
+    be: the factor's rounding, the product's, and half the type's step (of numbers below 2^-126
+    half of the least one, 2^-150, and as much again for rounding twice; bf16's is 2^-134)."""
+    g = torch.Generator().manual_seed(7)
+    grads = [torch.full((200_003,), 3e38, device=dev).to(types[0]), (torch.randn(5001, generator=g) * 10.0 ** torch.randint(-30, 38, (5001,), generator=g)).to(types[-1]).to(dev)]
+    ref = _norm64(grads)
+    assert ref > 1e41
+    for name, out in (("into bf16", BF), ("into fp32", F32), ("in place", None)):
+        here = [t.clone() for t in grads]
+        outs = None if out is None else [torch.full(t.shape, 7.0, dtype=out, device=dev) for t in grads]
+        assert clip_grad_norm(here, most, out=outs).item() == float("inf")  # in 32 bits; the factor has all of it
+        for t, o in zip(grads, here if outs is None else outs):
+            want = t.double() * (most / (ref + 1e-6))
+            least = 2.0 ** -134 if o.dtype == BF else 2.0 ** -150
+            assert ((o.double() - want).abs() <= (HALF[o.dtype] + 2.0 ** -23) * want.abs() + least + 2.0 ** -150).all(), name
