@@ -226,7 +226,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     the norm before.  None among the gradients is left out.
 
     Nothing is read back to the host, so the call can be captured into a graph.  A norm
-    that is NaN makes every result NaN.  No gradients are recorded.
+    that is NaN makes every result NaN; an infinite gradient makes the others 0, or, where
+    max_norm is infinite too, NaN.  No gradients are recorded.
     """
     if out is not None:
         if len(out) != len(grads):

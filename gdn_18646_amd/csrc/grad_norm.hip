@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void gdn_clip_kernel(Table t, const doubl
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(root);
     const double q = max_norm / (root + 1e-6);
     int e = 0;
-    const float f = q >= 1. ? 1.f : static_cast<float>(q < 0x1p-126 ? frexp(q, &e) : q);  // NaN stays NaN
+    const float f = q >= 1. ? 1.f : static_cast<float>(q < 0x1p-126 ? frexp(q, &e) : q);  // NaN stays NaN, and inf / inf is one
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const int i = tensor_of(t, c);
         const long long at = static_cast<long long>(c - t.first[i]) * kChunk;

@@ -544,9 +544,13 @@ int gdn_grad_norm_hip(const gdn_grad_t* grads, int64_t count, float* norm, void*
 /*
  * The same, and out = grad min(1, max_norm / (norm + 1e-6)) for each tensor: the factor
  * from the 64-bit sums and the product each rounded to 24 bits of mantissa (a factor below
- * fp32's normal numbers keeps them), then to type_out; out may be grad itself (then of its type; not written where the
- * factor is 1) and lies apart from the other tensors, or the call is refused.  A norm
- * that is NaN makes every result NaN, an infinite one zeros and NaN.  max_norm >= 0.
+ * fp32's normal numbers keeps them), then to type_out; out may be grad itself (then of its
+ * type; not written where the factor is 1) and lies apart from the other tensors, or the
+ * call is refused.  norm and workspace lie apart from all of them.  A norm that is NaN makes
+ * every result NaN.  An infinity among the gradients makes the factor 0: zeros, and NaN
+ * where it stands; with an infinite max_norm, of which the factor is NaN, NaN everywhere.
+ * (A norm that is infinite in 32 bits alone is not meant: its factor is as any other.)
+ * max_norm >= 0.
  */
 int gdn_clip_grad_norm_hip(const gdn_grad_t* grads, int64_t count, double max_norm, float* norm, void* workspace,
                            size_t workspace_bytes, void* stream);

@@ -225,3 +225,17 @@ def test_factors_below_32_bit_numbers(dev, most, types):
             want = t.double() * (most / (ref + 1e-6))
             least = 2.0 ** -134 if o.dtype == BF else 2.0 ** -150
             assert ((o.double() - want).abs() <= (HALF[o.dtype] + 2.0 ** -23) * want.abs() + least + 2.0 ** -150).all(), name
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_infinite_norm_and_infinite_limit(dev, bad):
+    """max_norm / norm is inf / inf: NaN, as the formula has it; without a limit alone nothing changes."""
+    grads = [torch.full((1000,), 2.0, device=dev), torch.full((33,), -3.0, dtype=BF, device=dev)]
+    want, outs = [g.clone() for g in grads], [torch.empty_like(g, dtype=F32) for g in grads]
+    clip_grad_norm(grads, float("inf"))
+    assert all(torch.equal(g, w) for g, w in zip(grads, want))
+    grads[0][7] = bad
+    norm = clip_grad_norm(grads, float("inf"), out=outs)
+    assert norm.isnan() if math.isnan(bad) else norm.item() == float("inf")
+    clip_grad_norm(grads, float("inf"))
+    assert all(t.isnan().all() for t in grads + outs)
