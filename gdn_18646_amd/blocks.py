@@ -213,7 +213,7 @@ def grad_norm(grads):
 
     grads: a list of bf16 and fp32 tensors on one GPU, such as ``[p.grad for p in
     parameters if p.grad is not None]``; None among them is left out, and without any
-    the norm is 0.  No gradients of the norm are recorded.
+    the norm is 0.  No gradients of the norm are recorded; a forward-mode tangent raises.
     """
     grads = [g for g in grads if g is not None]
     return native_extension().grads.norm(grads) if grads else torch.zeros(())
@@ -227,7 +227,8 @@ def clip_grad_norm(grads, max_norm, out=None):
 
     Nothing is read back to the host, so the call can be captured into a graph.  A norm
     that is NaN makes every result NaN; an infinite gradient makes the others 0, or, where
-    max_norm is infinite too, NaN.  No gradients are recorded.
+    max_norm is infinite too, NaN.  No gradients are recorded; a forward-mode tangent
+    raises.
     """
     if out is not None:
         if len(out) != len(grads):

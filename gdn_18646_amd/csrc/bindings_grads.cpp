@@ -7,8 +7,10 @@
 
 namespace {
 
-// A tensor whose elements fill one piece of memory, in any order.
+// A tensor whose elements fill one piece of memory, in any order, and stand for
+// themselves alone: a forward-mode tangent would not be carried along.
 void check_dense(const Tensor& t, const Tensor& first, const char* name, size_t i) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), name, "[", i, "] has a forward-mode tangent, which the norm and the clipping do not carry");
     TORCH_CHECK(t.is_cuda() && t.device() == first.device(), name, "[", i, "] must be a GPU tensor on the others' device");
     TORCH_CHECK(t.is_non_overlapping_and_dense(), name, "[", i, "] must fill its memory without gaps or overlaps");
 }

@@ -7,6 +7,7 @@ import re
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from gdn_18646_amd import abi, blocks, compile_kernels, native_extension
 from gdn_18646_amd.abi import GdnError, GradTensor
@@ -161,6 +162,18 @@ def test_layers_check_their_arguments():
     with pytest.raises(ValueError, match="weight"):
         blocks.Fp4Weight(w[0])
     assert blocks.grad_norm([]).item() == 0 and blocks.clip_grad_norm([None], 1.0).item() == 0
+
+
+def test_tangents_of_gradients_are_not_dropped():
+    t, plain = torch.ones(4, 5), torch.ones(4, 5)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(4, 5), t)
+        for call in (lambda: blocks.grad_norm([dual]), lambda: blocks.grad_norm([dual, plain]), lambda: blocks.clip_grad_norm([dual], 0.5),
+                     lambda: blocks.clip_grad_norm([dual, plain], 0.5)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward-mode tangent"):
+                    call()
+        assert torch.equal(forward_ad.unpack_dual(dual).primal, plain)
 
 
 def test_the_definition_that_the_kernels_are_held_to():

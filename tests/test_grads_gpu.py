@@ -9,6 +9,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from gdn_18646_amd import abi, native_extension
 from gdn_18646_amd.blocks import clip_grad_norm, grad_norm
@@ -239,3 +240,21 @@ def test_infinite_norm_and_infinite_limit(dev, bad):
     assert norm.isnan() if math.isnan(bad) else norm.item() == float("inf")
     clip_grad_norm(grads, float("inf"))
     assert all(t.isnan().all() for t in grads + outs)
+
+
+def test_tangents_and_transforms_are_refused(dev):
+    """Neither a dual tensor's tangent nor a transform is passed over in silence, in what is read or written."""
+    a, b, t = torch.ones(40, device=dev), torch.ones(40, dtype=BF, device=dev), torch.ones(40, device=dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(40, device=dev), t)
+        for call in (lambda: grad_norm([dual]), lambda: grad_norm([b, dual]), lambda: clip_grad_norm([b, dual], 0.5), lambda: clip_grad_norm([dual], 0.5, out=[a]),
+                     lambda: clip_grad_norm([a], 0.5, out=[dual])):
+            with pytest.raises(RuntimeError, match="forward-mode tangent"):
+                call()
+        assert (forward_ad.unpack_dual(dual).primal == 1).all()
+        _check_norm(grad_norm([a, b]), [a, b])  # operands without one are taken
+    assert (a == 1).all() and (b == 1).all()
+    for f in (lambda: torch.func.jvp(lambda x: grad_norm([x]), (a,), (t,)), lambda: torch.func.grad(lambda x: grad_norm([x]))(a),
+              lambda: torch.func.vmap(lambda x: grad_norm([x]))(a.view(5, 8))):
+        with pytest.raises(RuntimeError, match="tangent|storage"):
+            f()
