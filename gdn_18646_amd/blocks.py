@@ -101,16 +101,25 @@ def _adjacent(x):
     return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
 
 
+def _plain(weight):
+    """weight [N, K] as it is quantised once: without its graph; a forward-mode tangent,
+    which the codes do not carry, raises."""
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+    if forward_ad.unpack_dual(weight).tangent is not None:
+        raise RuntimeError("a weight that is quantised once has a forward-mode tangent")
+    return _adjacent(weight.detach())
+
+
 class Fp8Weight:
     """A weight [N, K] (bf16 or fp32) as e4m3 codes with a scale for each 128 x 128
     block: ``codes`` / ``scales`` for x W^T and, with ``transposed``, ``codes_t`` /
     ``scales_t`` for the gradient of x."""
 
     def __init__(self, weight, transposed=False):
-        if weight.dim() != 2:
-            raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+        w = _plain(weight)
         self.shape = tuple(weight.shape)
-        out = compile_kernels()["proj"].fp8_quantize(_adjacent(weight.detach()), block_rows=BLOCK, rows=True, columns=transposed)
+        out = compile_kernels()["proj"].fp8_quantize(w, block_rows=BLOCK, rows=True, columns=transposed)
         self.codes, self.scales = out[:2]
         self.codes_t, self.scales_t = out[2:] if transposed else (None, None)
 
@@ -172,10 +181,9 @@ class Fp4Weight:
     along each product's own sum."""
 
     def __init__(self, weight, transposed=False, block_rows=32):
-        if weight.dim() != 2:
-            raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+        w = _plain(weight)
         self.shape = tuple(weight.shape)
-        out = compile_kernels()["proj"].fp4_quantize(_adjacent(weight.detach()), block_rows=block_rows, rows=True, columns=transposed)
+        out = compile_kernels()["proj"].fp4_quantize(w, block_rows=block_rows, rows=True, columns=transposed)
         self.codes, self.scales = out[:2]
         self.codes_t, self.scales_t = out[2:] if transposed else (None, None)
 

@@ -76,3 +76,17 @@ def test_a_backward_pass_names_the_nodes_that_it_reaches():
         loss.backward() if asked is None else torch.autograd.grad(loss, asked)
         assert seen == [nodes]
     assert native_extension()._backward_nodes() == []
+
+
+@pytest.mark.parametrize("kind", [blocks.Fp8Weight, blocks.Fp4Weight])
+def test_tangents_of_weights_are_not_dropped(kind):
+    """Codes carry no tangent: a dual weight is turned down before anything else."""
+    w, t = torch.ones(64, 256, dtype=torch.bfloat16), torch.ones(64, 256, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward-mode tangent"):
+                kind(forward_ad.make_dual(w, t))
+        with pytest.raises(RuntimeError, match="GPU tensor"):
+            kind(w)
+    with pytest.raises(ValueError, match="weight must be"):
+        kind(w[0])
