@@ -43,10 +43,12 @@ __device__ __forceinline__ i32x8 codes4(const u32x4 v) {  // 32 4-bit codes: hal
 // supplies (of 8-bit ones all four lanes of a row have the same).  127 is 1.
 //
 // The sum of a block of 32 products of 4-bit codes is exact, and four blocks and the
-// accumulator are added with an error of at most 2^-21 of the largest product
-// (measured; a sum in fp32 has about that), so fp32 results are summed here too.  Of
-// products with 8-bit codes the instruction drops what lies below about 2^-17 of the
-// largest: good for bf16 results alone.
+// accumulator are added with an error of at most 2^-21 of the largest of the products, the
+// four sums, the accumulator and the result (measured: 2^-22.2 over 10^7 results, scales up
+// to 2^78 apart, terms that cancel or do not; a sum of 129 terms in fp32 may be off by 2^-17
+// of its largest partial sum), so fp32 results are summed here too.  Of products with 8-bit
+// codes the instruction drops what lies below about 2^-17 of the largest: good for bf16
+// results alone.
 template <int FA, int SX, int SW>
 __device__ __forceinline__ f32x4 mfma_fp4(const i32x8 x, const i32x8 w, const f32x4 c, uint32_t sx, uint32_t sw) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, c, FA == GDN_E2M1 ? 4 : FA, 4, SX, static_cast<int>(sx), SW,

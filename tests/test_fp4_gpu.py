@@ -386,6 +386,42 @@ def test_product_of_large_terms_that_cancel(exts, dev, M, N, K):
         _check(_product(exts, a, b, out), a, b)
 
 
+@pytest.mark.parametrize("kind", ["cancel", "one sign"])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 512), (2, 70, 2048), (16, 129, 1280), (48, 2048, 4096), (70, 2048, 512), (300, 1030, 512), (520, 4090, 512),
+                                   (2600, 2040, 512), (4096, 4118, 256)])
+def test_product_of_4_bit_codes_loses_little_beside_the_largest(exts, dev, M, N, K, kind):
+    """One instruction (128 products and the accumulator) is off by at most 2^-21 of the
+    largest of: its products, their four sums of 32, the accumulator, the result.  No
+    accumulator or result is larger than the sum of the instructions' magnitudes, nor any
+    of at most eight partial sums that are added in fp32 (2^-24 each).  Scales lie up to
+    2^78 apart; in every block of 128 products of 36 and -36 times the scales cancel, or
+    none do."""
+    g = torch.Generator().manual_seed(M + K)
+    a, b = _operands(M, N, K, E2, dev, lo=107, hi=147)
+    ca, cb = (torch.randint(0, 16, (n, K), generator=g) for n in (M, N))
+    if kind == "one sign":
+        ca, cb = ca & 7, cb & 7
+    else:
+        for k in range(0, K, 128):
+            at = k + 32 * torch.randint(0, 4, (1,), generator=g) + torch.randperm(32, generator=g)[:2]
+            ca[:, at], cb[:, at[0]], cb[:, at[1]] = 7, 7, 15
+    sa, sb = (_bits(t.scales.flatten(1).contiguous()) for t in (a, b))
+    a.codes, b.codes = pack(ca).to(dev), pack(cb).to(dev)
+    a.values, b.values = values(ca, sa).to(dev), values(cb, sb).to(dev)
+    ref, sums, largest = (torch.zeros(M, N, dtype=torch.float64, device=dev) for _ in range(3))
+    for k in range(0, K, 128):
+        parts = [a.values[:, i:i + 32] @ b.values[:, i:i + 32].t() for i in range(k, k + 128, 32)]
+        # of 32 products the largest is no larger than the product of the largest two
+        tops = [a.values[:, i:i + 32].abs().amax(1)[:, None] * b.values[:, i:i + 32].abs().amax(1) for i in range(k, k + 128, 32)]
+        ref, sums = ref + sum(parts), sums + sum(parts).abs()
+        largest = largest + torch.stack([p.abs() for p in parts] + tops).amax(0)
+    tol = 2.0 ** -21 * (largest + (K / 128 + 1) * sums * (1 + 2.0 ** -10))
+    for out in (torch.float32, torch.bfloat16):
+        y = _product(exts, a, b, out).double()
+        far = (y - ref).abs() - tol - (2.0 ** -8 * (ref.abs() + tol) if out == torch.bfloat16 else 0)
+        assert not (far > 0).any() and torch.isfinite(y).all(), f"{(far > 0).sum().item()} values of {out}, the worst {far.max().item():.3g} past its bound"
+
+
 def test_quantised_operands_go_straight_in(exts, dev):
     """The codes of block_norm, fp8_quantize and fp4_quantize as they come, K no multiple of 256."""
     g = torch.Generator().manual_seed(8)
