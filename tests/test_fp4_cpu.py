@@ -242,6 +242,53 @@ def test_stream_tiles_keep_their_counted_waits(asm, tile):
         assert not any(re.search(r"\bglobal_load_(?!lds)|\bflat_|\bbuffer_", ln) for ln in lines[:last])
 
 
+def _stream_functions(asm, tile):
+    x8, cw, tw, wmt, wnt, ns, per = STREAM[tile]
+    text = asm[tile.split()[0]]
+    names = _kernels(text, "stream", "".join(("%dE" % x8, *(f"Li{v}E" for v in (cw, tw, wmt, wnt, ns, per)))))
+    assert len(names) == (1 if x8 else 2), names  # bf16 and fp32 results
+    return [_function(text, name) for name in names]
+
+
+@pytest.mark.parametrize("tile", STREAM)
+def test_a_tile_inside_the_result_has_the_stores_that_are_counted(asm, tile):
+    """The wait for a stage's copies lets the stores of a tile inside the result, 4 a token tile
+    at least, be under way; those past the caches are that tile's (the edges' are ordinary)."""
+    wnt = STREAM[tile][4]
+    for lines in _stream_functions(asm, tile):
+        stores = [ln for ln in lines if re.search(r"\bglobal_store_", ln)]
+        inside = [i for i, ln in enumerate(lines) if re.search(r"\bglobal_store_\w+ .*\bnt\b", ln)]
+        assert 4 * wnt <= len(inside) < len(stores)
+        # all of them in one piece without branches: a tile issues them all or none
+        assert not any(re.search(r"\bs_c?branch|^\.L", ln.strip()) for ln in lines[inside[0]:inside[-1]])
+
+
+@pytest.mark.parametrize("tile", STREAM)
+def test_stream_tiles_keep_their_counted_lds_wait(asm, tile):
+    """The barrier after which W's buffer is copied over waits for all LDS reads but the last
+    ones, which have to be of x: they lie behind products of the half slice, before which
+    all of W and its scales were read, and no branch lies between."""
+    x8, cw, tw, wmt, wnt, ns, per = STREAM[tile]
+    first = wnt // 4  # the token tile behind whose reads the barrier stands
+    for lines in _stream_functions(asm, tile):
+        ops = [ln.split(";")[0].strip() for ln in lines]
+        counted = [i for i, ln in enumerate(ops) if ln == "s_barrier" and (m := re.fullmatch(r"s_waitcnt lgkmcnt\((\d+)\)", ops[i - 1])) and m.group(1) != "0"]
+        assert len(counted) == 1, counted
+        at = counted[0] - 1
+        n = int(re.search(r"\((\d+)\)", ops[at]).group(1))
+        assert n == (first + 1) * (1 + x8)
+        start = max(i for i in range(at) if re.search(r"^s_c?branch|^\.L\w+:", ops[i]))
+        window = ops[start + 1:at]
+        products = [i for i, ln in enumerate(window) if ln.startswith("v_mfma")]
+        reads = [i for i, ln in enumerate(window) if ln.startswith("ds_")]
+        assert len(products) == (first + 1) * wmt and all(window[i].startswith("ds_read") for i in reads)
+        behind = [window[i] for i in reads if i > products[0]]
+        before = [window[i] for i in reads if i < products[0]]
+        assert len(behind) == n and all(ln.startswith("ds_read_b128") for ln in behind)
+        assert sum(ln.startswith("ds_read_b128") for ln in before) == wmt  # W's codes
+        assert len(before) > wmt                                          # and scales
+
+
 def test_the_phased_tile(asm):
     """No spills, scalar bases, the counted waits of its phases, and none of the compiler's own before its stores."""
     (name,) = re.findall(r"^(_Z\w*gdn_fp4_phased_kernel\w*):", asm["e4m3"], re.M)
