@@ -490,3 +490,105 @@ def test_on_another_stream_and_replayed(exts, dev):
         exts["proj"].fp4_matmul(*exts["proj"].fp8_quantize(w), wq, ws)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(y, eager))
+
+
+# Kernels of the product by size: a token or two, rings of small tiles, the stream's tiles (inside the
+# result and past it, with columns in a launch of their own), the phased ones.
+SPREAD = [(1, 300, 512, E2), (2, 9001, 384, E4), (5, 33, 512, E2), (33, 65, 256, E5), (300, 1030, 512, E2), (513, 2100, 256, E4), (1030, 2050, 512, E2),
+          (2600, 2040, 768, E4), (4096, 4118, 256, E2), (1490, 8210, 1408, E4)]
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,N,K,fa", SPREAD, ids=str)
+def test_product_into_wider_rows_at_odd_addresses(exts, dev, M, N, K, fa, out):
+    """Through the C ABI: results at any address of their type, in rows further apart than they
+    are long, have the same bits; what lies around them is left as it is."""
+    a, b = _operands(M, N, K, fa, dev)
+    want = _product(exts, a, b, out)
+    sa = a.scales
+    if fa != E2:  # as fp8_quantize lays them out
+        sa = torch.full((K // 128, up(M, 16)), 255, dtype=torch.uint8, device=dev)
+        sa[:, :M] = a.scales.view(torch.uint8).t()
+    for ldo, at in ((N + 3, 1), (N + 8, 5), (N, 3)):
+        buf = torch.full((at + M * ldo + 7,), 7.0, dtype=out, device=dev)
+        print(f"{M} x {N} x {K} {fa} {out} rows of {ldo} from {at}", flush=True)
+        abi.call("gdn_fp4_matmul_hip", a.codes.data_ptr(), a.codes.shape[1], {E4: 0, E5: 1, E2: 2}[fa], sa.data_ptr(), up(M, 16), b.codes.data_ptr(),
+                 b.codes.shape[1], b.scales.data_ptr(), up(N, 16), buf[at:].data_ptr(), ldo, 1 if out == torch.float32 else 0, M, N, K,
+                 torch.cuda.current_stream().cuda_stream)
+        rows = buf[at:at + M * ldo].view(M, ldo)
+        assert torch.equal(rows[:, :N], want)
+        assert (rows[:, N:] == 7).all() and (buf[:at] == 7).all() and (buf[at + M * ldo:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 37), (3, 256), (70, 1001), (33, 2048)])
+def test_dequantize_into_wider_rows_at_odd_addresses(exts, dev, M, K, dtype):
+    """The same of the way back."""
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(dev)
+    codes, scales = exts["proj"].fp4_quantize(x)
+    want = exts["proj"].fp4_dequantize(codes, scales, columns=K, dtype=dtype)
+    for ldo, at in ((K + 3, 1), (K + 9, 5), (K, 3)):
+        buf = torch.full((at + M * ldo + 7,), 77.0, dtype=dtype, device=dev)
+        abi.call("gdn_fp4_dequantize_hip", codes.data_ptr(), codes.shape[1], scales.data_ptr(), up(M, 16), buf[at:].data_ptr(), ldo,
+                 1 if dtype == torch.float32 else 0, M, K, torch.cuda.current_stream().cuda_stream)
+        rows = buf[at:at + M * ldo].view(M, ldo)
+        assert torch.equal(rows[:, :K], want)
+        assert (rows[:, K:] == 77).all() and (buf[:at] == 77).all() and (buf[at + M * ldo:] == 77).all()
+
+
+@pytest.mark.parametrize("M,N,K,fa,out", [(16500, 131101, 256, E2, torch.bfloat16), (16500, 131101, 1280, E4, torch.bfloat16), (16500, 65601, 256, E4, torch.float32),
+                                          (16500, 65601, 256, E2, torch.float32), (40, 54_000_011, 256, E2, torch.bfloat16)],
+                         ids=["stream", "phased", "ring", "stream fp32", "few rows"])
+def test_results_past_32_bits(exts, dev, M, N, K, fa, out):
+    """Results of more than 2^32 bytes, of codes whose sums (quarters below 2^14 in magnitude) are
+    exact in fp32: rows from all over them have the bits that they have alone, in columns from
+    all over them."""
+    g = torch.Generator(device=dev).manual_seed(M)
+    codes_b = torch.randint(0, 256, (N, K // 2), generator=g, device=dev, dtype=torch.uint8)
+    sb = torch.full((K // 128, up(N, 16), 4), 127, dtype=torch.uint8, device=dev).view(E8)[:, :N].transpose(0, 1)
+    if fa == E2:
+        codes_a = torch.randint(0, 256, (M, K // 2), generator=g, device=dev, dtype=torch.uint8).view(E2)
+        sa = torch.full((K // 128, up(M, 16), 4), 127, dtype=torch.uint8, device=dev).view(E8)[:, :M].transpose(0, 1)
+    else:  # 0, 1/2 .. 2 in magnitude
+        codes_a = (torch.randint(-4, 5, (M, K), generator=g, device=dev).float() / 2).to(fa)
+        sa = torch.full((K // 128, up(M, 16)), 127, dtype=torch.uint8, device=dev).view(E8)[:, :M].t()
+    y = exts["proj"].fp4_matmul(codes_a, sa, codes_b.view(E2), sb, out_dtype=out)
+    size = 4 if out == torch.float32 else 2
+    border = 2 ** 32 // size // N  # the row that 2^32 bytes end in
+    assert border < M
+    row = torch.tensor(sorted({0, 1, M // 3, M // 2, border, M - 2, M - 1}), device=dev)
+    col = torch.unique(torch.cat([torch.arange(0, N, max(1, N // 500), device=dev), torch.arange(max(0, N - 300), N, device=dev)]))
+    four = lambda bytes_: exts["proj"].fp4_dequantize(bytes_.view(E2), torch.full((len(bytes_), K // 32), 127, dtype=torch.uint8, device=dev).view(E8), dtype=torch.float32)  # noqa: E731
+    va, vb = four(codes_a.view(torch.uint8)[row]) if fa == E2 else codes_a.float()[row], four(codes_b[col])
+    want = (va.double() @ vb.double().t()).float().to(out)
+    assert torch.equal(y[row][:, col], want)
+
+
+def test_dequantized_values_past_32_bits(exts, dev):
+    """2.3 billion values, 4.6 GB of bf16."""
+    M, K = 140_000, 16384
+    codes, scales = torch.zeros(M, K // 2, dtype=torch.uint8, device=dev), torch.full((K // 128, up(M, 16), 4), 127, dtype=torch.uint8, device=dev)
+    rows = torch.tensor([0, 65535, 131071, 131072, M - 1], device=dev)
+    some = torch.randint(0, 256, (len(rows), K // 2), generator=torch.Generator().manual_seed(5)).to(torch.uint8).to(dev)
+    codes[rows] = some
+    s = scales.view(E8)[:, :M].transpose(0, 1)
+    v = exts["proj"].fp4_dequantize(codes.view(E2), s)
+    assert v.numel() * 2 > 2 ** 32 and torch.equal(v[rows], exts["proj"].fp4_dequantize(some.view(E2), s[:len(rows)]))
+    assert torch.count_nonzero(v).item() == torch.count_nonzero(v[rows]).item()
+
+
+@pytest.mark.parametrize("block", [1, 32])
+def test_quantized_values_past_32_bits(exts, dev, block):
+    """2.2 billion values, 4.3 GB of bf16: rows and columns from all over them have the codes that they have alone."""
+    M, K = 262_200, 8320
+    x = torch.randn(1024, K, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16).to(dev).repeat(257, 1)[:M]
+    x[-1, -1] = 40.0  # no period in the last row's or column's block
+    assert x.numel() * 2 > 2 ** 32
+    c, s, ct, st = exts["proj"].fp4_quantize(x, block_rows=block, rows=True, columns=True)
+    for lo, hi in ((0, 64), (131072, 131136), (261_952, M)):  # of whole blocks
+        part = exts["proj"].fp4_quantize(x[lo:hi].clone(), block_rows=block, rows=True, columns=True)
+        assert torch.equal(_bits(c[lo:hi]), _bits(part[0])) and torch.equal(_bits(s[lo:hi]), _bits(part[1]))
+        n = (hi - lo + 1) // 2
+        assert torch.equal(_bits(ct.view(torch.uint8)[:, lo // 2:lo // 2 + n]), _bits(part[2])[:, :n])
+        blocks_t = st.view(torch.uint8).flatten(1)[:, lo // 32:-(-hi // 32)]
+        assert torch.equal(blocks_t.cpu(), _bits(part[3]).flatten(1)[:, :blocks_t.shape[1]])

@@ -306,3 +306,22 @@ def test_checkpoints_saved_tensors_and_transforms(dev, activations):
         torch.func.grad(lambda t: fp4_linear(t, w, activations).float().sum())(x.detach())
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="jvp"):
         fp4_linear(forward_ad.make_dual(x.detach(), torch.ones_like(x)), w, activations)
+
+
+@pytest.mark.parametrize("activations", [E4, E2], ids=["e4m3", "e2m1"])
+@pytest.mark.parametrize("tx,tw", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)], ids=["bf16 by fp32", "fp32 by bf16"])
+@pytest.mark.parametrize("shape,N", [((2, 37, 256), 384), ((300, 130), 300), ((1, 640), 2048)], ids=str)
+def test_activations_and_weight_of_two_types(dev, shape, N, tx, tw, activations):
+    """y and dx have x's type, dw the weight's, each rounded as its type is."""
+    K, name = shape[-1], {torch.bfloat16: "bf16", torch.float32: "fp32"}
+    x, w = _rand(shape, tx, dev, 1), _rand((N, K), tw, dev, 2, 0.05)
+    y = fp4_linear(x, w, activations=activations)
+    dy = _rand(y.shape, tx, dev, 3, 0.01, grad=False)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.dtype == tx and dx.dtype == tx and dw.dtype == tw
+    x2, d2 = x.reshape(-1, K), dy.reshape(-1, N)
+    xv, wv = _value64(x2, 1, E4) if activations == E4 else _value4(x2, 1), _value4(w, 32)
+    dv, xt, dt = _value64(d2, 1, E5), _value64(x2.t(), 1, E4), _value64(d2.t(), 1, E5)
+    _near(y.reshape(-1, N), xv @ wv.t(), xv.abs() @ wv.abs().t(), K, name[tx] + " y")
+    _near(dx.reshape(-1, K), dv @ wv, dv.abs() @ wv.abs(), N, name[tx] + " dx")
+    _near(dw, dt @ xt.t(), dt.abs() @ xt.abs().t(), x2.shape[0], name[tw] + " dw")

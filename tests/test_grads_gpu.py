@@ -258,3 +258,31 @@ def test_tangents_and_transforms_are_refused(dev):
               lambda: torch.func.vmap(lambda x: grad_norm([x]))(a.view(5, 8))):
         with pytest.raises(RuntimeError, match="tangent|storage"):
             f()
+
+
+@pytest.mark.parametrize("scale", [1e30, 1e-30, 3e38, 1e-38])
+def test_clipped_values_of_far_gradients(dev, scale):
+    """Each clipped value against what it should be, whatever is left of it, in both types."""
+    for most in (1e-3 * scale, 0.5 * scale, 1e3):
+        grads = [torch.full((1000,), scale, device=dev), torch.full((77,), -scale, dtype=BF, device=dev)]
+        f = min(1.0, most / (_norm64(grads) + 1e-6))
+        want = [g.double() * f for g in grads]
+        clip_grad_norm(grads, most)
+        for g, w in zip(grads, want):
+            least = 2.0 ** -134 if g.dtype == BF else 2.0 ** -150
+            assert ((g.double() - w).abs() <= (HALF[g.dtype] + 2.0 ** -23) * w.abs() + least + 2.0 ** -150).all()
+
+
+def test_tensors_past_32_bits(dev):
+    """More than 2^31 elements and 2^32 bytes in one tensor, few of them not zero."""
+    n = 2 ** 31 + 54_321
+    big, small = torch.zeros(n, dtype=BF, device=dev), torch.full((100,), 2.0, device=dev)
+    at = torch.tensor([0, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 16_385, n - 1], device=dev)
+    big[at] = torch.arange(1.0, 7.0, device=dev).to(BF)
+    ref = math.sqrt(sum(i * i for i in range(1, 7)) + 400)
+    assert abs(grad_norm([big, small]).item() - ref) <= 2.0 ** -23 * ref
+    clip_grad_norm([big, small], 0.25 * ref)
+    f = 0.25 * ref / (ref + 1e-6)
+    want = torch.arange(1.0, 7.0, device=dev).double() * f
+    assert ((big[at].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -23) * want).all() and torch.count_nonzero(big).item() == 6
+    assert ((small.double() - 2 * f).abs() <= 2.0 ** -22).all()
