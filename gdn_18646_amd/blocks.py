@@ -202,7 +202,11 @@ def fp4_linear(x, weight, activations=E4M3):
     or fp32; fp32 ones get fp32 results.  In the backward pass the incoming gradient is
     quantised to e5m2 in blocks of 1 x 128 along each product's own sum, and multiplied
     with the 4-bit weight for the gradient of x and with x in e4m3 along its tokens for
-    the weight's.
+    the weight's.  bf16 results of 8-bit codes (dx is always one of those) leave out what
+    lies below 2^-17 of the largest of 128 products, a bf16 result's own rounding being
+    2^-8; fp32 ones have all of it.  4-bit weights halve what is read of them, which sets
+    the time of a few tokens by a large one; for many tokens 8-bit activations set the
+    speed, and ``fp8_linear`` takes as long.
     """
     if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"fp4_linear: x [..., {x.shape[-1] if x.dim() else ''}] and weight {tuple(weight.shape)}")

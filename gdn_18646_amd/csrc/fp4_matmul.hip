@@ -7,9 +7,9 @@
 // the waves' sums meet in LDS.  The workgroups of an XCD begin at different
 // places: 16 rows at a stride of a power of two lie in one or two of its L2's
 // channels, and in step they would all wait for the same ones.  A token by 8224 x 2048
-// takes 3.9 us with 4-bit codes and 4.4 with 8-bit ones, by 65536 x 2048 (71 MB) 14.3, 5.0
-// TB/s, and 18.0; the 16 x 16 tile of fp4_tiles.hpp, which takes three tokens and more, 4.4,
-// 4.3, 20.8 and 23.1, and fp32 results of 8-bit codes 5-30% longer than here.
+// takes 4.0 us with 4-bit codes and 4.3-4.5 with 8-bit ones, by 65536 x 2048 (71 MB) 13.4,
+// 5.3 TB/s, and 17.4; the 16 x 16 tile of fp4_tiles.hpp, which takes three tokens and more,
+// 4.4, 4.3 (level), 20.8 and 23.1, and fp32 results of 8-bit codes 5-30% longer than here.
 #include "fp4_matmul.hpp"
 
 namespace {
@@ -163,10 +163,14 @@ int launch(const gdn_fp4::MatmulParams& p, bool f32, hipStream_t stream) {
             hipLaunchKernelGGL((gdn_fp4_few_kernel<FA, decltype(out32)::value, W>), dim3((p.N + 15) / 16), dim3(64 * W), 0, stream, p, mask - 1);
             return gdn_host::check_launch("gdn_fp4_few_kernel");
         };
-        // The CUs hold 512 workgroups of eight waves or 1024 of four: between those
-        // numbers the smaller ones need one round, the others two (9216 x 4096, 8-bit codes,
-        // 8.7 us with four and 9.5 with eight); else eight read more at a time (8192 x 4096
-        // 8.2 and 7.2, 2048 x 8192 9.5 and 6.1, 65536 x 2048 18.9 and 18.0).
+        // The CUs hold 512 workgroups of eight waves or 1024 of four.  Eight read more at a
+        // time, which wins where they fit one round (a token in 8-bit codes by 8192 x 4096 7.3
+        // us with four and 6.4 with eight, by 2048 x 4096 5.5 and 3.9).  Past it they need a
+        // second one and four do not (8224 x 4096 7.7 and 8.2, 9216 8.1 and 8.8, 12288 8.8 and
+        // 9.3), until that one is full: level just below 1024 workgroups (16368 x 4096 10.5 and
+        // 10.4), eight ahead there (16384 10.5 and 10.3) and beyond, where four need more than
+        // one round too (16400 11.3 and 10.9, 24576 15.8 and 14.4, 65536 x 2048 17.9 and 17.4).
+        // 4-bit codes rank alike, closer together.
         const auto of_n = [&](auto out32) {
             return p.N > 8192 && p.N < 16384 ? few(out32, std::integral_constant<int, 4>{}) : few(out32, std::integral_constant<int, 8>{});
         };

@@ -23,12 +23,17 @@
 // What bounds it, by leaving parts out (256 x 256 tiles, us a slice): products and LDS reads
 // without copies 1.3 with codes of zero and 1.6 with random ones (the card's power; the
 // products alone 1.1), copies alone 1.1, all of it 1.7 and 2.2: the copies' writes and the
-// waves' reads meet in LDS.  And 6.7 us a tile on every CU, of which 256 x 128 KiB of bf16
-// results to HBM take 6.  16384 x 6144 x 2048 111 us (3.7 PFLOP/s), 8192 x 8192 x 8192
-// 282-303 (3.6-3.9).  Slower were two groups of waves in turn with barriers around each
-// quarter of a slice (124 us for the former), four waves of 128 x 128 (237: half the
-// accumulators move between register files), and lines fetched into the L2 two stages
-// ahead (126: the fetches take the copies' time).
+// waves' reads meet in LDS.  And 6.7 us a tile on every CU for its results: 256 x 128 KiB of
+// bf16 take 6 to HBM, but a later stage's wait also has all of a tile's stores, issued in
+// one piece, retire first; the two were not told apart (fp32 results take 15 to 18 more).
+// 16384 x 6144 x 2048 110-117 us (3.5-3.7 PFLOP/s; after a hundred calls: an idle card's
+// first ones take 120 to 150, until its power has settled), fp32 results 228; 8192 x 8192 x
+// 8192 250-303 (3.6-4.4) and 312.  Slower were, for the former in bf16 at 111, two groups of
+// waves in turn with barriers around each quarter of a slice (124), four waves of 128 x 128
+// (237: half the accumulators move between register files), and lines fetched into the L2
+// two stages ahead (126: the fetches take the copies' time); workgroups that start in 2 to 8
+// classes, 0.5 to 3.2 us apart, gained nothing (117-125 against 120, in the middle of a
+// run).
 //
 // Of 8-bit x the same loop runs 256 x 128 tiles; the whole of 256 x 256 does not fit its
 // stages (fp4_phased.hpp has another loop for them).

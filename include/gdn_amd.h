@@ -468,7 +468,8 @@ int gdn_fp8_matmul_hip(const uint8_t* a, int64_t lda, int format_a, const uint8_
  * one power-of-two scale a block of block_rows (1 or 32) x 32 values: 2^e with the
  * least e >= -127 for which the block's largest magnitude over 2^e is no larger than
  * 6 (e = 0 for zeros), kept as the byte e + 127 (e8m0); a code is value / 2^e to the
- * nearest, ties to even.  A block with an infinity or NaN gets scale NaN (0xff), codes
+ * nearest, ties to even.  (Encoders that take 2^(floor(log2 max) - 2) and cut off at 6 give
+ * other codes; they are decoded and multiplied alike.)  A block with an infinity or NaN gets scale NaN (0xff), codes
  * 0.  Along the rows: codes [M, ldc bytes], two a byte, the earlier one low, columns K
  * up to the next multiple of 256 zero; scales [K / 128, lds >= M, 4], blocks of 128
  * columns first (as many as the codes have), a row's four bytes adjacent.  Along the
@@ -510,7 +511,8 @@ int gdn_fp4_dequantize_hip(const uint8_t* codes, int64_t ldc, const uint8_t* sca
  *   gdn_fp8_quantize_hip write them).
  * Code rows are 16-byte aligned and at most 2^22 bytes apart.  Scales: 16-byte aligned
  * rows of K's blocks, ld % 4 == 0 (of 8-bit codes % 16), readable in whole.  M, N up to
- * 2^28.  With 8-bit codes, bf16 results leave 128 products to one instruction, which
+ * 2^28, M N / 256 up to 2^31 and as far as a launch of 2^32 threads reaches (else
+ * GDN_ERR_UNSUPPORTED).  With 8-bit codes, bf16 results leave 128 products to one instruction, which
  * drops what lies below 2^-17 of the largest; fp32 results sum every product in full.
  * With 4-bit ones, results of either type are sums of which each 128 products are added
  * with an error of at most 2^-21 of the largest among them, their sums of 32, the sum so
